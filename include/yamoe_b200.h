@@ -328,6 +328,50 @@ int yamoe_b200_experts_backward_saved(const void *grad_out, int grad_out_per_slo
                                       void *d_down_proj_bias, int64_t T, int H, int E, int K, int64_t expert_capacity,
                                       int dtype, void *saved, size_t saved_bytes, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * 8-bit operands (no counterpart in the reference): e4m3 codes with one fp32 scale per group of 128
+ * along the columns, over 1 row (activations, gradients) or 128 rows (weights); the last groups of a
+ * matrix are smaller.  A group's scale is a / 448 with a = max(max |x|, 2^-100), a code is
+ * e4m3(x * (448 / a)), every step in fp32 and to nearest even; a NaN, or an infinity, makes its group NaN.
+ *
+ * yamoe_fp8_matrix_t describes `batch` matrices of R rows and C columns (given by the call):
+ *   q       codes, row pitch `ld` and matrix pitch `q_batch` bytes; q 16-byte aligned, both pitches
+ *           multiples of 16, ld >= C.  Bytes between C and ld may be written.
+ *   scale   of (matrix b, row or row block r, column group g) at b * scale_batch + r * scale_row + g * scale_group
+ *           (in floats)
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+  void *q;
+  float *scale;
+  int64_t ld, q_batch, scale_row, scale_group, scale_batch;
+} yamoe_fp8_matrix_t;
+
+/* Quantises x, dtype [batch, M, K] contiguous, in groups of `block_rows` (1 or 128) x 128.
+ *   out         codes of x [M, K]: groups along K             } either may be NULL
+ *   transposed  codes of x^T [K, M]: groups along M           }
+ * With both and block_rows = 128 their codes agree. */
+int yamoe_b200_fp8_quantize(const void *x, const yamoe_fp8_matrix_t *out, const yamoe_fp8_matrix_t *transposed,
+                            int64_t batch, int64_t M, int64_t K, int block_rows, int dtype, void *stream);
+
+/* out[b] [M, N] = A[b] [M, K] @ B[b] [N, K]^T of quantised matrices, A with groups of 1 x 128, B with
+ * groups of b_block_rows (1 or 128) x 128.  Products are summed in fp32, exactly scaled block by block, and
+ * rounded once to out_dtype; rows of out are N elements apart, matrices M * N.  The workspace holds the status word. */
+size_t yamoe_b200_fp8_mm_workspace_bytes(int64_t batch, int64_t M, int64_t N, int64_t K);
+int yamoe_b200_fp8_mm(const yamoe_fp8_matrix_t *a, const yamoe_fp8_matrix_t *b, int b_block_rows, void *out,
+                      int64_t batch, int64_t M, int64_t N, int64_t K, int out_dtype, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
+/* Expert forward on quantised weights: yamoe_b200_experts_forward with
+ *   gate_up   E matrices [2H, H], down E matrices [H, H], groups of 128 x 128 (the transposed weights of that call)
+ * and the token rows and the activations of the GLU quantised in groups of 1 x 128.  Everything between is fp32 and
+ * the K rows of a token are summed in fp32; hidden_states, routing_weights, biases and out are of `dtype`. */
+size_t yamoe_b200_experts_fp8_workspace_bytes(int64_t T, int H, int E, int K, int dtype);
+int yamoe_b200_experts_fp8_forward(const void *hidden_states, const int64_t *router_indices,
+                                   const void *routing_weights, int routing_cols, const yamoe_fp8_matrix_t *gate_up,
+                                   const void *gate_up_bias, const yamoe_fp8_matrix_t *down, const void *down_bias,
+                                   void *out, int64_t T, int H, int E, int K, int64_t expert_capacity, int dtype,
+                                   void *workspace, size_t workspace_bytes, void *stream);
+
 /* Device status word of the last forward/backward call that used `workspace`: 0 when every
  * bounded device-side wait completed, otherwise a code naming the wait that gave up.  Reads
  * 4 bytes from the device with cudaMemcpyAsync on `stream` and synchronises that stream. */

@@ -28,7 +28,14 @@ class EpCtx(ctypes.Structure):
                 [("wait_ns", ctypes.c_uint64)])
 
 
+class Fp8Matrix(ctypes.Structure):
+    """yamoe_fp8_matrix_t of include/yamoe_b200.h."""
+    _fields_ = ([(n, c_void_p) for n in ("q", "scale")] +
+                [(n, c_int64) for n in ("ld", "q_batch", "scale_row", "scale_group", "scale_batch")])
+
+
 _ctx_p = ctypes.POINTER(EpCtx)
+_fp8_p = ctypes.POINTER(Fp8Matrix)
 PATH_AUTO, PATH_SIMT, PATH_TCGEN05, PATH_GEMV = 0, 1, 2, 3
 
 # name -> (restype, argtypes); mirrors include/yamoe_b200.h one to one
@@ -74,6 +81,13 @@ SIGNATURES = {
                                           [c_int64, c_int, c_int, c_int, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
     "yamoe_b200_experts_backward_saved": (c_int, [c_void_p, c_int, c_void_p, c_int] + [c_void_p] * 9 +
                                           [c_int64, c_int, c_int, c_int, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
+    "yamoe_b200_fp8_quantize": (c_int, [c_void_p, _fp8_p, _fp8_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "yamoe_b200_fp8_mm_workspace_bytes": (c_size_t, [c_int64] * 4),
+    "yamoe_b200_fp8_mm": (c_int, [_fp8_p, _fp8_p, c_int, c_void_p] + [c_int64] * 4 + [c_int, c_void_p, c_size_t, c_void_p]),
+    "yamoe_b200_experts_fp8_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int]),
+    "yamoe_b200_experts_fp8_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_int, _fp8_p, c_void_p, _fp8_p, c_void_p,
+                                               c_void_p, c_int64, c_int, c_int, c_int, c_int64, c_int, c_void_p, c_size_t,
+                                               c_void_p]),
     "yamoe_b200_mbar_wait_probe": (c_int, [c_void_p, ctypes.c_uint64, c_void_p]),
     "yamoe_b200_device_status": (c_int, [c_void_p, c_void_p, ctypes.POINTER(ctypes.c_int32)]),
 }
@@ -90,7 +104,10 @@ def lib() -> ctypes.CDLL:
                 "yamoe_b200 has no CPU or PyTorch fallback.")
         handle = ctypes.CDLL(LIB_PATH)
         for name, (res, args) in SIGNATURES.items():
-            fn = getattr(handle, name)
+            fn = getattr(handle, name, None)
+            if fn is None:
+                raise RuntimeError(f"{LIB_PATH} has no {name}: it is older than this package, build it again with "
+                                   "`python -m yamoe_b200.build`")
             fn.restype, fn.argtypes = res, args
         _lib = handle
     return _lib

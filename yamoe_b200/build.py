@@ -1,6 +1,6 @@
 """Build recipe, output in-tree: libyamoe_b200.so (one nvcc invocation for sm_100a: all kernels and
-the C ABI) and libyamoe_b200_torch.so (host compiler only: the C++ torch binding of `experts` and
-`experts_backward` over that C ABI).
+the C ABI) and libyamoe_b200_torch.so (host compiler only: the C++ torch binding of `experts`,
+`experts_backward`, the 8-bit operators and `moe_layer` over that C ABI).
 
     python -m yamoe_b200.build [--force] [--verbose]
 """
@@ -16,9 +16,9 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "libyamoe_b200.so")
 BINDING_PATH = os.path.join(PKG_DIR, "libyamoe_b200_torch.so")
 BINDING_SRC = os.path.join(CSRC, "torch_binding.cpp")
-SOURCES = ["yamoe_b200.cu"]
+SOURCES = ["yamoe_b200.cu", "fp8.cu"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
-              "-shared", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-ldl"]
+              "-shared", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-ldl", "--threads", "0"]
 
 
 def _nvcc() -> str:

@@ -1,0 +1,161 @@
+// 8-bit operands: quantisation, products, and the grouped products of the expert pass.  C entry points of the first two;
+// the expert pass is put together in yamoe_b200.cu.
+#include "fp8.h"
+
+#include "fp8_gemm.cuh"
+
+namespace yb {
+
+bool fp8_matrix_ok(const yamoe_fp8_matrix_t* m, int64_t batch, int64_t cols) {
+  if (m->q == nullptr || m->scale == nullptr) return false;
+  if ((reinterpret_cast<uintptr_t>(m->q) & 15) != 0 || (reinterpret_cast<uintptr_t>(m->scale) & 3) != 0) return false;
+  if (m->ld < cols || m->ld % 16 != 0 || m->ld >= (int64_t)1 << 40) return false;
+  return batch <= 1 || (m->q_batch > 0 && m->q_batch % 16 == 0 && m->q_batch < (int64_t)1 << 40);
+}
+
+static QuantOut quant_out(const yamoe_fp8_matrix_t* m) {
+  if (m == nullptr) return QuantOut{};
+  return QuantOut{reinterpret_cast<uint8_t*>(m->q), m->scale, m->ld, m->q_batch, m->scale_row, m->scale_group, m->scale_batch};
+}
+
+template <typename T>
+static int quantize_impl(const T* x, const yamoe_fp8_matrix_t* out, const yamoe_fp8_matrix_t* turned, int64_t B, int64_t M,
+                         int64_t K, int block_rows, cudaStream_t st) {
+  if (block_rows == 1 && turned == nullptr && (B == 1 || out->q_batch == M * out->ld)) {
+    const QuantRows d{reinterpret_cast<uint8_t*>(out->q), out->scale, out->ld, out->scale_row, out->scale_group, out->scale_batch,
+                      nullptr, 0};
+    return launch_quantize_rows<T>(x, d, B * M, M, (int)K, false, st);
+  }
+  return launch_quantize_tiles<T>(x, B, M, K, block_rows == 128, quant_out(out), quant_out(turned), st);
+}
+
+template <typename T>
+int fp8_gather(const T* hidden, uint8_t* q, float* scale, int64_t ld, int64_t scale_group, const int32_t* flat_row, int64_t tokens,
+               int H, int K, cudaStream_t st) {
+  const QuantRows d{q, scale, ld, 1, scale_group, 0, flat_row, K};
+  return launch_quantize_rows<T>(hidden, d, tokens, tokens, H, true, st);
+}
+template int fp8_gather<float>(const float*, uint8_t*, float*, int64_t, int64_t, const int32_t*, int64_t, int, int, cudaStream_t);
+template int fp8_gather<__nv_bfloat16>(const __nv_bfloat16*, uint8_t*, float*, int64_t, int64_t, const int32_t*, int64_t, int, int,
+                                       cudaStream_t);
+
+// Rows per expert from which the grouped products go by CTA pairs (tiles of 256 rows)
+static bool fp8_pairs(const Fp8Rows& r, int E) { return r.S > 128 * (int64_t)E; }
+
+static Fp8Params grouped_params(const Fp8Rows& r, const float* a_scale, const yamoe_fp8_matrix_t& w, int N, int K, int E, bool pairs) {
+  Fp8Params p{};
+  p.M = r.max_rows; p.N = N; p.K = K; p.B = E;
+  p.sa = a_scale; p.sa_m = 1; p.sa_k = r.max_rows;
+  p.sb = w.scale; p.sb_b = w.scale_batch; p.sb_n = w.scale_row; p.sb_k = w.scale_group;
+  p.tile_expert = pairs ? r.pair_expert : r.tile_expert;
+  p.tile_first = pairs ? r.pair_off : nullptr;
+  p.pad_off = r.pad_off;
+  p.n_tiles = r.header + (pairs ? kHdrPairs : kHdrRowTiles);
+  p.status = const_cast<int32_t*>(r.header) + kHdrStatus;
+  return p;
+}
+
+template <class Epi>
+static int grouped(const Fp8Rows& r, const uint8_t* a, const float* a_scale, int64_t ld, const yamoe_fp8_matrix_t& w, int N, int K,
+                   int E, const Epi& epi, cudaStream_t st) {
+  const bool pairs = fp8_pairs(r, E);
+  const Fp8Params p = grouped_params(r, a_scale, w, N, K, E, pairs);
+  const Fp8Operand A{a, r.max_rows, ld, 0}, B{w.q, N, w.ld, w.q_batch};
+  return pairs ? launch_fp8_gemm<2, 256, false, true>(A, B, p, epi, r.max_tiles, true, st)
+               : launch_fp8_gemm<1, 256, false, true>(A, B, p, epi, r.max_tiles, true, st);
+}
+
+template <typename T>
+int fp8_gate_up(const Fp8Rows& r, const uint8_t* x, const float* x_scale, int64_t ld, const yamoe_fp8_matrix_t& w, const T* bias,
+                uint8_t* act, float* act_scale, int H, int E, cudaStream_t st) {
+  return grouped(r, x, x_scale, ld, w, 2 * H, H, E, Fp8GluQuant<T>{bias, act, act_scale, ld, r.max_rows}, st);
+}
+template <typename T>
+int fp8_down(const Fp8Rows& r, const uint8_t* act, const float* act_scale, int64_t ld, const yamoe_fp8_matrix_t& w, const T* bias,
+             float* y, int H, int E, cudaStream_t st) {
+  return grouped(r, act, act_scale, ld, w, H, H, E, Fp8WeightedRows<T>{bias, y, r.row_token, r.row_flat, r.row_weight, H}, st);
+}
+#define YB_INSTANTIATE(T)                                                                                                  \
+  template int fp8_gate_up<T>(const Fp8Rows&, const uint8_t*, const float*, int64_t, const yamoe_fp8_matrix_t&, const T*,   \
+                              uint8_t*, float*, int, int, cudaStream_t);                                                    \
+  template int fp8_down<T>(const Fp8Rows&, const uint8_t*, const float*, int64_t, const yamoe_fp8_matrix_t&, const T*,      \
+                           float*, int, int, cudaStream_t);
+YB_INSTANTIATE(float)
+YB_INSTANTIATE(__nv_bfloat16)
+#undef YB_INSTANTIATE
+
+template <typename T, bool BROWS>
+static int mm_impl(const Fp8Operand& A, const Fp8Operand& B, Fp8Params p, T* out, cudaStream_t st) {
+  const int vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.N * (int64_t)sizeof(T) % 16 == 0;
+  const Fp8Store<T> epi{out, p.N, p.M * p.N, vec};
+  if (p.M > 128) {
+    p.MT = (int)ceil_div(p.M, 256);
+    return launch_fp8_gemm<2, 256, BROWS, false>(A, B, p, epi, (int64_t)p.B * p.MT, false, st);
+  }
+  p.MT = (int)ceil_div(p.M, 128);
+  return launch_fp8_gemm<1, 256, BROWS, false>(A, B, p, epi, (int64_t)p.B * p.MT, false, st);
+}
+
+}  // namespace yb
+
+using namespace yb;
+
+extern "C" {
+
+int yamoe_b200_fp8_quantize(const void* x, const yamoe_fp8_matrix_t* out, const yamoe_fp8_matrix_t* transposed, int64_t batch,
+                            int64_t M, int64_t K, int block_rows, int dtype, void* stream) {
+  if (dtype != YAMOE_F32 && dtype != YAMOE_BF16) return YAMOE_ERR_DTYPE;
+  if (batch < 0 || M < 0 || K < 0 || (block_rows != 1 && block_rows != 128)) return YAMOE_ERR_BAD_ARG;
+  if (out == nullptr && transposed == nullptr) return YAMOE_ERR_BAD_ARG;
+  if (batch == 0 || M == 0 || K == 0) return YAMOE_OK;
+  if (x == nullptr || (reinterpret_cast<uintptr_t>(x) & (dtype == YAMOE_F32 ? 3 : 1)) != 0) return YAMOE_ERR_BAD_ARG;
+  if ((out != nullptr && !fp8_matrix_ok(out, batch, K)) || (transposed != nullptr && !fp8_matrix_ok(transposed, batch, M)))
+    return YAMOE_ERR_BAD_ARG;
+  if (M >= (int64_t)1 << 31 || K >= (int64_t)1 << 31) return YAMOE_ERR_UNSUPPORTED;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == YAMOE_BF16
+             ? quantize_impl(reinterpret_cast<const __nv_bfloat16*>(x), out, transposed, batch, M, K, block_rows, st)
+             : quantize_impl(reinterpret_cast<const float*>(x), out, transposed, batch, M, K, block_rows, st);
+}
+
+size_t yamoe_b200_fp8_mm_workspace_bytes(int64_t batch, int64_t M, int64_t N, int64_t K) {
+  if (batch < 0 || M < 0 || N < 0 || K < 0) return 0;
+  return 256;
+}
+
+int yamoe_b200_fp8_mm(const yamoe_fp8_matrix_t* a, const yamoe_fp8_matrix_t* b, int b_block_rows, void* out, int64_t batch,
+                      int64_t M, int64_t N, int64_t K, int out_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (out_dtype != YAMOE_F32 && out_dtype != YAMOE_BF16) return YAMOE_ERR_DTYPE;
+  if (batch < 0 || M < 0 || N < 0 || K < 0 || (b_block_rows != 1 && b_block_rows != 128)) return YAMOE_ERR_BAD_ARG;
+  if (batch == 0 || M == 0 || N == 0) return YAMOE_OK;
+  const size_t size = out_dtype == YAMOE_F32 ? 4 : 2;
+  if (out == nullptr || (reinterpret_cast<uintptr_t>(out) & (size - 1)) != 0) return YAMOE_ERR_BAD_ARG;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (K == 0) {
+    YB_CUDA_OK(cudaMemsetAsync(out, 0, (size_t)batch * M * N * size, st));
+    return YAMOE_OK;
+  }
+  if (a == nullptr || b == nullptr || !fp8_matrix_ok(a, batch, K) || !fp8_matrix_ok(b, batch, K)) return YAMOE_ERR_BAD_ARG;
+  // coordinates and tile counts are 32-bit numbers
+  if (M >= (int64_t)1 << 30 || N >= (int64_t)1 << 30 || K >= (int64_t)1 << 30 || batch >= (int64_t)1 << 30)
+    return YAMOE_ERR_UNSUPPORTED;
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
+      workspace_bytes < yamoe_b200_fp8_mm_workspace_bytes(batch, M, N, K))
+    return YAMOE_ERR_WORKSPACE;
+  Fp8Params p{};
+  p.M = M; p.N = N; p.K = (int)K; p.B = (int)batch;
+  p.sa = a->scale; p.sa_b = a->scale_batch; p.sa_m = a->scale_row; p.sa_k = a->scale_group;
+  p.sb = b->scale; p.sb_b = b->scale_batch; p.sb_n = b->scale_row; p.sb_k = b->scale_group;
+  p.status = reinterpret_cast<int32_t*>(workspace) + kHdrStatus;
+  p.clear_status = 1;
+  const Fp8Operand A{a->q, M, a->ld, a->q_batch}, B{b->q, N, b->ld, b->q_batch};
+  const bool rows = b_block_rows == 1;
+  if (out_dtype == YAMOE_BF16) {
+    auto o = reinterpret_cast<__nv_bfloat16*>(out);
+    return rows ? mm_impl<__nv_bfloat16, true>(A, B, p, o, st) : mm_impl<__nv_bfloat16, false>(A, B, p, o, st);
+  }
+  auto o = reinterpret_cast<float*>(out);
+  return rows ? mm_impl<float, true>(A, B, p, o, st) : mm_impl<float, false>(A, B, p, o, st);
+}
+
+}  // extern "C"

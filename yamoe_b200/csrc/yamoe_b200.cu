@@ -21,6 +21,7 @@
 #include "gemv.cuh"
 #include "ep_fused.cuh"
 #include "router.cuh"
+#include "fp8.h"
 
 namespace yb {
 
@@ -321,6 +322,67 @@ static int forward_impl(const void* hidden, const int64_t* ridx, const void* rw,
         p.acc32, reinterpret_cast<T*>(out), nv);
   }
   return cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Expert forward on 8-bit operands: routing tables as above, codes and scales of the gathered token rows, of the
+// activations, and fp32 result rows at their flat positions.
+// ---------------------------------------------------------------------------------------------
+struct Fp8Plan {
+  Plan t;                        // tables
+  int64_t ld = 0;                // pitch of the codes
+  uint8_t *x = nullptr, *act = nullptr;
+  float *x_scale = nullptr, *act_scale = nullptr;   // [groups, max_rows]
+  float* y = nullptr;            // bf16: [S, H], fp32: [max_rows, H] (see Fp8WeightedRows)
+  size_t bytes = 0;
+};
+
+static Fp8Plan plan_experts_fp8(void* ws, int64_t T, int H, int E, int K, int dtype) {
+  Fp8Plan p;
+  Bump b(ws);
+  carve_tables(b, p.t, T, E, K, true);
+  p.ld = round_up(H, 16);
+  const size_t groups = (size_t)ceil_div(H, 128);
+  p.x = b.take<uint8_t>((size_t)p.t.max_rows * p.ld);
+  p.act = b.take<uint8_t>((size_t)p.t.max_rows * p.ld);
+  p.x_scale = b.take<float>(groups * p.t.max_rows);
+  p.act_scale = b.take<float>(groups * p.t.max_rows);
+  p.y = b.take<float>((size_t)(dtype == YAMOE_F32 ? p.t.max_rows : p.t.S) * H);
+  p.bytes = b.off + 256;
+  return p;
+}
+
+template <typename T>
+static int experts_fp8_impl(const void* hidden, const int64_t* ridx, const void* rw, int rcols, const yamoe_fp8_matrix_t& gate_up,
+                            const void* bgu, const yamoe_fp8_matrix_t& down, const void* bd, void* out, int64_t Tn, int H, int E,
+                            int K, int64_t cap, void* ws, cudaStream_t st) {
+  const Fp8Plan p = plan_experts_fp8(ws, Tn, H, E, K, sizeof(T) == 4 ? YAMOE_F32 : YAMOE_BF16);
+  const RouteTables& rt = p.t.rt;
+  int rc;
+  {
+    StageTimer tm(kStageRoute, st);
+    rc = launch_route_rows<T>(ridx, reinterpret_cast<const T*>(rw), rcols, Tn, E, K, cap, rt, p.t.row_tables_bytes, st);
+  }
+  if (rc) return rc;
+  {
+    StageTimer tm(kStageGather, st);
+    rc = fp8_gather<T>(reinterpret_cast<const T*>(hidden), p.x, p.x_scale, p.ld, p.t.max_rows, rt.flat_row, Tn, H, K, st);
+  }
+  if (rc) return rc;
+  const Fp8Rows rows{rt.pad_off, rt.pair_expert, rt.pair_off, rt.tile_expert, rt.header, rt.row_token, rt.row_flat, rt.row_weight,
+                     p.t.max_rows, p.t.max_tiles, p.t.S};
+  {
+    StageTimer tm(kStageGateUp, st);
+    rc = fp8_gate_up<T>(rows, p.x, p.x_scale, p.ld, gate_up, reinterpret_cast<const T*>(bgu), p.act, p.act_scale, H, E, st);
+  }
+  if (rc) return rc;
+  {
+    StageTimer tm(kStageDown, st);
+    rc = fp8_down<T>(rows, p.act, p.act_scale, p.ld, down, reinterpret_cast<const T*>(bd), p.y, H, E, st);
+  }
+  if (rc) return rc;
+  StageTimer tm(kStageCombine, st);
+  return launch_combine(p.y, rt.flat_row, reinterpret_cast<T*>(out), Tn, H, K, st);
 }
 
 // Forward pass that leaves what the backward pass needs in a workspace with the BACKWARD layout:
@@ -1117,6 +1179,36 @@ int yamoe_b200_experts_forward(const void* hidden_states, const int64_t* router_
   return forward_impl<float>(hidden_states, router_indices, routing_weights, routing_cols, gate_up_proj,
                              gate_up_proj_bias, down_proj, down_proj_bias, out, T, H, E, K, expert_capacity,
                              dtype, workspace, st);
+}
+
+size_t yamoe_b200_experts_fp8_workspace_bytes(int64_t T, int H, int E, int K, int dtype) {
+  if (check_common(T, H, E, K, dtype)) return 0;
+  return plan_experts_fp8(nullptr, T, H, E, K, dtype).bytes;
+}
+
+int yamoe_b200_experts_fp8_forward(const void* hidden_states, const int64_t* router_indices, const void* routing_weights,
+                                   int routing_cols, const yamoe_fp8_matrix_t* gate_up, const void* gate_up_bias,
+                                   const yamoe_fp8_matrix_t* down, const void* down_bias, void* out, int64_t T, int H, int E,
+                                   int K, int64_t expert_capacity, int dtype, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  int rc = check_common(T, H, E, K, dtype);
+  if (rc) return rc;
+  if (routing_cols != E && routing_cols != K) return YAMOE_ERR_BAD_ARG;
+  if (expert_capacity < 0) return YAMOE_ERR_BAD_ARG;
+  if (T > 0 && (!hidden_states || !router_indices || !routing_weights || !out)) return YAMOE_ERR_BAD_ARG;
+  if (!gate_up || !gate_up_bias || !down || !down_bias) return YAMOE_ERR_BAD_ARG;
+  if (!fp8_matrix_ok(gate_up, E, H) || !fp8_matrix_ok(down, E, H)) return YAMOE_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(hidden_states) | reinterpret_cast<uintptr_t>(out)) & 15) return YAMOE_ERR_BAD_ARG;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
+      workspace_bytes < yamoe_b200_experts_fp8_workspace_bytes(T, H, E, K, dtype))
+    return YAMOE_ERR_WORKSPACE;
+  if (T == 0) return YAMOE_OK;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == YAMOE_BF16
+             ? experts_fp8_impl<__nv_bfloat16>(hidden_states, router_indices, routing_weights, routing_cols, *gate_up, gate_up_bias,
+                                               *down, down_bias, out, T, H, E, K, expert_capacity, workspace, st)
+             : experts_fp8_impl<float>(hidden_states, router_indices, routing_weights, routing_cols, *gate_up, gate_up_bias, *down,
+                                       down_bias, out, T, H, E, K, expert_capacity, workspace, st);
 }
 
 size_t yamoe_b200_backward_workspace_bytes(int64_t T, int H, int E, int K, int dtype) {

@@ -28,7 +28,10 @@ def _load_cpp_binding() -> bool:
     from .build import BINDING_PATH
     if not os.path.exists(BINDING_PATH):
         return False
-    _lib.lib()                       # the CUDA library must be loaded first (and must exist)
+    try:
+        _lib.lib()                   # the CUDA library must be loaded first
+    except RuntimeError:
+        return False                 # missing or out of date: the first call says so, and `build` can still be imported
     torch.ops.load_library(BINDING_PATH)
     return True
 
@@ -442,3 +445,28 @@ gather = torch.ops.yamoe_b200.gather
 scatter = torch.ops.yamoe_b200.scatter
 index_select_out = torch.ops.yamoe_b200.index_select_out
 bincount_cumsum = torch.ops.yamoe_b200.bincount_cumsum
+
+
+def _needs_cpp_binding(name):
+    def missing(*_args, **_kwargs):
+        raise RuntimeError(f"yamoe_b200: {name} needs the C++ binding libyamoe_b200_torch.so (python -m yamoe_b200.build) "
+                           "and neither YAMOE_B200_PY_BINDING nor YAMOE_B200_LIB set")
+    missing.__name__ = name
+    return missing
+
+
+def _cpp_operator(name):
+    return getattr(torch.ops.yamoe_b200, name) if CPP_BINDING else _needs_cpp_binding(name)
+
+
+quantize_fp8 = _cpp_operator("quantize_fp8")
+fp8_mm = _cpp_operator("fp8_mm")
+fp8_linear = _cpp_operator("fp8_linear")
+experts_fp8 = _cpp_operator("experts_fp8")
+
+
+def quantize_experts(gate_up_proj, down_proj):
+    """Expert weights as `experts_fp8` and `moe_layer` take them: (gate_up, gate_up_scale, down, down_scale) from
+    gate_up_proj [E, H, 2H] and down_proj [E, H, H].  Codes are those of the transposed matrices, [E, 2H, H] and [E, H, H],
+    with one scale per 128 x 128 block."""
+    return (*quantize_fp8(gate_up_proj, 128, True), *quantize_fp8(down_proj, 128, True))
