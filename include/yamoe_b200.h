@@ -372,6 +372,22 @@ int yamoe_b200_experts_fp8_forward(const void *hidden_states, const int64_t *rou
                                    void *out, int64_t T, int H, int E, int K, int64_t expert_capacity, int dtype,
                                    void *workspace, size_t workspace_bytes, void *stream);
 
+/* The layer around the expert op for a few tokens, in two launches: router, top-k, softmax, scores and experts.
+ *   logits = hidden_states [T,H] @ router_weight [E,H]^T + router_bias [E] (may be NULL), in fp32 and not rounded;
+ *   the K largest of a token (equal ones: lower id first; NaN above all) and the softmax over them are its experts and
+ *   their weights, of which router_scores [T,E] is the dense matrix; out = the expert forward with expert_capacity.
+ * bf16 tensors; the weights are either bf16 (gate_up [E,H,2H], down [E,H,H]; gate_up_fp8 and down_fp8 NULL) or quantised as
+ * yamoe_b200_experts_fp8_forward takes them (gate_up and down NULL); activations are not quantised.  Sums and weights are
+ * fp32, nothing depends on the order in which CTAs finish.
+ * T <= 32, T*K <= 256, K <= 32, K <= E <= 1024, H a multiple of 8 up to 65536: otherwise YAMOE_ERR_UNSUPPORTED, and 0
+ * workspace bytes.  The second launch is cooperative: its CTAs, one per SM, wait for one another. */
+size_t yamoe_b200_moe_layer_workspace_bytes(int64_t T, int H, int E, int K);
+int yamoe_b200_moe_layer(const void *hidden_states, const void *router_weight, const void *router_bias,
+                         const void *gate_up, const yamoe_fp8_matrix_t *gate_up_fp8, const void *gate_up_bias,
+                         const void *down, const yamoe_fp8_matrix_t *down_fp8, const void *down_bias, void *out,
+                         void *router_scores, int64_t T, int H, int E, int K, int64_t expert_capacity, int dtype,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
 /* Device status word of the last forward/backward call that used `workspace`: 0 when every
  * bounded device-side wait completed, otherwise a code naming the wait that gave up.  Reads
  * 4 bytes from the device with cudaMemcpyAsync on `stream` and synchronises that stream. */

@@ -88,6 +88,9 @@ SIGNATURES = {
     "yamoe_b200_experts_fp8_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_int, _fp8_p, c_void_p, _fp8_p, c_void_p,
                                                c_void_p, c_int64, c_int, c_int, c_int, c_int64, c_int, c_void_p, c_size_t,
                                                c_void_p]),
+    "yamoe_b200_moe_layer_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
+    "yamoe_b200_moe_layer": (c_int, [c_void_p] * 4 + [_fp8_p, c_void_p, c_void_p, _fp8_p, c_void_p, c_void_p, c_void_p] +
+                             [c_int64, c_int, c_int, c_int, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
     "yamoe_b200_mbar_wait_probe": (c_int, [c_void_p, ctypes.c_uint64, c_void_p]),
     "yamoe_b200_device_status": (c_int, [c_void_p, c_void_p, ctypes.POINTER(ctypes.c_int32)]),
 }

@@ -1,8 +1,9 @@
-// 8-bit operands: quantisation, products, and the grouped products of the expert pass.  C entry points of the first two;
-// the expert pass is put together in yamoe_b200.cu.
+// 8-bit operands: quantisation, products, and the grouped products of the expert pass; the layer for a few tokens.
+// C entry points but that of the expert pass, which is put together in yamoe_b200.cu.
 #include "fp8.h"
 
 #include "fp8_gemm.cuh"
+#include "moe_layer.cuh"
 
 namespace yb {
 
@@ -156,6 +157,65 @@ int yamoe_b200_fp8_mm(const yamoe_fp8_matrix_t* a, const yamoe_fp8_matrix_t* b, 
   }
   auto o = reinterpret_cast<float*>(out);
   return rows ? mm_impl<float, true>(A, B, p, o, st) : mm_impl<float, false>(A, B, p, o, st);
+}
+
+size_t yamoe_b200_moe_layer_workspace_bytes(int64_t T, int H, int E, int K) {
+  if (!layer_shape_ok(T, H, E, K)) return 0;
+  LayerArgs a{};
+  a.T = (int)T; a.H = H; a.E = E; a.K = K;
+  return layer_workspace(a, nullptr);
+}
+
+int yamoe_b200_moe_layer(const void* hidden_states, const void* router_weight, const void* router_bias, const void* gate_up,
+                         const yamoe_fp8_matrix_t* gate_up_fp8, const void* gate_up_bias, const void* down,
+                         const yamoe_fp8_matrix_t* down_fp8, const void* down_bias, void* out, void* router_scores, int64_t T, int H,
+                         int E, int K, int64_t expert_capacity, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype != YAMOE_BF16) return YAMOE_ERR_DTYPE;
+  if (T < 0 || H <= 0 || E <= 0 || K <= 0 || H % 8 != 0 || K > E || expert_capacity < 0) return YAMOE_ERR_BAD_ARG;
+  if (!layer_shape_ok(T, H, E, K)) return YAMOE_ERR_UNSUPPORTED;
+  const bool fp8 = gate_up_fp8 != nullptr;
+  if (fp8 ? down_fp8 == nullptr : (gate_up == nullptr || down == nullptr || down_fp8 != nullptr)) return YAMOE_ERR_BAD_ARG;
+  if (T > 0 && (!hidden_states || !out || !router_scores)) return YAMOE_ERR_BAD_ARG;
+  if (!router_weight || !gate_up_bias || !down_bias) return YAMOE_ERR_BAD_ARG;
+  const void* wide[] = {hidden_states, router_weight, gate_up, down, out};
+  for (const void* q : wide)
+    if (reinterpret_cast<uintptr_t>(q) & 15) return YAMOE_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(gate_up_bias) | reinterpret_cast<uintptr_t>(down_bias)) & 3) return YAMOE_ERR_BAD_ARG;
+  if (fp8 && (!fp8_matrix_ok(gate_up_fp8, E, H) || !fp8_matrix_ok(down_fp8, E, H))) return YAMOE_ERR_BAD_ARG;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
+      workspace_bytes < yamoe_b200_moe_layer_workspace_bytes(T, H, E, K))
+    return YAMOE_ERR_WORKSPACE;
+  if (T == 0) return YAMOE_OK;
+  if (!umma_available()) return YAMOE_ERR_UNSUPPORTED;
+  using bf = __nv_bfloat16;
+  LayerArgs a{};
+  a.T = (int)T; a.H = H; a.E = E; a.K = K; a.capacity = expert_capacity;
+  layer_workspace(a, reinterpret_cast<char*>(workspace));
+  a.x = reinterpret_cast<const bf*>(hidden_states);
+  a.router = reinterpret_cast<const bf*>(router_weight);
+  a.router_bias = reinterpret_cast<const bf*>(router_bias);
+  a.bias_gu = reinterpret_cast<const bf*>(gate_up_bias);
+  a.bias_dn = reinterpret_cast<const bf*>(down_bias);
+  a.out = reinterpret_cast<bf*>(out);
+  a.scores = reinterpret_cast<bf*>(router_scores);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  CUtensorMap gu, dn;
+  const uint64_t h = (uint64_t)H, n = (uint64_t)E;
+  if (fp8) {
+    const yamoe_fp8_matrix_t &g = *gate_up_fp8, &d = *down_fp8;
+    a.scale_gu = g.scale; a.gu_b = g.scale_batch; a.gu_r = g.scale_row; a.gu_g = g.scale_group;
+    a.scale_dn = d.scale; a.dn_b = d.scale_batch; a.dn_r = d.scale_row; a.dn_g = d.scale_group;
+    const uint64_t dg[3] = {h, 2 * h, n}, dd[3] = {h, h, n};
+    const uint64_t sg[2] = {(uint64_t)g.ld, (uint64_t)(E > 1 ? g.q_batch : g.ld)}, sd[2] = {(uint64_t)d.ld, (uint64_t)(E > 1 ? d.q_batch : d.ld)};
+    const uint32_t box[3] = {128, kLayerUnit, 1};
+    if (!encode_map(&gu, g.q, 3, dg, sg, box, kMapU8) || !encode_map(&dn, d.q, 3, dd, sd, box, kMapU8)) return YAMOE_ERR_CUDA;
+    return launch_moe_layer<true>(a, gu, dn, st);
+  }
+  const uint64_t dg[3] = {2 * h, h, n}, dd[3] = {h, h, n};
+  const uint64_t sg[2] = {4 * h, 4 * h * h}, sd[2] = {2 * h, 2 * h * h};
+  const uint32_t box[3] = {kLayerUnit, 64, 1};
+  if (!encode_map(&gu, gate_up, 3, dg, sg, box, kMapBf16) || !encode_map(&dn, down, 3, dd, sd, box, kMapBf16)) return YAMOE_ERR_CUDA;
+  return launch_moe_layer<false>(a, gu, dn, st);
 }
 
 }  // extern "C"

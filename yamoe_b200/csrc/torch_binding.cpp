@@ -15,6 +15,7 @@
 #include <torch/library.h>
 
 #include <cstdlib>
+#include <optional>
 #include <tuple>
 #include <vector>
 
@@ -385,6 +386,78 @@ at::Tensor experts_fp8_cuda(const at::Tensor& hidden_states, const at::Tensor& r
   return out;
 }
 
+// contiguous, on the 16-byte boundary that the kernels' wide loads and copies want
+at::Tensor aligned(const at::Tensor& t) {
+  const at::Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+std::tuple<at::Tensor, at::Tensor> moe_layer_cuda(const at::Tensor& hidden_states, const at::Tensor& router_weight,
+                                                  const std::optional<at::Tensor>& router_bias, const at::Tensor& gate_up,
+                                                  const at::Tensor& gate_up_bias, const at::Tensor& down,
+                                                  const at::Tensor& down_bias, int64_t expert_capacity, int64_t num_experts,
+                                                  int64_t top_k, const std::optional<at::Tensor>& gate_up_scale,
+                                                  const std::optional<at::Tensor>& down_scale) {
+  const int64_t T = hidden_states.size(0), H = hidden_states.size(-1), E = num_experts, K = top_k;
+  TORCH_CHECK(hidden_states.dim() == 2, "moe_layer: hidden_states must be 2D [T, H]");
+  TORCH_CHECK(hidden_states.scalar_type() == at::kBFloat16, "moe_layer: bfloat16 expected, got ", hidden_states.scalar_type());
+  TORCH_CHECK(T <= 32 && T * K <= 256, "moe_layer: at most 32 tokens and 256 assignments, got ", T, " tokens of ", K,
+              " (use router_forward and experts, or experts_fp8, for more)");
+  const bool has_bias = router_bias.has_value() && router_bias->defined();
+  const at::Tensor rb = has_bias ? *router_bias : at::Tensor();
+  const at::Tensor* tensors[] = {&router_weight, &gate_up_bias, &down_bias, &rb};
+  const char* names[] = {"router_weight", "gate_up_bias", "down_bias", "router_bias"};
+  for (int i = 0; i < (has_bias ? 4 : 3); ++i)
+    TORCH_CHECK(tensors[i]->device() == hidden_states.device() && tensors[i]->scalar_type() == at::kBFloat16, "moe_layer: ",
+                names[i], " must be bfloat16 on the device of hidden_states");
+  TORCH_CHECK(router_weight.dim() == 2 && router_weight.size(0) == E && router_weight.size(1) == H,
+              "moe_layer: router_weight must be [E, H]");
+  TORCH_CHECK(!has_bias || rb.numel() == E, "moe_layer: router_bias must be [E]");
+  TORCH_CHECK(gate_up_bias.dim() == 2 && gate_up_bias.size(0) == E && gate_up_bias.size(1) == 2 * H,
+              "moe_layer: gate_up_bias must be [E, 2*H]");
+  TORCH_CHECK(down_bias.dim() == 2 && down_bias.size(0) == E && down_bias.size(1) == H, "moe_layer: down_bias must be [E, H]");
+  TORCH_CHECK(K >= 1 && K <= E, "moe_layer: top_k must be between 1 and the number of experts");
+  TORCH_CHECK(gate_up.device() == hidden_states.device() && down.device() == hidden_states.device(),
+              "moe_layer: weights must be on the device of hidden_states");
+  const bool fp8 = gate_up.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK(gate_up_scale.has_value() == fp8 && down_scale.has_value() == fp8,
+              "moe_layer: scales belong to float8_e4m3fn weights, and to both of them");
+  const c10::cuda::CUDAGuard guard(hidden_states.device());
+  Quantised g, d;
+  at::Tensor gu = gate_up, dn = down;
+  yamoe_fp8_matrix_t mg{}, md{};
+  if (fp8) {
+    TORCH_CHECK(gate_up.dim() == 3 && gate_up.size(0) == E && gate_up.size(1) == 2 * H && gate_up.size(2) == H,
+                "moe_layer: float8_e4m3fn gate_up must be [E, 2*H, H]");
+    TORCH_CHECK(down.dim() == 3 && down.size(0) == E && down.size(1) == H && down.size(2) == H, "moe_layer: down must be [E, H, H]");
+    g = operand("moe_layer", "gate_up", gate_up, *gate_up_scale, 3, true);
+    d = operand("moe_layer", "down", down, *down_scale, 3, true);
+    mg = matrix_of(g);
+    md = matrix_of(d);
+  } else {
+    TORCH_CHECK(gate_up.scalar_type() == at::kBFloat16 && down.scalar_type() == at::kBFloat16,
+                "moe_layer: weights must be bfloat16 or float8_e4m3fn");
+    TORCH_CHECK(gate_up.dim() == 3 && gate_up.size(0) == E && gate_up.size(1) == H && gate_up.size(2) == 2 * H,
+                "moe_layer: gate_up must be [E, H, 2*H]");
+    TORCH_CHECK(down.dim() == 3 && down.size(0) == E && down.size(1) == H && down.size(2) == H, "moe_layer: down must be [E, H, H]");
+    gu = aligned(gate_up);
+    dn = aligned(down);
+  }
+  const at::Tensor hs = aligned(hidden_states), rw = aligned(router_weight), bg = aligned(gate_up_bias), bd = aligned(down_bias),
+                   br = has_bias ? rb.contiguous() : rb;
+  at::Tensor out = at::empty({T, H}, hs.options()), scores = at::empty({T, E}, hs.options());
+  const size_t nbytes = yamoe_b200_moe_layer_workspace_bytes(T, (int)H, (int)E, (int)K);
+  TORCH_CHECK(nbytes > 0, "yamoe_b200: unsupported shape (H must be a positive multiple of 8, E <= 1024, top_k <= 32)");
+  const at::Tensor ws = workspace(nbytes, hs);
+  check(yamoe_b200_moe_layer(hs.data_ptr(), rw.data_ptr(), has_bias ? br.data_ptr() : nullptr, fp8 ? nullptr : gu.data_ptr(),
+                             fp8 ? &mg : nullptr, bg.data_ptr(), fp8 ? nullptr : dn.data_ptr(), fp8 ? &md : nullptr, bd.data_ptr(),
+                             out.data_ptr(), scores.data_ptr(), T, (int)H, (int)E, (int)K, expert_capacity, YAMOE_BF16, ws.data_ptr(),
+                             (size_t)ws.numel(), current_stream()),
+        "moe_layer");
+  if (T > 0) check_device_status(ws, current_stream(), "moe_layer");
+  return {out, scores};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(yamoe_b200, m) {
@@ -403,6 +476,10 @@ TORCH_LIBRARY_FRAGMENT(yamoe_b200, m) {
       "experts_fp8(Tensor hidden_states, Tensor router_indices, Tensor routing_weights, Tensor gate_up, Tensor gate_up_scale, "
       "Tensor gate_up_bias, Tensor down, Tensor down_scale, Tensor down_bias, int expert_capacity, int num_experts, int top_k) "
       "-> Tensor");
+  m.def(
+      "moe_layer(Tensor hidden_states, Tensor router_weight, Tensor? router_bias, Tensor gate_up, Tensor gate_up_bias, Tensor down, "
+      "Tensor down_bias, int expert_capacity, int num_experts, int top_k, Tensor? gate_up_scale=None, Tensor? down_scale=None) -> "
+      "(Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(yamoe_b200, AutogradCUDA, m) {
@@ -416,4 +493,5 @@ TORCH_LIBRARY_IMPL(yamoe_b200, CUDA, m) {
   m.impl("fp8_mm", &fp8_mm_cuda);
   m.impl("fp8_linear", &fp8_linear_cuda);
   m.impl("experts_fp8", &experts_fp8_cuda);
+  m.impl("moe_layer", &moe_layer_cuda);
 }

@@ -463,6 +463,7 @@ quantize_fp8 = _cpp_operator("quantize_fp8")
 fp8_mm = _cpp_operator("fp8_mm")
 fp8_linear = _cpp_operator("fp8_linear")
 experts_fp8 = _cpp_operator("experts_fp8")
+moe_layer = _cpp_operator("moe_layer")
 
 
 def quantize_experts(gate_up_proj, down_proj):
