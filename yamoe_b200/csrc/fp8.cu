@@ -213,7 +213,7 @@ int yamoe_b200_moe_layer(const void* hidden_states, const void* router_weight, c
   }
   const uint64_t dg[3] = {2 * h, h, n}, dd[3] = {h, h, n};
   const uint64_t sg[2] = {4 * h, 4 * h * h}, sd[2] = {2 * h, 2 * h * h};
-  const uint32_t box[3] = {kLayerUnit, 64, 1};
+  const uint32_t box[3] = {64, 64, 1};
   if (!encode_map(&gu, gate_up, 3, dg, sg, box, kMapBf16) || !encode_map(&dn, down, 3, dd, sd, box, kMapBf16)) return YAMOE_ERR_CUDA;
   return launch_moe_layer<false>(a, gu, dn, st);
 }
