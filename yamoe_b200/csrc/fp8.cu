@@ -22,10 +22,10 @@ static QuantOut quant_out(const yamoe_fp8_matrix_t* m) {
 template <typename T>
 static int quantize_impl(const T* x, const yamoe_fp8_matrix_t* out, const yamoe_fp8_matrix_t* turned, int64_t B, int64_t M,
                          int64_t K, int block_rows, cudaStream_t st) {
-  if (block_rows == 1 && turned == nullptr && (B == 1 || out->q_batch == M * out->ld)) {
-    const QuantRows d{reinterpret_cast<uint8_t*>(out->q), out->scale, out->ld, out->scale_row, out->scale_group, out->scale_batch,
-                      nullptr, 0};
-    return launch_quantize_rows<T>(x, d, B * M, M, (int)K, false, st);
+  if (block_rows == 1 && turned == nullptr) {
+    const QuantRows d{reinterpret_cast<uint8_t*>(out->q), out->scale, out->ld, out->q_batch, out->scale_row, out->scale_group,
+                      out->scale_batch, nullptr, 0};
+    return launch_quantize_rows<T>(x, d, B, M, (int)K, false, st);
   }
   return launch_quantize_tiles<T>(x, B, M, K, block_rows == 128, quant_out(out), quant_out(turned), st);
 }
@@ -33,8 +33,8 @@ static int quantize_impl(const T* x, const yamoe_fp8_matrix_t* out, const yamoe_
 template <typename T>
 int fp8_gather(const T* hidden, uint8_t* q, float* scale, int64_t ld, int64_t scale_group, const int32_t* flat_row, int64_t tokens,
                int H, int K, cudaStream_t st) {
-  const QuantRows d{q, scale, ld, 1, scale_group, 0, flat_row, K};
-  return launch_quantize_rows<T>(hidden, d, tokens, tokens, H, true, st);
+  const QuantRows d{q, scale, ld, 0, 1, scale_group, 0, flat_row, K};
+  return launch_quantize_rows<T>(hidden, d, 1, tokens, H, true, st);
 }
 template int fp8_gather<float>(const float*, uint8_t*, float*, int64_t, int64_t, const int32_t*, int64_t, int, int, cudaStream_t);
 template int fp8_gather<__nv_bfloat16>(const __nv_bfloat16*, uint8_t*, float*, int64_t, int64_t, const int32_t*, int64_t, int, int,

@@ -34,82 +34,118 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   return e4m3x2(a, b) | (e4m3x2(c, d) << 16);
 }
 
-// Eight neighbouring values of a row, of which `n` exist (the others 0); VEC: 16-byte loads, rows being aligned to them.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int n, float (&v)[8]) {
-  if (VEC && n >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(p));
-      const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[2 * j] = __uint_as_float(u[j] << 16);
-        v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
-      }
+// Eight neighbouring values of a row as loaded, of which `n` exist (the others 0); VEC: 16-byte loads, rows being aligned to them.
+template <typename T> struct Eight;
+template <> struct Eight<__nv_bfloat16> {
+  uint4 q;
+  template <bool VEC>
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, int n) {
+    if (VEC && n >= 8) {
+      q = __ldg(reinterpret_cast<const uint4*>(p));
     } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+      uint32_t w[4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float4 q = __ldg(reinterpret_cast<const float4*>(p) + j);
-        v[4 * j] = q.x; v[4 * j + 1] = q.y; v[4 * j + 2] = q.z; v[4 * j + 3] = q.w;
-      }
+      for (int j = 0; j < 4; ++j)
+        w[j] = (2 * j < n ? (uint32_t)__ldg(h + 2 * j) : 0u) | (2 * j + 1 < n ? (uint32_t)__ldg(h + 2 * j + 1) << 16 : 0u);
+      q = make_uint4(w[0], w[1], w[2], w[3]);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? DT<T>::ld(p + j) : 0.f;
   }
+  __device__ __forceinline__ uint32_t word(int j) const { return j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w; }
+  __device__ __forceinline__ float value(int j) const {
+    const uint32_t w = word(j >> 1);
+    return __uint_as_float((j & 1) ? w & 0xffff0000u : w << 16);
+  }
+  // two magnitudes at a time: as 16-bit numbers they are ordered like the values, NaN above all
+  __device__ __forceinline__ uint32_t most() const {
+    const uint32_t m = __vmaxu2(__vmaxu2(q.x & 0x7fff7fffu, q.y & 0x7fff7fffu), __vmaxu2(q.z & 0x7fff7fffu, q.w & 0x7fff7fffu));
+    return max(m & 0xffff0000u, m << 16);
+  }
+  __device__ __forceinline__ void most_by_column(uint32_t (&m)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = __vmaxu2(m[j], word(j) & 0x7fff7fffu);
+  }
+};
+template <> struct Eight<float> {
+  float4 q[2];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const float* p, int n) {
+    if (VEC && n >= 8) {
+      q[0] = __ldg(reinterpret_cast<const float4*>(p));
+      q[1] = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    } else {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < n ? __ldg(p + j) : 0.f;
+      q[0] = make_float4(v[0], v[1], v[2], v[3]);
+      q[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+  }
+  __device__ __forceinline__ float value(int j) const {
+    const float4& r = q[j >> 2];
+    return (j & 3) == 0 ? r.x : (j & 3) == 1 ? r.y : (j & 3) == 2 ? r.z : r.w;
+  }
+  __device__ __forceinline__ uint32_t most() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(value(j)));
+    return m;
+  }
+  __device__ __forceinline__ void most_by_column(uint32_t (&m)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m[j] = max(m[j], abs_bits(value(j)));
+  }
+};
+template <class E>
+__device__ __forceinline__ uint2 fp8_codes(const E& e, float inv) {
+  return make_uint2(e4m3x4(e.value(0) * inv, e.value(1) * inv, e.value(2) * inv, e.value(3) * inv),
+                    e4m3x4(e.value(4) * inv, e.value(5) * inv, e.value(6) * inv, e.value(7) * inv));
 }
 
 // ---- rows: groups of 1 x 128 --------------------------------------------------------------------------------------
-// A half warp holds a group, eight values to a lane; a warp takes kQuantRows pairs of groups, whose loads are in flight
-// together.  With `flat_row` a row is a token and goes to the rows of its K assignments (negative: dropped), read once.
+// A half warp holds a group, eight values to a lane; a warp takes up to kQuantPairs neighbouring pairs of groups of one row, whose loads
+// are in flight together.  With `flat_row` a row is a token and goes to the rows of its K assignments (negative: dropped),
+// read once.
 constexpr int kQuantWarps = 8, kQuantPairs = 4;
 
 struct QuantRows {
   uint8_t* q;          // [.., ldq]
-  float* scale;        // (row, group) at row * scale_row + group * scale_group within its matrix
-  int64_t ldq, scale_row, scale_group, scale_batch;
+  float* scale;        // (matrix, row, group) at matrix * scale_batch + row * scale_row + group * scale_group
+  int64_t ldq, q_batch, scale_row, scale_group, scale_batch;
   const int32_t* flat_row;
   int slots;
 };
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kQuantWarps * 32)
-quantize_rows_kernel(const T* __restrict__ x, const QuantRows d, int64_t rows, int64_t rows_per_matrix, int K) {
+quantize_rows_kernel(const T* __restrict__ x, const QuantRows d, int64_t rows, int K) {
   pdl_trigger();
   const int lane = threadIdx.x & 31, l16 = lane & 15;
-  const int pairs = (K + 2 * kFp8Group - 1) / (2 * kFp8Group);
-  const int64_t total = rows * pairs;
-  const int64_t first = ((int64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5)) * kQuantPairs;
-  float v[kQuantPairs][8];
+  // the pieces of a row are neighbours in the grid
+  const unsigned pieces = (unsigned)((K + 2 * kQuantPairs * kFp8Group - 1) / (2 * kQuantPairs * kFp8Group));
+  const unsigned unit = blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
+  const int64_t row = unit / pieces;
+  const int k0 = (int)(unit - (unsigned)row * pieces) * (2 * kQuantPairs * kFp8Group) + lane * 8;
+  if (row >= rows) return;
+  const T* src = x + ((int64_t)blockIdx.y * rows + row) * K;
+  Eight<T> v[kQuantPairs];
 #pragma unroll
-  for (int i = 0; i < kQuantPairs; ++i) {
-    const int64_t u = first + i, row = u / pairs;
-    const int k = (int)(u - row * pairs) * 2 * kFp8Group + lane * 8;
-    load8<T, VEC>(x + row * K + k, u < total ? K - k : 0, v[i]);
-  }
+  for (int i = 0; i < kQuantPairs; ++i) v[i].template load<VEC>(src + k0 + i * 2 * kFp8Group, K - k0 - i * 2 * kFp8Group);
   pdl_wait();
   const int32_t* flat_row = d.flat_row != nullptr ? after_wait(d.flat_row) : nullptr;
 #pragma unroll
   for (int i = 0; i < kQuantPairs; ++i) {
-    const int64_t u = first + i, row = u / pairs;
-    const int k = (int)(u - row * pairs) * 2 * kFp8Group + lane * 8;
-    uint32_t most = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) most = max(most, abs_bits(v[i][j]));
+    const int k = k0 + i * 2 * kFp8Group;
+    if (k - lane * 8 >= K) break;
+    uint32_t most = v[i].most();
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (u >= total || k >= K) continue;
-    const float a = fp8_group_max(most), inv = fp8_inverse(a);
-    uint2 out;
-    out.x = e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-    out.y = e4m3x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
-    const float s = fp8_scale(a);
+    if (k >= K) continue;
+    const float a = fp8_group_max(most), s = fp8_scale(a);
+    const uint2 out = fp8_codes(v[i], fp8_inverse(a));
     if (flat_row == nullptr) {
-      *reinterpret_cast<uint2*>(d.q + row * d.ldq + k) = out;
-      if (l16 == 0) {
-        const int64_t b = row / rows_per_matrix, m = row - b * rows_per_matrix;
-        d.scale[b * d.scale_batch + m * d.scale_row + (k / kFp8Group) * d.scale_group] = s;
-      }
+      *reinterpret_cast<uint2*>(d.q + blockIdx.y * d.q_batch + row * d.ldq + k) = out;
+      if (l16 == 0) d.scale[blockIdx.y * d.scale_batch + row * d.scale_row + (k / kFp8Group) * d.scale_group] = s;
     } else {
       for (int j = 0; j < d.slots; ++j) {
         const int64_t r = flat_row[row * d.slots + j];
@@ -134,29 +170,26 @@ struct QuantOut {
 // Codes are turned around in shared memory with the 8-byte units of a row permuted (unit rg of row k lies at
 // rg ^ (k / 8)), so that neither the writing by columns nor the reading by rows meets bank conflicts.
 template <typename T, bool VEC, bool BLOCK>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, sizeof(T) == 2 && VEC ? 4 : 2)
 quantize_tile_kernel(const T* __restrict__ x, int64_t batch_stride, int M, int K, const QuantOut out, const QuantOut turned) {
+  constexpr int kWords = sizeof(T) == 2 ? 4 : 8;           // largest magnitudes of eight columns: bf16 two to a word
   __shared__ __align__(16) uint8_t s_codes[128 * 128];
-  __shared__ uint32_t s_max[8][128];
-  pdl_trigger();
+  __shared__ uint32_t s_max[8][16 * kWords];
+  __shared__ float s_inv[128];
   const int cg = threadIdx.x & 15, rg = threadIdx.x >> 4, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int m0 = blockIdx.y * 128, k0 = blockIdx.x * 128;
   const int64_t b = blockIdx.z;
   const int m = m0 + 8 * rg, k = k0 + 8 * cg;
-  float v[8][8];
-  pdl_wait();
+  Eight<T> v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    load8<T, VEC>(x + b * batch_stride + (int64_t)(m + i) * K + k, m + i < M ? K - k : 0, v[i]);
+    v[i].template load<VEC>(x + b * batch_stride + (int64_t)(m + i) * K + k, m + i < M ? K - k : 0);
 
   float inv_block = 0.f;
-  [[maybe_unused]] uint2 codes_t[8];
   if constexpr (BLOCK) {
     uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) most = max(most, abs_bits(v[i][j]));
+    for (int i = 0; i < 8; ++i) most = max(most, v[i].most());
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) s_max[0][warp] = most;
     __syncthreads();
@@ -165,65 +198,73 @@ quantize_tile_kernel(const T* __restrict__ x, int64_t batch_stride, int M, int K
     const float a = fp8_group_max(most);
     inv_block = fp8_inverse(a);
     if (threadIdx.x == 0) {
-      if (out.q != nullptr) out.scale[b * out.scale_batch + blockIdx.y * out.scale_row + blockIdx.x * out.scale_group] = fp8_scale(a);
+      const float s = fp8_scale(a);
+      if (out.q != nullptr) out.scale[b * out.scale_batch + blockIdx.y * out.scale_row + blockIdx.x * out.scale_group] = s;
       if (turned.q != nullptr)
-        turned.scale[b * turned.scale_batch + blockIdx.x * turned.scale_row + blockIdx.y * turned.scale_group] = fp8_scale(a);
+        turned.scale[b * turned.scale_batch + blockIdx.x * turned.scale_row + blockIdx.y * turned.scale_group] = s;
+    }
+  } else if (turned.q != nullptr) {
+    uint32_t most[kWords];
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) most[j] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i].most_by_column(most);
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, most[j], 16);       // the other row group of this warp
+      most[j] = sizeof(T) == 2 ? __vmaxu2(most[j], other) : max(most[j], other);
+      if (lane < 16) s_max[warp][kWords * cg + j] = most[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < 128) {
+      const int c = threadIdx.x;
+      uint32_t top = 0;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        if constexpr (sizeof(T) == 2) {
+          const uint32_t two = s_max[w][c >> 1];
+          top = max(top, (c & 1) ? two & 0xffff0000u : two << 16);
+        } else {
+          top = max(top, s_max[w][c]);
+        }
+      }
+      const float a = fp8_group_max(top);
+      s_inv[c] = fp8_inverse(a);
+      if (k0 + c < K)
+        turned.scale[b * turned.scale_batch + (int64_t)(k0 + c) * turned.scale_row + blockIdx.y * turned.scale_group] = fp8_scale(a);
     }
   }
   if (out.q != nullptr) {
+    float inv = inv_block;
+    if constexpr (!BLOCK) {
+      // lane cg of the sixteen that hold a row takes up row cg's division
+      uint32_t mine = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float inv = inv_block;
-      if constexpr (!BLOCK) {
-        uint32_t most = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) most = max(most, abs_bits(v[i][j]));
+      for (int i = 0; i < 8; ++i) {
+        uint32_t most = v[i].most();
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-        const float a = fp8_group_max(most);
-        inv = fp8_inverse(a);
-        if (cg == 0 && m + i < M)
-          out.scale[b * out.scale_batch + (int64_t)(m + i) * out.scale_row + blockIdx.x * out.scale_group] = fp8_scale(a);
+        if (cg == i) mine = most;
       }
-      if (m + i < M && k < K) {
-        uint2 c;
-        c.x = e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-        c.y = e4m3x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv);
-        *reinterpret_cast<uint2*>(out.q + b * out.q_batch + (int64_t)(m + i) * out.ld + k) = c;
-      }
+      const float a = fp8_group_max(mine);
+      inv = fp8_inverse(a);
+      if (cg < 8 && m + cg < M)
+        out.scale[b * out.scale_batch + (int64_t)(m + cg) * out.scale_row + blockIdx.x * out.scale_group] = fp8_scale(a);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float f = BLOCK ? inv : __shfl_sync(0xffffffffu, inv, (lane & 16) + i);
+      if (m + i < M && k < K) *reinterpret_cast<uint2*>(out.q + b * out.q_batch + (int64_t)(m + i) * out.ld + k) = fp8_codes(v[i], f);
     }
   }
   if (turned.q == nullptr) return;
-  float inv_col[8];
-  if constexpr (!BLOCK) {
-    uint32_t most[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      most[j] = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most[j] = max(most[j], abs_bits(v[i][j]));
-      most[j] = max(most[j], __shfl_xor_sync(0xffffffffu, most[j], 16));     // the other row group of this warp
-      if (lane < 16) s_max[warp][8 * cg + j] = most[j];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-#pragma unroll
-      for (int w = 0; w < 8; ++w) most[j] = max(most[j], s_max[w][8 * cg + j]);
-      const float a = fp8_group_max(most[j]);
-      inv_col[j] = fp8_inverse(a);
-      if (rg == 0 && k + j < K)
-        turned.scale[b * turned.scale_batch + (int64_t)(k + j) * turned.scale_row + blockIdx.y * turned.scale_group] = fp8_scale(a);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) inv_col[j] = inv_block;
-  }
+  if constexpr (!BLOCK) __syncthreads();
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
+    const float f = BLOCK ? inv_block : s_inv[8 * cg + j];
     uint2 c;
-    c.x = e4m3x4(v[0][j] * inv_col[j], v[1][j] * inv_col[j], v[2][j] * inv_col[j], v[3][j] * inv_col[j]);
-    c.y = e4m3x4(v[4][j] * inv_col[j], v[5][j] * inv_col[j], v[6][j] * inv_col[j], v[7][j] * inv_col[j]);
+    c.x = e4m3x4(v[0].value(j) * f, v[1].value(j) * f, v[2].value(j) * f, v[3].value(j) * f);
+    c.y = e4m3x4(v[4].value(j) * f, v[5].value(j) * f, v[6].value(j) * f, v[7].value(j) * f);
     *reinterpret_cast<uint2*>(s_codes + (8 * cg + j) * 128 + ((rg ^ cg) << 3)) = c;
   }
   __syncthreads();
@@ -243,16 +284,14 @@ inline bool rows_of_16_bytes(const void* x, int64_t K) {
   return (reinterpret_cast<uintptr_t>(x) & 15) == 0 && K * (int64_t)sizeof(T) % 16 == 0;
 }
 
+// `batch` matrices of `rows` rows
 template <typename T>
-inline int launch_quantize_rows(const T* x, const QuantRows& d, int64_t rows, int64_t rows_per_matrix, int K, bool pdl,
-                                cudaStream_t st) {
-  const int64_t work = ceil_div(rows * ceil_div(K, 2 * kFp8Group), kQuantPairs);
-  const int64_t ctas = ceil_div(work, kQuantWarps);
-  if (ctas == 0) return YAMOE_OK;
-  if (ctas > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
+inline int launch_quantize_rows(const T* x, const QuantRows& d, int64_t batch, int64_t rows, int K, bool pdl, cudaStream_t st) {
+  const int64_t ctas = ceil_div(rows * ceil_div(K, 2 * kQuantPairs * kFp8Group), kQuantWarps);
+  if (ctas == 0 || batch == 0) return YAMOE_OK;
+  if (ctas * kQuantWarps > 0x7fffffff || batch > 65535) return YAMOE_ERR_UNSUPPORTED;
   auto kern = rows_of_16_bytes<T>(x, K) ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
-  const cudaError_t rc =
-      launch_pdl_opt(pdl, kern, dim3((unsigned)ctas), dim3(kQuantWarps * 32), 0, st, x, d, rows, rows_per_matrix, K);
+  const cudaError_t rc = launch_pdl_opt(pdl, kern, dim3((unsigned)ctas, (unsigned)batch), dim3(kQuantWarps * 32), 0, st, x, d, rows, K);
   return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
 }
 
