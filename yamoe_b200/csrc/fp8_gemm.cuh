@@ -28,10 +28,10 @@
 namespace yb {
 
 // Three warpgroups: the first issues copies (warp 0) and instructions (warp 1), the others hold 128 fp32 sums per thread.
-// Registers go where they are needed: 384 threads start with 168 each, which is 56 + 2 x 224 for the three groups.
+// Registers go where they are needed: 384 threads start with 168 each, which is 40 + 2 x 232 for the three groups.
 constexpr int kFp8EpiWarps = 8, kFp8FirstEpiWarp = 4;
 constexpr int kFp8Threads = 32 * (kFp8FirstEpiWarp + kFp8EpiWarps);
-constexpr int kFp8FewRegs = 56, kFp8ManyRegs = 224;
+constexpr int kFp8FewRegs = 40, kFp8ManyRegs = 232;
 
 struct Fp8Params {
   int64_t M, N;                 // rows per matrix (not grouped), columns
@@ -72,20 +72,6 @@ __device__ __forceinline__ void tc_mma_fp8(uint32_t d, uint64_t a, uint64_t b, u
         "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void tc_ld_32x16_issue(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tc_ld_wait16(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :: "memory");
-}
 __device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -120,7 +106,7 @@ __global__ void __launch_bounds__(kFp8Threads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Fp8Params p,
                 const Epi epi) {
   using SM = Fp8Smem<CG, BN>;
-  constexpr int kStages = SM::kStages, kCols = BN / 2, kChunks = kCols / 16;
+  constexpr int kStages = SM::kStages, kCols = BN / 2, kChunks = kCols / 32;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kStages];       // CG = 2: used in the leader CTA
   __shared__ __align__(8) uint64_t bar_empty[kStages];      // per CTA
@@ -342,22 +328,23 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         if (ok) {
           tc_fence_after();
           const uint64_t s2 = BROWS ? pack_f32x2(sa_now, sa_now) : pack_f32x2(sa_now * sb_now, sa_now * sb_now);
-          uint32_t r[2][16];
+          // 32 columns at a time, the next ones on their way while these are added
+          uint32_t r[2][32];
           if (width > 0) {
-            tc_ld_32x16_issue(t_row + acc * BN, r[0]);
+            tc_ld_32x32_issue(t_row + acc * BN, r[0]);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
-              if (c * 16 < width) {
-                tc_ld_wait16(r[c & 1]);
-                if (c + 1 < kChunks && (c + 1) * 16 < width) tc_ld_32x16_issue(t_row + acc * BN + (c + 1) * 16, r[(c + 1) & 1]);
+              if (c * 32 < width) {
+                tc_ld_wait(r[c & 1]);
+                if (c + 1 < kChunks && (c + 1) * 32 < width) tc_ld_32x32_issue(t_row + acc * BN + (c + 1) * 32, r[(c + 1) & 1]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < 16; ++i) {
                   const uint64_t v = pack_f32x2(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1]));
                   if constexpr (BROWS) {
-                    const float2 s = *reinterpret_cast<const float2*>(&s_sb[acc][half * kCols + c * 16 + 2 * i]);
-                    sum[c * 8 + i] = fma_f32x2(v, mul_f32x2(s2, pack_f32x2(s.x, s.y)), sum[c * 8 + i]);
+                    const float2 s = *reinterpret_cast<const float2*>(&s_sb[acc][half * kCols + c * 32 + 2 * i]);
+                    sum[c * 16 + i] = fma_f32x2(v, mul_f32x2(s2, pack_f32x2(s.x, s.y)), sum[c * 16 + i]);
                   } else {
-                    sum[c * 8 + i] = fma_f32x2(v, s2, sum[c * 8 + i]);
+                    sum[c * 16 + i] = fma_f32x2(v, s2, sum[c * 16 + i]);
                   }
                 }
               }
