@@ -85,16 +85,34 @@ YB_INSTANTIATE(float)
 YB_INSTANTIATE(__nv_bfloat16)
 #undef YB_INSTANTIATE
 
+// Tiles of a product: estimated clocks of each kind, the least of them.  A block takes a pair's 256 x 256 tile some 700 clocks, a
+// 128 x 256 tile as many (what L2 delivers to one SM), 128 x 128 450; a tile's beginning and end 3000; meeting in shared memory 1500 more.
+struct Fp8Choice { int cg, bn, splits; };
+static Fp8Choice choose_tiles(int64_t B, int64_t M, int64_t N, int64_t K) {
+  const int64_t kb = ceil_div(K, kFp8Group);
+  Fp8Choice best{2, 256, 1};
+  double least = (double)ceil_div(B * ceil_div(M, 256) * ceil_div(N, 256), kSMs / 2) * (double)(kb * 700 + 3000);
+  const double one = (double)ceil_div(B * ceil_div(M, 128) * ceil_div(N, 256), kSMs) * (double)(kb * 700 + 3000);
+  if (one < least) { least = one; best = Fp8Choice{1, 256, 1}; }
+  const int64_t tiles = B * ceil_div(M, 128) * ceil_div(N, 128);
+  for (int s = 1; s <= kFp8MaxSplits && s <= kb; ++s) {
+    const double t = (double)ceil_div(tiles * s, kSMs) * (double)(ceil_div(kb, s) * 450 + 3000 + (s > 1 ? 1500 : 0));
+    if (t < least) { least = t; best = Fp8Choice{1, 128, s}; }
+  }
+  return best;
+}
+
 template <typename T, bool BROWS>
 static int mm_impl(const Fp8Operand& A, const Fp8Operand& B, Fp8Params p, T* out, cudaStream_t st) {
   const int vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.N * (int64_t)sizeof(T) % 16 == 0;
   const Fp8Store<T> epi{out, p.N, p.M * p.N, vec};
-  if (p.M > 128) {
-    p.MT = (int)ceil_div(p.M, 256);
-    return launch_fp8_gemm<2, 256, BROWS, false>(A, B, p, epi, (int64_t)p.B * p.MT, false, st);
-  }
-  p.MT = (int)ceil_div(p.M, 128);
-  return launch_fp8_gemm<1, 256, BROWS, false>(A, B, p, epi, (int64_t)p.B * p.MT, false, st);
+  const Fp8Choice c = choose_tiles(p.B, p.M, p.N, p.K);
+  p.MT = (int)ceil_div(p.M, 128 * c.cg);
+  p.splits = c.splits;
+  const int64_t tiles = (int64_t)p.B * p.MT;
+  if (c.cg == 2) return launch_fp8_gemm<2, 256, BROWS, false>(A, B, p, epi, tiles, false, st);
+  if (c.bn == 256) return launch_fp8_gemm<1, 256, BROWS, false>(A, B, p, epi, tiles, false, st);
+  return launch_fp8_gemm<1, 128, BROWS, false>(A, B, p, epi, tiles, false, st);
 }
 
 }  // namespace yb

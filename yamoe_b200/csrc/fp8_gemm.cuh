@@ -3,15 +3,20 @@
 //   C[m, n] = sum over blocks kb of 128:  sa[m, kb] * sb[n, kb] * (sum over k in kb of qa[m, k] * qb[n, k])
 //
 // The inner sums are exact products accumulated in fp32 in TMEM; scales differ from block to block, so an accumulator
-// holds ONE block (four instructions of 128 or 256 x N x 32) and is then added, times its scales, to fp32 registers of
-// the warps that later write the tile.  Two accumulators take turns: while the tensor core fills one, eight warps take
-// up the other.  A lane holds a row of C: with sb per 128 columns (weights) both scales are one number per thread and
-// block, and the whole addition is one packed multiply-add for two elements.  With a scale per row of B too (BROWS: weight
-// gradients) the columns' scales go through shared memory.
+// holds ONE block (four instructions of 128 or 256 x 128 x 32) and is then added, times its scales, to fp32 registers of
+// the warps that later write the tile.  A lane holds a row of C: with sb per 128 columns (weights) both scales are one
+// number per thread and accumulator, and the whole addition is one packed multiply-add for two elements.  With a scale per
+// row of B too (BROWS: weight gradients) the columns' scales go through shared memory.
+//
+// What bounds it are the adding warps, two on each scheduler, and the round trip of an accumulator: instructions, commit, loads
+// and additions, the arrivals, the issuer's wait.  So an accumulator has the whole width of the tile (one wait and one arrival
+// per block and warp), a load of 32 columns is always on its way while those before it are added, across blocks too, and
+// the scales are brought to shared memory by a warp of their own, four blocks at a time.
 //
 // Both operands are K-major with 128-byte swizzle: a block of 128 is one swizzle row.  CG = 2: CTA pairs
 // (cta_group::2), 256 x 256 tiles of which each CTA stages 128 rows of either operand, 32 KB per block where a CTA
-// alone stages 48 for a tile of 128 x 256.
+// alone stages 48 for a tile of 128 x 256.  Few tiles: 128 x 128, and a cluster of up to four CTAs shares a tile's blocks
+// (split), the sums of the others meeting in the first one's shared memory, added in order.
 //
 // Rows come as they are (`tile_expert` null: B matrices of M rows) or sorted by expert in the padded layout of the
 // expert pass, an expert's tiles following each other with the row tile varying fastest.
@@ -27,7 +32,8 @@
 
 namespace yb {
 
-// Three warpgroups: the first issues copies (warp 0) and instructions (warp 1), the others hold 128 fp32 sums per thread.
+// Three warpgroups: the first issues copies (warp 0), instructions (warp 1) and fetches scales (warp 2), the others hold 128 fp32
+// sums per thread.
 // Registers go where they are needed: 384 threads start with 168 each, which is 40 + 2 x 232 for the three groups.
 constexpr int kFp8EpiWarps = 8, kFp8FirstEpiWarp = 4;
 constexpr int kFp8Threads = 32 * (kFp8FirstEpiWarp + kFp8EpiWarps);
@@ -47,15 +53,24 @@ struct Fp8Params {
   const int32_t* n_tiles;       // how many there are
   int32_t* status;              // device status word
   int clear_status;             // no earlier kernel of the call has set it to 0
+  int splits;                   // CTAs of a cluster that share a tile's blocks (BN = 128); each cluster has one tile then
 };
+constexpr int kFp8MaxSplits = 4;
 
-template <int CG, int BN>
+constexpr int kFp8ScaleBlocks = 4, kFp8ScaleSlots = 2;     // blocks of 128 whose scales come together, such groups on their way
+constexpr int kFp8ParkBytes = 32 * 64;                     // per epilogue warp: 64 bytes of each of its rows
+
+template <int CG, int BN, bool BROWS>
 struct Fp8Smem {
   static constexpr int kABytes = 128 * 128;
   static constexpr int kBBytes = BN / CG * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
   static constexpr int kStages = 196608 / kStageBytes;     // 4 (one CTA, 256 columns) or 6
-  static constexpr int kTables = kStages * kStageBytes + 1024;
+  static_assert(kStages * kStageBytes >= (kFp8MaxSplits - 1) * 128 * 128 * 4, "the sums of the others of a cluster");
+  static constexpr int kScaleFloats = 128 + (BROWS ? BN : 4);                    // of a block: rows, columns or column blocks
+  static constexpr int kPark = kStages * kStageBytes;                            // from the 1024-byte boundary on
+  static constexpr int kScales = kPark + kFp8EpiWarps * kFp8ParkBytes;
+  static constexpr int kTables = kScales + kFp8ScaleSlots * kFp8ScaleBlocks * kScaleFloats * 4 + 1024;
 };
 inline int fp8_smem_bytes(int tables, int experts) { return tables + (experts > 0 ? 2 * (experts + 1) * 4 : 0); }
 
@@ -91,13 +106,18 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
   return d;
 }
 
-// What an epilogue gets: the thread's row and the COLS columns from n0 on whose sums it holds (columns in pairs).
+__device__ __forceinline__ void copy_float(uint32_t dst, const float* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
+
+// What an epilogue gets: the thread's row and the COLS columns from n0 on whose sums it holds, in pairs.
 struct Fp8Tile {
   int b;               // matrix or expert
   int64_t row;         // row of the matrix, or padded row of the expert pass
   int64_t row_end;     // rows from here on are another's
   int n0, n_end;       // n_end: columns of the matrix
   int q, half, lane;   // lane quarter and column half of the warp
+  uint32_t park;       // kFp8ParkBytes of shared memory of the warp's own
   bool ok;             // false: take part in barriers only
 };
 
@@ -105,22 +125,26 @@ template <int CG, int BN, bool BROWS, bool GROUPED, class Epi>
 __global__ void __launch_bounds__(kFp8Threads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Fp8Params p,
                 const Epi epi) {
-  using SM = Fp8Smem<CG, BN>;
-  constexpr int kStages = SM::kStages, kCols = BN / 2, kChunks = kCols / 32;
+  using SM = Fp8Smem<CG, BN, BROWS>;
+  constexpr int kStages = SM::kStages, kAccs = 512 / BN, kCols = BN / 2;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_full[kStages];       // CG = 2: used in the leader CTA
   __shared__ __align__(8) uint64_t bar_empty[kStages];      // per CTA
-  __shared__ __align__(8) uint64_t bar_tmem_full[2];        // per CTA
-  __shared__ __align__(8) uint64_t bar_tmem_empty[2];       // CG = 2: used in the leader CTA
+  __shared__ __align__(8) uint64_t bar_tmem_full[kAccs];       // per CTA
+  __shared__ __align__(8) uint64_t bar_tmem_empty[kAccs];      // CG = 2: used in the leader CTA
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
-  __shared__ __align__(16) float s_sb[BROWS ? 2 : 1][BROWS ? BN : 1];
+  __shared__ __align__(8) uint64_t bar_scale_full[kFp8ScaleSlots], bar_scale_empty[kFp8ScaleSlots];
   __shared__ typename Epi::Shared s_epi;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
   const bool leader = rank == 0;
+  const int splits = CG == 1 && BN == 128 && !GROUPED ? p.splits : 1;
+  const int part = splits > 1 ? (int)cluster_ctarank() : 0;       // of the tile's blocks
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* const aligned = smem_raw + (smem_base - smem_u32(smem_raw));
+  float* const s_scale = reinterpret_cast<float*>(aligned + SM::kScales);
   int32_t* s_first = reinterpret_cast<int32_t*>(smem_raw + SM::kTables);   // grouped: first tile of each expert
   int32_t* s_pad = s_first + p.B + 1;                                      // first padded row of each expert
 
@@ -129,9 +153,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       mbar_init(smem_u32(&bar_full[s]), CG);
       mbar_init(smem_u32(&bar_empty[s]), 1);
     }
-    for (int a = 0; a < 2; ++a) {
+    for (int a = 0; a < kAccs; ++a) {
       mbar_init(smem_u32(&bar_tmem_full[a]), 1);
       mbar_init(smem_u32(&bar_tmem_empty[a]), CG * kFp8EpiWarps);
+    }
+    for (int i = 0; i < kFp8ScaleSlots; ++i) {
+      mbar_init(smem_u32(&bar_scale_full[i]), 32);
+      mbar_init(smem_u32(&bar_scale_empty[i]), kFp8EpiWarps);
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -139,11 +167,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   if (warp == 1) {
     if constexpr (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                   ::"r"(smem_u32(&tmem_base_slot)), "r"(2u * BN) : "memory");
+                   ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else {
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
-                   ::"r"(smem_u32(&tmem_base_slot)), "r"(2u * BN) : "memory");
+                   ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
   }
@@ -163,8 +191,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   }
   if (p.clear_status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = kStatusOk;   // waits give up after seconds at the earliest
   const int64_t total = GROUPED ? (int64_t)*after_wait(p.n_tiles) * p.NT : (int64_t)p.B * p.MT * p.NT;
-  const int64_t first_id = blockIdx.x / CG, n_workers = gridDim.x / CG;
-  const int kblocks = (p.K + kFp8Group - 1) / kFp8Group;
+  const int64_t first_id = blockIdx.x / (CG * splits), n_workers = gridDim.x / (CG * splits);
+  const int kblocks_all = (p.K + kFp8Group - 1) / kFp8Group;
+  const int kb_first = part * kblocks_all / splits, kb_end = (part + 1) * kblocks_all / splits;
 
   // work item -> matrix or expert, first row of the tile, first column
   auto decode = [&](int64_t id, int& b, int64_t& m0, int& n0) {
@@ -205,7 +234,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         decode(id, b, m0, n0);
         const int width = min(BN, ((int)p.N - n0 + 15) & ~15);
         const int am = (int)m0 + (int)rank * 128, bn = n0 + (int)rank * (width / CG);
-        for (int kb = 0; kb < kblocks; ++kb) {
+        for (int kb = kb_first; kb < kb_end; ++kb) {
           ok = mbar_wait_warp(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag);
           if (!ok) break;
           if (elected) {
@@ -248,31 +277,29 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           int b, n0;
           int64_t m0;
           decode(id, b, m0, n0);
-          const uint32_t width = min(BN, ((int)p.N - n0 + 15) & ~15);
-          const uint32_t idesc = idesc_base | ((width >> 3) << 17);
-          for (int kb = 0; kb < kblocks; ++kb) {
-            ok = mbar_wait_warp(smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, &abort_flag);
-            if (ok) ok = mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &abort_flag);
+          const uint32_t idesc = idesc_base | ((uint32_t)(min(BN, ((int)p.N - n0 + 15) & ~15) >> 3) << 17);
+          for (int kb = kb_first; kb < kb_end; ++kb) {
+            ok = mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &abort_flag);
+            if (ok) ok = mbar_wait_warp(smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, &abort_flag);
             if (!ok) break;
             tc_fence_after();
             if (elected) {
               const uint64_t adesc = adesc0 + (uint64_t)(stage * (SM::kStageBytes >> 4));
               const uint64_t bdesc = bdesc0 + (uint64_t)(stage * (SM::kStageBytes >> 4));
-  #pragma unroll
+#pragma unroll
               for (int k = 0; k < kFp8Group / 32; ++k)
                 tc_mma_fp8<CG>(tmem_base + acc * BN, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, (uint32_t)(k != 0));
               if constexpr (CG == 1) {
-                tc_commit(smem_u32(&bar_empty[stage]));
                 tc_commit(smem_u32(&bar_tmem_full[acc]));
+                tc_commit(smem_u32(&bar_empty[stage]));
               } else {
-                tc2_commit_pair(smem_u32(&bar_empty[stage]));
                 tc2_commit_pair(smem_u32(&bar_tmem_full[acc]));
+                tc2_commit_pair(smem_u32(&bar_empty[stage]));
               }
             }
             __syncwarp();
             if (++stage == kStages) { stage = 0; phase ^= 1u; }
-            acc ^= 1;
-            if (acc == 0) acc_phase ^= 1u;
+            if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
           }
         }
         if (!ok && lane == 0) {
@@ -281,15 +308,59 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         }
       }
       __syncwarp();
+    } else if (warp == 2) {
+      // =========================== scales (of each CTA) ========================================
+      // Four bytes at a time, each on its way by itself; rows and columns that do not exist are 0.
+      int slot = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int64_t id = first_id; id < total && ok; id += n_workers) {
+        int b, n0;
+        int64_t m0;
+        decode(id, b, m0, n0);
+        const int64_t row0 = m0 + rank * 128, row_end = GROUPED ? (int64_t)s_pad[b + 1] : p.M;
+        const float* sa = p.sa + (GROUPED ? 0 : b * p.sa_b);
+        const float* sb = p.sb + b * p.sb_b;
+        for (int kb = kb_first; kb < kb_end; kb += kFp8ScaleBlocks) {
+          ok = mbar_wait_warp(smem_u32(&bar_scale_empty[slot]), phase ^ 1u, &abort_flag);
+          if (!ok) break;
+          for (int i = 0; i < kFp8ScaleBlocks && kb + i < kb_end; ++i) {
+            const uint32_t dst = smem_u32(s_scale + (slot * kFp8ScaleBlocks + i) * SM::kScaleFloats);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int64_t row = row0 + j * 32 + lane;
+              copy_float(dst + (j * 32 + lane) * 4, sa + (row < row_end ? row : 0) * p.sa_m + (kb + i) * p.sa_k, row < row_end);
+            }
+            if constexpr (BROWS) {
+#pragma unroll
+              for (int j = 0; j < BN / 32; ++j) {
+                const int col = n0 + j * 32 + lane;
+                copy_float(dst + (128 + j * 32 + lane) * 4, sb + (int64_t)(col < p.N ? col : 0) * p.sb_n + (kb + i) * p.sb_k, col < p.N);
+              }
+            } else if (lane < BN / 128) {
+              const bool there = n0 + lane * 128 < p.N;
+              copy_float(dst + (128 + lane) * 4, sb + (int64_t)(n0 / kFp8Group + (there ? lane : 0)) * p.sb_n + (kb + i) * p.sb_k, there);
+            }
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bar_scale_full[slot])) : "memory");
+          if (++slot == kFp8ScaleSlots) { slot = 0; phase ^= 1u; }
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (!ok && lane == 0) {
+        abort_flag = 1;
+        atomicMax(p.status, (int)kStatusProducerTimeout);
+      }
+      __syncwarp();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFp8ManyRegs));
     // =========================== scaled sums and epilogue (warps 4 .. 11 of each CTA) ========
     const int q = warp & 3;                      // TMEM lane quarter this warp may read
-    const int half = (warp - kFp8FirstEpiWarp) >> 2;            // its columns: kCols from half * kCols on
+    const int half = (warp - kFp8FirstEpiWarp) >> 2;      // its columns: kCols from half * kCols on
     const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + half * kCols;
-    int acc = 0;
-    uint32_t acc_phase = 0, parity = 0;
+    int acc = 0, slot = 0;
+    uint32_t acc_phase = 0, slot_phase = 0, parity = 0;
     bool ok = true;
     for (int64_t id = first_id; id < total; id += n_workers, parity ^= 1u) {
       Fp8Tile t;
@@ -301,66 +372,103 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       t.n0 = n0 + half * kCols;
       t.n_end = (int)p.N;
       t.q = q; t.half = half; t.lane = lane;
-      const int width = min(BN, ((int)p.N - n0 + 15) & ~15) - half * kCols;    // columns computed; may be <= 0
+      t.park = smem_base + SM::kPark + (warp - kFp8FirstEpiWarp) * kFp8ParkBytes;
       const bool row_ok = t.row < t.row_end;
       const auto pre = epi.begin(t, row_ok);
-      const float* sa = p.sa + (GROUPED ? 0 : t.b * p.sa_b) + (row_ok ? t.row : 0) * p.sa_m;
-      const float* sb;
-      const bool col_mine = BROWS && t.n0 + q * 32 + lane < p.N && (kCols == 128 || q * 32 < kCols);
-      if constexpr (BROWS) sb = p.sb + t.b * p.sb_b + (col_mine ? (int64_t)(t.n0 + q * 32 + lane) : 0) * p.sb_n;
-      else sb = p.sb + t.b * p.sb_b + (int64_t)(min(t.n0, (int)p.N - 1) / kFp8Group) * p.sb_n;
-      float sa_next = *sa, sb_next = *sb;
       uint64_t sum[kCols / 2];
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) sum[i] = 0;
-      for (int kb = 0; kb < kblocks; ++kb) {
-        const float sa_now = sa_next, sb_now = sb_next;
-        if (kb + 1 < kblocks) {
-          sa_next = sa[(kb + 1) * p.sa_k];
-          sb_next = sb[(kb + 1) * p.sb_k];
-        }
-        if constexpr (BROWS) {
-          // the columns' scales of this half; of the other buffer the warps of this half are done once they meet here
-          if (kCols == 128 || q * 32 < kCols) s_sb[acc][half * kCols + q * 32 + lane] = col_mine ? sb_now : 0.f;
-          named_sync(1 + half, 128);
-        }
-        if (ok) ok = mbar_wait_warp(smem_u32(&bar_tmem_full[acc]), acc_phase, &abort_flag);
+      // (Columns behind the matrix are loaded and added like others; nobody reads their sums.)
+      uint32_t r[2][32];
+      if (ok) ok = mbar_wait_warp(smem_u32(&bar_tmem_full[acc]), acc_phase, &abort_flag);
+      if (ok) {
+        tc_fence_after();
+        tc_ld_32x32_issue(t_row + acc * BN, r[0]);
+      }
+      for (int kb = kb_first; kb < kb_end; ++kb) {
+        const int in_slot = (kb - kb_first) % kFp8ScaleBlocks;
+        if (in_slot == 0 && ok) ok = mbar_wait_warp(smem_u32(&bar_scale_full[slot]), slot_phase, &abort_flag);
+        const float* scale = s_scale + (slot * kFp8ScaleBlocks + in_slot) * SM::kScaleFloats;
+        const float sa = scale[q * 32 + lane], s = BROWS ? sa : sa * scale[128 + half * kCols / 128];
+        const uint64_t s2 = pack_f32x2(s, s);
+        const bool last = kb + 1 == kb_end;
+        const int next = acc + 1 == kAccs ? 0 : acc + 1;
+        const uint32_t next_phase = acc_phase ^ (next == 0 ? 1u : 0u);
+        uint32_t early = 0;
         if (ok) {
-          tc_fence_after();
-          const uint64_t s2 = BROWS ? pack_f32x2(sa_now, sa_now) : pack_f32x2(sa_now * sb_now, sa_now * sb_now);
-          // 32 columns at a time, the next ones on their way while these are added
-          uint32_t r[2][32];
-          if (width > 0) {
-            tc_ld_32x32_issue(t_row + acc * BN, r[0]);
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-              if (c * 32 < width) {
-                tc_ld_wait(r[c & 1]);
-                if (c + 1 < kChunks && (c + 1) * 32 < width) tc_ld_32x32_issue(t_row + acc * BN + (c + 1) * 32, r[(c + 1) & 1]);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const uint64_t v = pack_f32x2(__uint_as_float(r[c & 1][2 * i]), __uint_as_float(r[c & 1][2 * i + 1]));
-                  if constexpr (BROWS) {
-                    const float2 s = *reinterpret_cast<const float2*>(&s_sb[acc][half * kCols + c * 32 + 2 * i]);
-                    sum[c * 16 + i] = fma_f32x2(v, mul_f32x2(s2, pack_f32x2(s.x, s.y)), sum[c * 16 + i]);
-                  } else {
-                    sum[c * 16 + i] = fma_f32x2(v, s2, sum[c * 16 + i]);
-                  }
+          for (int c = 0; c < kCols / 32; ++c) {
+            uint32_t (&now)[32] = r[c & 1], (&then)[32] = r[(c + 1) & 1];
+            tc_ld_wait(now);
+            if (c + 1 < kCols / 32) {
+              tc_ld_32x32_issue(t_row + acc * BN + (c + 1) * 32, then);
+              if (c + 2 == kCols / 32) early = last ? 1u : mbar_try_wait(smem_u32(&bar_tmem_full[next]), next_phase);
+            } else {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                if constexpr (CG == 1) mbar_arrive(smem_u32(&bar_tmem_empty[acc]));
+                else mbar_arrive_cluster(mapa_u32(smem_u32(&bar_tmem_empty[acc]), 0));
+              }
+              if (!last) {
+                if (!__all_sync(0xffffffffu, early != 0)) ok = mbar_wait_warp(smem_u32(&bar_tmem_full[next]), next_phase, &abort_flag);
+                if (ok) {
+                  tc_fence_after();
+                  tc_ld_32x32_issue(t_row + next * BN, then);
                 }
               }
             }
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (CG == 1) mbar_arrive(smem_u32(&bar_tmem_empty[acc]));
-            else mbar_arrive_cluster(mapa_u32(smem_u32(&bar_tmem_empty[acc]), 0));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint64_t v = pack_f32x2(__uint_as_float(now[2 * i]), __uint_as_float(now[2 * i + 1]));
+              if constexpr (BROWS) {
+                const float2 f = *reinterpret_cast<const float2*>(scale + 128 + half * kCols + c * 32 + 2 * i);
+                sum[c * 16 + i] = fma_f32x2(v, mul_f32x2(s2, pack_f32x2(f.x, f.y)), sum[c * 16 + i]);
+              } else {
+                sum[c * 16 + i] = fma_f32x2(v, s2, sum[c * 16 + i]);
+              }
+            }
           }
         }
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1u;
+        acc = next;
+        acc_phase = next_phase;
+        if (in_slot == kFp8ScaleBlocks - 1 || last) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bar_scale_empty[slot]));
+          if (++slot == kFp8ScaleSlots) { slot = 0; slot_phase ^= 1u; }
+        }
       }
       t.ok = ok;
+      if constexpr (CG == 1 && BN == 128 && !GROUPED) {
+        if (splits > 1) {
+          // [part - 1][column of the tile][row]: a warp stores 128 contiguous bytes
+          const int row = q * 32 + lane;
+          cluster_sync_all();                    // the first CTA's copies and instructions are done with its shared memory
+          if (part > 0 && row_ok) {
+            const uint32_t dst = mapa_u32(smem_base, 0) + (uint32_t)((((part - 1) * 128 + half * kCols) * 128 + row) * 4);
+#pragma unroll
+            for (int i = 0; i < kCols / 2; ++i) {
+              float lo, hi;
+              unpack_f32x2(sum[i], lo, hi);
+              asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + (uint32_t)(2 * i) * 512u), "f"(lo) : "memory");
+              asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + (uint32_t)(2 * i + 1) * 512u), "f"(hi) : "memory");
+            }
+          }
+          cluster_sync_all();
+          if (part > 0) break;
+          for (int o = 1; o < splits; ++o) {
+            const uint32_t src = smem_base + (uint32_t)((((o - 1) * 128 + half * kCols) * 128 + row) * 4);
+#pragma unroll
+            for (int i = 0; i < kCols / 2; ++i) {
+              float lo, hi, x, y;
+              unpack_f32x2(sum[i], lo, hi);
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(src + (uint32_t)(2 * i) * 512u));
+              asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(src + (uint32_t)(2 * i + 1) * 512u));
+              sum[i] = pack_f32x2(lo + x, hi + y);
+            }
+          }
+        }
+      }
       epi.template finish<kCols>(t, row_ok, pre, sum, s_epi, parity);
     }
     if (!ok) {
@@ -369,6 +477,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
   }
 
+  if (splits > 1 && warp < kFp8FirstEpiWarp) {     // what the other warps do between their sums and their epilogue
+    cluster_sync_all();
+    cluster_sync_all();
+  }
   // ---- teardown ---------------------------------------------------------------------------
   tc_fence_before();
   __syncthreads();
@@ -382,15 +494,38 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   if (warp == 1) {
     tc_fence_after();
     if constexpr (CG == 1)
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2u * BN) : "memory");
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
     else
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2u * BN) : "memory");
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
   }
 }
 
 // ---------------------------------------------------------------------------------------------
 // Epilogues
 // ---------------------------------------------------------------------------------------------
+
+// 64 bytes of each of the warp's 32 rows (a lane's own, in `v`) to `dst` (null: nowhere), of which `pieces` of 16 bytes
+// exist.  By way of shared memory, so that four lanes write a row's bytes side by side: straight from the lanes that hold
+// them, 16 bytes to 32 rows at a time, the stores of a 256 x 256 tile of bf16 took 6000 clocks, during which no
+// accumulator is taken up.
+__device__ __forceinline__ void store_rows_64(uint32_t park, int lane, const uint4 (&v)[4], char* dst, int pieces) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(park + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)), "r"(v[k].x),
+                 "r"(v[k].y), "r"(v[k].z), "r"(v[k].w) : "memory");
+  __syncwarp();
+  const int k = lane & 3;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    char* to = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+    uint4 x;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "r"(park + r * 64 + ((k ^ ((r >> 1) & 3)) << 4)) : "memory");
+    if (to != nullptr && k < pieces) *reinterpret_cast<uint4*>(to + 16 * k) = x;
+  }
+  __syncwarp();
+}
 
 // C[b, m, n] rounded to T
 template <typename T>
@@ -405,25 +540,32 @@ struct Fp8Store {
   template <int COLS>
   __device__ __forceinline__ void finish(const Fp8Tile& t, bool row_ok, const Pre&, const uint64_t (&sum)[COLS / 2], Shared&,
                                          uint32_t) const {
-    if (!t.ok || !row_ok) return;
+    if (!t.ok) return;
+    constexpr int VE = 16 / (int)sizeof(T), kCols = 64 / (int)sizeof(T);     // columns of 16 and of 64 bytes
     T* c = C + t.b * batch + t.row * ld + t.n0;
-    constexpr int VE = 16 / (int)sizeof(T);
-    const int cols = t.n_end - t.n0;
 #pragma unroll
-    for (int i = 0; i < COLS; i += VE) {
-      float v[VE];
+    for (int i = 0; i < COLS; i += kCols) {
+      const int cols = t.n_end - t.n0 - i;
+      if (cols <= 0) break;
+      float v[kCols];
 #pragma unroll
-      for (int j = 0; j < VE; j += 2) unpack_f32x2(sum[(i + j) / 2], v[j], v[j + 1]);
-      if (vec && i + VE <= cols) {
-        if constexpr (sizeof(T) == 2)
-          *reinterpret_cast<uint4*>(c + i) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                                                        pack_bf16x2(v[6], v[7]));
-        else
-          *reinterpret_cast<float4*>(c + i) = make_float4(v[0], v[1], v[2], v[3]);
-      } else {
+      for (int j = 0; j < kCols; j += 2) unpack_f32x2(sum[(i + j) / 2], v[j], v[j + 1]);
+      if (vec) {
+        uint4 w[4];
 #pragma unroll
-        for (int j = 0; j < VE; ++j)
-          if (i + j < cols) DT<T>::st(c + i + j, v[j]);
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (sizeof(T) == 2)
+            w[k] = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                              pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+          else
+            w[k] = make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
+                              __float_as_uint(v[4 * k + 3]));
+        }
+        store_rows_64(t.park, t.lane, w, row_ok ? reinterpret_cast<char*>(c + i) : nullptr, cols / VE);
+      } else if (row_ok) {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+          if (j < cols) DT<T>::st(c + i + j, v[j]);
       }
     }
   }
@@ -446,35 +588,36 @@ struct Fp8GluQuant {
   __device__ __forceinline__ void finish(const Fp8Tile& t, bool row_ok, const Pre&, const uint64_t (&sum)[COLS / 2], Shared& s,
                                          uint32_t parity) const {
     static_assert(COLS == 128, "a group of 128 activations is a tile of 256 columns");
-    float a[COLS / 2];
+    float a[64];
     uint32_t most = 0;
     const T* bs = bias + (int64_t)t.b * t.n_end + t.n0;
 #pragma unroll
-    for (int i = 0; i < COLS / 2; ++i) {
-      float g, u;
-      unpack_f32x2(sum[i], g, u);
-      a[i] = 0.f;
-      if (t.n0 + 2 * i < t.n_end) a[i] = glu_act(g + DT<T>::ld(bs + 2 * i), u + DT<T>::ld(bs + 2 * i + 1));
-      most = max(most, abs_bits(a[i]));
+    for (int i = 0; i < 64; i += 4) {
+      float b[8];                                  // eight columns: n_end is a multiple of 16, and so is n0
+      if (t.n0 + 2 * i < t.n_end) load_vec<T, 8>(bs + 2 * i, b);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float g, v;
+        unpack_f32x2(sum[i + j], g, v);
+        a[i + j] = t.n0 + 2 * i < t.n_end ? glu_act(g + b[2 * j], v + b[2 * j + 1]) : 0.f;
+        most = max(most, abs_bits(a[i + j]));
+      }
     }
     const int r = t.q * 32 + t.lane;
     s.most[parity][t.half][r] = most;
     named_sync(4 + t.q, 64);
-    if (!t.ok || !row_ok || t.n0 >= t.n_end) return;
+    if (!t.ok || t.n0 >= t.n_end) return;
     const float top = fp8_group_max(max(most, s.most[parity][t.half ^ 1][r])), inv = fp8_inverse(top);
-    const int64_t col = t.n0 / 2;
-    uint8_t* dst = act + t.row * ld + col;
+    uint4 w[4];
 #pragma unroll
-    for (int i = 0; i < COLS / 2; i += 16)
-      if (col + i < ld) {
-        uint4 c;
-        c.x = e4m3x4(a[i] * inv, a[i + 1] * inv, a[i + 2] * inv, a[i + 3] * inv);
-        c.y = e4m3x4(a[i + 4] * inv, a[i + 5] * inv, a[i + 6] * inv, a[i + 7] * inv);
-        c.z = e4m3x4(a[i + 8] * inv, a[i + 9] * inv, a[i + 10] * inv, a[i + 11] * inv);
-        c.w = e4m3x4(a[i + 12] * inv, a[i + 13] * inv, a[i + 14] * inv, a[i + 15] * inv);
-        *reinterpret_cast<uint4*>(dst + i) = c;
-      }
-    if (t.half == 0) scale[(t.n0 / (2 * kFp8Group)) * scale_group + t.row] = fp8_scale(top);
+    for (int k = 0; k < 4; ++k)
+      w[k] = make_uint4(e4m3x4(a[16 * k] * inv, a[16 * k + 1] * inv, a[16 * k + 2] * inv, a[16 * k + 3] * inv),
+                        e4m3x4(a[16 * k + 4] * inv, a[16 * k + 5] * inv, a[16 * k + 6] * inv, a[16 * k + 7] * inv),
+                        e4m3x4(a[16 * k + 8] * inv, a[16 * k + 9] * inv, a[16 * k + 10] * inv, a[16 * k + 11] * inv),
+                        e4m3x4(a[16 * k + 12] * inv, a[16 * k + 13] * inv, a[16 * k + 14] * inv, a[16 * k + 15] * inv));
+    const int64_t col = t.n0 / 2;
+    store_rows_64(t.park, t.lane, w, row_ok ? reinterpret_cast<char*>(act + t.row * ld + col) : nullptr, (int)(ld - col) / 16);
+    if (row_ok && t.half == 0) scale[(t.n0 / (2 * kFp8Group)) * scale_group + t.row] = fp8_scale(top);
   }
 };
 
@@ -503,19 +646,27 @@ struct Fp8WeightedRows {
   template <int COLS>
   __device__ __forceinline__ void finish(const Fp8Tile& t, bool, const Pre& p, const uint64_t (&sum)[COLS / 2], Shared&,
                                          uint32_t) const {
-    if (!t.ok || p.at < 0) return;
+    if (!t.ok) return;
     float* dst = y + p.at * N + t.n0;
     const T* bs = bias + t.b * N + t.n0;
-    const int cols = t.n_end - t.n0;                   // a multiple of 8
 #pragma unroll
-    for (int i = 0; i < COLS; i += 4)
-      if (i < cols) {
+    for (int i = 0; i < COLS; i += 16) {
+      const int cols = t.n_end - t.n0 - i;         // a multiple of 8
+      if (cols <= 0) break;
+      float b[16];
+      load_vec<T, 8>(bs + i, *reinterpret_cast<float(*)[8]>(b));
+      if (cols > 8) load_vec<T, 8>(bs + i + 8, *reinterpret_cast<float(*)[8]>(b + 8));
+      uint4 w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
         float v[4];
-        unpack_f32x2(sum[i / 2], v[0], v[1]);
-        unpack_f32x2(sum[i / 2 + 1], v[2], v[3]);
-        *reinterpret_cast<float4*>(dst + i) = make_float4(p.w * (v[0] + DT<T>::ld(bs + i)), p.w * (v[1] + DT<T>::ld(bs + i + 1)),
-                                                          p.w * (v[2] + DT<T>::ld(bs + i + 2)), p.w * (v[3] + DT<T>::ld(bs + i + 3)));
+        unpack_f32x2(sum[(i + 4 * k) / 2], v[0], v[1]);
+        unpack_f32x2(sum[(i + 4 * k) / 2 + 1], v[2], v[3]);
+        w[k] = make_uint4(__float_as_uint(p.w * (v[0] + b[4 * k])), __float_as_uint(p.w * (v[1] + b[4 * k + 1])),
+                          __float_as_uint(p.w * (v[2] + b[4 * k + 2])), __float_as_uint(p.w * (v[3] + b[4 * k + 3])));
       }
+      store_rows_64(t.park, t.lane, w, p.at >= 0 ? reinterpret_cast<char*>(dst + i) : nullptr, cols / 4);
+    }
   }
 };
 
@@ -529,7 +680,7 @@ inline int fp8_resident(void (*kern)(KArgs...), PerDevice<int>& known) {
   const int dev = current_device_index();
   int n = known.get(dev);
   if (n > 0) return n;
-  constexpr int kMost = 227 * 1024 - 8192;     // static shared memory beside it
+  constexpr int kMost = 227 * 1024 - 3072;     // static shared memory beside it
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess) return 0;
   if (CG == 1) {
     n = umma_sm_count();
@@ -563,7 +714,7 @@ template <int CG, int BN, bool BROWS, bool GROUPED, class Epi>
 inline int launch_fp8_gemm(const Fp8Operand& a, const Fp8Operand& b, Fp8Params p, const Epi& epi, int64_t max_tiles, bool pdl,
                            cudaStream_t st) {
   if (!umma_available()) return YAMOE_ERR_UNSUPPORTED;
-  using SM = Fp8Smem<CG, BN>;
+  using SM = Fp8Smem<CG, BN, BROWS>;
   CUtensorMap tmA, tmB;
   const uint64_t na = GROUPED ? 1 : (uint64_t)p.B;
   const uint64_t da[3] = {(uint64_t)p.K, (uint64_t)a.rows, na}, db[3] = {(uint64_t)p.K, (uint64_t)b.rows, (uint64_t)p.B};
@@ -578,14 +729,16 @@ inline int launch_fp8_gemm(const Fp8Operand& a, const Fp8Operand& b, Fp8Params p
   p.NT = (int)ceil_div(p.N, BN);
   const int64_t total = max_tiles * p.NT;
   if (total <= 0) return YAMOE_OK;
+  const bool split = CG == 1 && BN == 128 && !GROUPED && p.splits > 1;
+  if (!split) p.splits = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(total, workers)));
+  cfg.gridDim = dim3((unsigned)(split ? p.splits * total : CG * std::min<int64_t>(total, workers)));
   cfg.blockDim = dim3(kFp8Threads);
   cfg.dynamicSmemBytes = (size_t)fp8_smem_bytes(SM::kTables, GROUPED ? p.B : 0);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.x = CG * p.splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled(pdl) ? 1 : 0;
