@@ -40,30 +40,18 @@ template int fp8_gather<float>(const float*, uint8_t*, float*, int64_t, int64_t,
 template int fp8_gather<__nv_bfloat16>(const __nv_bfloat16*, uint8_t*, float*, int64_t, int64_t, const int32_t*, int64_t, int, int,
                                        cudaStream_t);
 
-// Rows per expert from which the grouped products go by CTA pairs (tiles of 256 rows)
-static bool fp8_pairs(const Fp8Rows& r, int E) { return r.S > 128 * (int64_t)E; }
-
-static Fp8Params grouped_params(const Fp8Rows& r, const float* a_scale, const yamoe_fp8_matrix_t& w, int N, int K, int E, bool pairs) {
+template <class Epi>
+static int grouped(const Fp8Rows& r, const uint8_t* a, const float* a_scale, int64_t ld, const yamoe_fp8_matrix_t& w, int N, int K,
+                   int E, const Epi& epi, cudaStream_t st) {
   Fp8Params p{};
   p.M = r.max_rows; p.N = N; p.K = K; p.B = E;
   p.sa = a_scale; p.sa_m = 1; p.sa_k = r.max_rows;
   p.sb = w.scale; p.sb_b = w.scale_batch; p.sb_n = w.scale_row; p.sb_k = w.scale_group;
-  p.tile_expert = pairs ? r.pair_expert : r.tile_expert;
-  p.tile_first = pairs ? r.pair_off : nullptr;
   p.pad_off = r.pad_off;
-  p.n_tiles = r.header + (pairs ? kHdrPairs : kHdrRowTiles);
+  p.n_tiles = r.header + kHdrRowTiles;
   p.status = const_cast<int32_t*>(r.header) + kHdrStatus;
-  return p;
-}
-
-template <class Epi>
-static int grouped(const Fp8Rows& r, const uint8_t* a, const float* a_scale, int64_t ld, const yamoe_fp8_matrix_t& w, int N, int K,
-                   int E, const Epi& epi, cudaStream_t st) {
-  const bool pairs = fp8_pairs(r, E);
-  const Fp8Params p = grouped_params(r, a_scale, w, N, K, E, pairs);
   const Fp8Operand A{a, r.max_rows, ld, 0}, B{w.q, N, w.ld, w.q_batch};
-  return pairs ? launch_fp8_gemm<2, 256, false, true>(A, B, p, epi, r.max_tiles, true, st)
-               : launch_fp8_gemm<1, 256, false, true>(A, B, p, epi, r.max_tiles, true, st);
+  return launch_fp8_gemm<256, false, true>(A, B, p, epi, r.max_tiles, true, st);
 }
 
 template <typename T>
@@ -85,19 +73,17 @@ YB_INSTANTIATE(float)
 YB_INSTANTIATE(__nv_bfloat16)
 #undef YB_INSTANTIATE
 
-// Tiles of a product: estimated clocks of each kind, the least of them.  A block takes a pair's 256 x 256 tile some 700 clocks, a
-// 128 x 256 tile as many (what L2 delivers to one SM), 128 x 128 450; a tile's beginning and end 3000; meeting in shared memory 1500 more.
-struct Fp8Choice { int cg, bn, splits; };
+// Tiles of a product: estimated clocks of each kind, the least of them.  A block takes a 128 x 256 tile some 1150 clocks, a 128 x 128
+// one 650; a tile's beginning and end 3000; meeting in shared memory 1500 more.
+struct Fp8Choice { int bn, splits; };
 static Fp8Choice choose_tiles(int64_t B, int64_t M, int64_t N, int64_t K) {
-  const int64_t kb = ceil_div(K, kFp8Group);
-  Fp8Choice best{2, 256, 1};
-  double least = (double)ceil_div(B * ceil_div(M, 256) * ceil_div(N, 256), kSMs / 2) * (double)(kb * 700 + 3000);
-  const double one = (double)ceil_div(B * ceil_div(M, 128) * ceil_div(N, 256), kSMs) * (double)(kb * 700 + 3000);
-  if (one < least) { least = one; best = Fp8Choice{1, 256, 1}; }
-  const int64_t tiles = B * ceil_div(M, 128) * ceil_div(N, 128);
+  const int64_t kb = ceil_div(K, kFp8Group), rows = B * ceil_div(M, 128);
+  Fp8Choice best{256, 1};
+  double least = (double)ceil_div(rows * ceil_div(N, 256), kSMs) * (double)(kb * 1150 + 3000);
   for (int s = 1; s <= kFp8MaxSplits && s <= kb; ++s) {
-    const double t = (double)ceil_div(tiles * s, kSMs) * (double)(ceil_div(kb, s) * 450 + 3000 + (s > 1 ? 1500 : 0));
-    if (t < least) { least = t; best = Fp8Choice{1, 128, s}; }
+    const double t =
+        (double)ceil_div(rows * ceil_div(N, 128) * s, kSMs) * (double)(ceil_div(kb, s) * 650 + 3000 + (s > 1 ? 1500 : 0));
+    if (t < least) { least = t; best = Fp8Choice{128, s}; }
   }
   return best;
 }
@@ -107,12 +93,11 @@ static int mm_impl(const Fp8Operand& A, const Fp8Operand& B, Fp8Params p, T* out
   const int vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.N * (int64_t)sizeof(T) % 16 == 0;
   const Fp8Store<T> epi{out, p.N, p.M * p.N, vec};
   const Fp8Choice c = choose_tiles(p.B, p.M, p.N, p.K);
-  p.MT = (int)ceil_div(p.M, 128 * c.cg);
+  p.MT = (int)ceil_div(p.M, 128);
   p.splits = c.splits;
   const int64_t tiles = (int64_t)p.B * p.MT;
-  if (c.cg == 2) return launch_fp8_gemm<2, 256, BROWS, false>(A, B, p, epi, tiles, false, st);
-  if (c.bn == 256) return launch_fp8_gemm<1, 256, BROWS, false>(A, B, p, epi, tiles, false, st);
-  return launch_fp8_gemm<1, 128, BROWS, false>(A, B, p, epi, tiles, false, st);
+  return c.bn == 256 ? launch_fp8_gemm<256, BROWS, false>(A, B, p, epi, tiles, false, st)
+                     : launch_fp8_gemm<128, BROWS, false>(A, B, p, epi, tiles, false, st);
 }
 
 }  // namespace yb

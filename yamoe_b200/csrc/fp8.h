@@ -17,12 +17,11 @@ int fp8_gather(const T* hidden, uint8_t* q, float* scale, int64_t ld, int64_t sc
 
 // The two grouped products of the expert pass over rows in the padded, expert-sorted layout.
 struct Fp8Rows {
-  const int32_t *pad_off, *pair_expert, *pair_off, *tile_expert;
-  const int32_t* header;        // row tiles, pairs of them, status
+  const int32_t* pad_off;
+  const int32_t* header;        // row tiles, status
   const int32_t *row_token, *row_flat;
   const float* row_weight;
   int64_t max_rows, max_tiles;
-  int64_t S;                    // assignments
 };
 template <typename T>
 int fp8_gate_up(const Fp8Rows& r, const uint8_t* x, const float* x_scale, int64_t ld, const yamoe_fp8_matrix_t& w, const T* bias,

@@ -3,7 +3,7 @@
 //   C[m, n] = sum over blocks kb of 128:  sa[m, kb] * sb[n, kb] * (sum over k in kb of qa[m, k] * qb[n, k])
 //
 // The inner sums are exact products accumulated in fp32 in TMEM; scales differ from block to block, so an accumulator
-// holds ONE block (four instructions of 128 or 256 x 128 x 32) and is then added, times its scales, to fp32 registers of
+// holds ONE block (four instructions of 128 x 256 x 32) and is then added, times its scales, to fp32 registers of
 // the warps that later write the tile.  A lane holds a row of C: with sb per 128 columns (weights) both scales are one
 // number per thread and accumulator, and the whole addition is one packed multiply-add for two elements.  With a scale per
 // row of B too (BROWS: weight gradients) the columns' scales go through shared memory.
@@ -13,12 +13,12 @@
 // per block and warp), a load of 32 columns is always on its way while those before it are added, across blocks too, and
 // the scales are brought to shared memory by a warp of their own, four blocks at a time.
 //
-// Both operands are K-major with 128-byte swizzle: a block of 128 is one swizzle row.  CG = 2: CTA pairs
-// (cta_group::2), 256 x 256 tiles of which each CTA stages 128 rows of either operand, 32 KB per block where a CTA
-// alone stages 48 for a tile of 128 x 256.  Few tiles: 128 x 128, and a cluster of up to four CTAs shares a tile's blocks
-// (split), the sums of the others meeting in the first one's shared memory, added in order.
+// Both operands are K-major with 128-byte swizzle: a block of 128 is one swizzle row.  A CTA has tiles of 128 x 256 (CTA pairs
+// with tiles of 256 x 256 were no faster, 150.5 and 151.2 us for 8192 x 5760 x 2880: L2's bytes are not what bounds it, and
+// tiles of 256 rows fit experts' rows less well).  Few tiles: 128 x 128, and a cluster of up to four CTAs shares a
+// tile's blocks (split), the sums of the others meeting in the first one's shared memory, added in order.
 //
-// Rows come as they are (`tile_expert` null: B matrices of M rows) or sorted by expert in the padded layout of the
+// Rows come as they are (B matrices of M rows) or (GROUPED) sorted by expert in the padded layout of the
 // expert pass, an expert's tiles following each other with the row tile varying fastest.
 //
 // Every wait is bounded as in umma_gemm.cuh.  A warp whose wait gave up walks on through the remaining tiles without
@@ -42,14 +42,12 @@ constexpr int kFp8FewRegs = 40, kFp8ManyRegs = 232;
 struct Fp8Params {
   int64_t M, N;                 // rows per matrix (not grouped), columns
   int K, B;                     // reduction length, matrices
-  int MT, NT;                   // tiles of 128 * CG rows (not grouped), of BN columns
+  int MT, NT;                   // tiles of 128 rows (not grouped), of BN columns
   const float* sa;              // scale of (matrix b, row m, block kb) at b * sa_b + m * sa_m + kb * sa_k
   const float* sb;              // of (matrix b, row or 128-row block n, block kb)
   int64_t sa_b, sa_m, sa_k, sb_b, sb_n, sb_k;
   // grouped
-  const int32_t* tile_expert;   // expert of every tile of 128 * CG rows
-  const int32_t* tile_first;    // [E + 1] prefix sums of those tiles; null: pad_off / 128
-  const int32_t* pad_off;       // [E + 1]
+  const int32_t* pad_off;       // [E + 1] first padded row of each expert, in tiles of 128 rows
   const int32_t* n_tiles;       // how many there are
   int32_t* status;              // device status word
   int clear_status;             // no earlier kernel of the call has set it to 0
@@ -60,12 +58,12 @@ constexpr int kFp8MaxSplits = 4;
 constexpr int kFp8ScaleBlocks = 4, kFp8ScaleSlots = 2;     // blocks of 128 whose scales come together, such groups on their way
 constexpr int kFp8ParkBytes = 32 * 64;                     // per epilogue warp: 64 bytes of each of its rows
 
-template <int CG, int BN, bool BROWS>
+template <int BN, bool BROWS>
 struct Fp8Smem {
   static constexpr int kABytes = 128 * 128;
-  static constexpr int kBBytes = BN / CG * 128;
+  static constexpr int kBBytes = BN * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 196608 / kStageBytes;     // 4 (one CTA, 256 columns) or 6
+  static constexpr int kStages = 196608 / kStageBytes;     // 4 (256 columns) or 6
   static_assert(kStages * kStageBytes >= (kFp8MaxSplits - 1) * 128 * 128 * 4, "the sums of the others of a cluster");
   static constexpr int kScaleFloats = 128 + (BROWS ? BN : 4);                    // of a block: rows, columns or column blocks
   static constexpr int kPark = kStages * kStageBytes;                            // from the 1024-byte boundary on
@@ -74,18 +72,11 @@ struct Fp8Smem {
 };
 inline int fp8_smem_bytes(int tables, int experts) { return tables + (experts > 0 ? 2 * (experts + 1) * 4 : 0); }
 
-template <int CG>
 __device__ __forceinline__ void tc_mma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (CG == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
   uint64_t r;
@@ -121,26 +112,21 @@ struct Fp8Tile {
   bool ok;             // false: take part in barriers only
 };
 
-template <int CG, int BN, bool BROWS, bool GROUPED, class Epi>
+template <int BN, bool BROWS, bool GROUPED, class Epi>
 __global__ void __launch_bounds__(kFp8Threads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Fp8Params p,
                 const Epi epi) {
-  using SM = Fp8Smem<CG, BN, BROWS>;
+  using SM = Fp8Smem<BN, BROWS>;
   constexpr int kStages = SM::kStages, kAccs = 512 / BN, kCols = BN / 2;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[kStages];       // CG = 2: used in the leader CTA
-  __shared__ __align__(8) uint64_t bar_empty[kStages];      // per CTA
-  __shared__ __align__(8) uint64_t bar_tmem_full[kAccs];       // per CTA
-  __shared__ __align__(8) uint64_t bar_tmem_empty[kAccs];      // CG = 2: used in the leader CTA
+  __shared__ __align__(8) uint64_t bar_full[kStages], bar_empty[kStages], bar_tmem_full[kAccs], bar_tmem_empty[kAccs];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
   __shared__ __align__(8) uint64_t bar_scale_full[kFp8ScaleSlots], bar_scale_empty[kFp8ScaleSlots];
   __shared__ typename Epi::Shared s_epi;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
-  const bool leader = rank == 0;
-  const int splits = CG == 1 && BN == 128 && !GROUPED ? p.splits : 1;
+  const int splits = BN == 128 && !GROUPED ? p.splits : 1;
   const int part = splits > 1 ? (int)cluster_ctarank() : 0;       // of the tile's blocks
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const aligned = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -150,12 +136,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(smem_u32(&bar_full[s]), CG);
+      mbar_init(smem_u32(&bar_full[s]), 1);
       mbar_init(smem_u32(&bar_empty[s]), 1);
     }
     for (int a = 0; a < kAccs; ++a) {
       mbar_init(smem_u32(&bar_tmem_full[a]), 1);
-      mbar_init(smem_u32(&bar_tmem_empty[a]), CG * kFp8EpiWarps);
+      mbar_init(smem_u32(&bar_tmem_empty[a]), kFp8EpiWarps);
     }
     for (int i = 0; i < kFp8ScaleSlots; ++i) {
       mbar_init(smem_u32(&bar_scale_full[i]), 32);
@@ -165,19 +151,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    if constexpr (CG == 1) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                   ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    } else {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
-                   ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
-      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    }
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (CG == 2) cluster_sync_all();     // the peer's barriers exist before any remote signal is sent
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_slot;
   pdl_trigger();
@@ -185,13 +164,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   if constexpr (GROUPED) {
     for (int i = threadIdx.x; i <= p.B; i += kFp8Threads) {
       s_pad[i] = p.pad_off[i];
-      s_first[i] = p.tile_first != nullptr ? p.tile_first[i] : p.pad_off[i] / kTileM;
+      s_first[i] = p.pad_off[i] / kTileM;
     }
     __syncthreads();
   }
   if (p.clear_status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = kStatusOk;   // waits give up after seconds at the earliest
   const int64_t total = GROUPED ? (int64_t)*after_wait(p.n_tiles) * p.NT : (int64_t)p.B * p.MT * p.NT;
-  const int64_t first_id = blockIdx.x / (CG * splits), n_workers = gridDim.x / (CG * splits);
+  const int64_t first_id = blockIdx.x / splits, n_workers = gridDim.x / splits;
   const int kblocks_all = (p.K + kFp8Group - 1) / kFp8Group;
   const int kb_first = part * kblocks_all / splits, kb_end = (part + 1) * kblocks_all / splits;
 
@@ -208,14 +187,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       const int cnt = s_first[b + 1] - s_first[b];
       const int local = (int)(id - (int64_t)s_first[b] * p.NT);
       const int nt = local / cnt;
-      m0 = s_pad[b] + (int64_t)(local - nt * cnt) * (kTileM * CG);
+      m0 = s_pad[b] + (int64_t)(local - nt * cnt) * kTileM;
       n0 = nt * BN;
     } else {
       const int64_t per = (int64_t)p.MT * p.NT;
       b = (int)(id / per);
       const int64_t local = id - b * per;
       const int nt = (int)(local / p.MT);
-      m0 = (local - (int64_t)nt * p.MT) * (kTileM * CG);
+      m0 = (local - (int64_t)nt * p.MT) * kTileM;
       n0 = nt * BN;
     }
   };
@@ -223,7 +202,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   if (warp < kFp8FirstEpiWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp8FewRegs));
     if (warp == 0) {
-      // =========================== TMA producer (of each CTA) ==================================
+      // =========================== TMA producer ================================================
       const bool elected = elect_one();
       int stage = 0;
       uint32_t phase = 0;
@@ -232,24 +211,15 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         int b, n0;
         int64_t m0;
         decode(id, b, m0, n0);
-        const int width = min(BN, ((int)p.N - n0 + 15) & ~15);
-        const int am = (int)m0 + (int)rank * 128, bn = n0 + (int)rank * (width / CG);
         for (int kb = kb_first; kb < kb_end; ++kb) {
           ok = mbar_wait_warp(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag);
           if (!ok) break;
           if (elected) {
             const uint32_t sa = smem_base + stage * SM::kStageBytes;
-            if constexpr (CG == 1) {
-              const uint32_t full = smem_u32(&bar_full[stage]);
-              mbar_expect_tx(full, SM::kStageBytes);
-              tma_load_3d(sa, &tmA, kb * kFp8Group, am, GROUPED ? 0 : b, full);
-              tma_load_3d(sa + SM::kABytes, &tmB, kb * kFp8Group, bn, b, full);
-            } else {
-              const uint32_t full = mapa_u32(smem_u32(&bar_full[stage]), 0);
-              mbar_expect_tx_cluster(full, SM::kStageBytes);
-              tma2_load_3d(sa, &tmA, kb * kFp8Group, am, GROUPED ? 0 : b, full);
-              tma2_load_3d(sa + SM::kABytes, &tmB, kb * kFp8Group, bn, b, full);
-            }
+            const uint32_t full = smem_u32(&bar_full[stage]);
+            mbar_expect_tx(full, SM::kStageBytes);
+            tma_load_3d(sa, &tmA, kb * kFp8Group, (int)m0, GROUPED ? 0 : b, full);
+            tma_load_3d(sa + SM::kABytes, &tmB, kb * kFp8Group, n0, b, full);
           }
           __syncwarp();
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
@@ -264,52 +234,45 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       }
       __syncwarp();
     } else if (warp == 1) {
-      // =========================== MMA issuer (of the leader) ==================================
-      if (leader) {
-        const uint32_t idesc_base = (1u << 4) | ((uint32_t)(128 * CG >> 4) << 24);   // e4m3 x e4m3 -> fp32, both K-major
-        const uint64_t adesc0 = make_smem_desc(smem_base, 16, 1024);
-        const uint64_t bdesc0 = make_smem_desc(smem_base + SM::kABytes, 16, 1024);
-        const bool elected = elect_one();
-        int stage = 0, acc = 0;
-        uint32_t phase = 0, acc_phase = 0;
-        bool ok = true;
-        for (int64_t id = first_id; id < total && ok; id += n_workers) {
-          int b, n0;
-          int64_t m0;
-          decode(id, b, m0, n0);
-          const uint32_t idesc = idesc_base | ((uint32_t)(min(BN, ((int)p.N - n0 + 15) & ~15) >> 3) << 17);
-          for (int kb = kb_first; kb < kb_end; ++kb) {
-            ok = mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &abort_flag);
-            if (ok) ok = mbar_wait_warp(smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, &abort_flag);
-            if (!ok) break;
-            tc_fence_after();
-            if (elected) {
-              const uint64_t adesc = adesc0 + (uint64_t)(stage * (SM::kStageBytes >> 4));
-              const uint64_t bdesc = bdesc0 + (uint64_t)(stage * (SM::kStageBytes >> 4));
+      // =========================== MMA issuer ==================================================
+      const uint32_t idesc_base = (1u << 4) | ((uint32_t)(128 >> 4) << 24);   // e4m3 x e4m3 -> fp32, both K-major
+      const uint64_t adesc0 = make_smem_desc(smem_base, 16, 1024);
+      const uint64_t bdesc0 = make_smem_desc(smem_base + SM::kABytes, 16, 1024);
+      const bool elected = elect_one();
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int64_t id = first_id; id < total && ok; id += n_workers) {
+        int b, n0;
+        int64_t m0;
+        decode(id, b, m0, n0);
+        const uint32_t idesc = idesc_base | ((uint32_t)(min(BN, ((int)p.N - n0 + 15) & ~15) >> 3) << 17);
+        for (int kb = kb_first; kb < kb_end; ++kb) {
+          ok = mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &abort_flag);
+          if (ok) ok = mbar_wait_warp(smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, &abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (elected) {
+            const uint64_t adesc = adesc0 + (uint64_t)(stage * (SM::kStageBytes >> 4));
+            const uint64_t bdesc = bdesc0 + (uint64_t)(stage * (SM::kStageBytes >> 4));
 #pragma unroll
-              for (int k = 0; k < kFp8Group / 32; ++k)
-                tc_mma_fp8<CG>(tmem_base + acc * BN, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, (uint32_t)(k != 0));
-              if constexpr (CG == 1) {
-                tc_commit(smem_u32(&bar_tmem_full[acc]));
-                tc_commit(smem_u32(&bar_empty[stage]));
-              } else {
-                tc2_commit_pair(smem_u32(&bar_tmem_full[acc]));
-                tc2_commit_pair(smem_u32(&bar_empty[stage]));
-              }
-            }
-            __syncwarp();
-            if (++stage == kStages) { stage = 0; phase ^= 1u; }
-            if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
+            for (int k = 0; k < kFp8Group / 32; ++k)
+              tc_mma_fp8(tmem_base + acc * BN, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, (uint32_t)(k != 0));
+            tc_commit(smem_u32(&bar_tmem_full[acc]));
+            tc_commit(smem_u32(&bar_empty[stage]));
           }
+          __syncwarp();
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
         }
-        if (!ok && lane == 0) {
-          abort_flag = 1;
-          atomicMax(p.status, (int)kStatusMmaTimeout);
-        }
+      }
+      if (!ok && lane == 0) {
+        abort_flag = 1;
+        atomicMax(p.status, (int)kStatusMmaTimeout);
       }
       __syncwarp();
     } else if (warp == 2) {
-      // =========================== scales (of each CTA) ========================================
+      // =========================== scales ======================================================
       // Four bytes at a time, each on its way by itself; rows and columns that do not exist are 0.
       int slot = 0;
       uint32_t phase = 0;
@@ -318,7 +281,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         int b, n0;
         int64_t m0;
         decode(id, b, m0, n0);
-        const int64_t row0 = m0 + rank * 128, row_end = GROUPED ? (int64_t)s_pad[b + 1] : p.M;
+        const int64_t row0 = m0, row_end = GROUPED ? (int64_t)s_pad[b + 1] : p.M;
         const float* sa = p.sa + (GROUPED ? 0 : b * p.sa_b);
         const float* sb = p.sb + b * p.sb_b;
         for (int kb = kb_first; kb < kb_end; kb += kFp8ScaleBlocks) {
@@ -355,7 +318,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFp8ManyRegs));
-    // =========================== scaled sums and epilogue (warps 4 .. 11 of each CTA) ========
+    // =========================== scaled sums and epilogue (warps 4 .. 11) ====================
     const int q = warp & 3;                      // TMEM lane quarter this warp may read
     const int half = (warp - kFp8FirstEpiWarp) >> 2;      // its columns: kCols from half * kCols on
     const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + half * kCols;
@@ -367,7 +330,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       int n0;
       int64_t m0;
       decode(id, t.b, m0, n0);
-      t.row = m0 + rank * 128 + q * 32 + lane;
+      t.row = m0 + q * 32 + lane;
       t.row_end = GROUPED ? (int64_t)s_pad[t.b + 1] : p.M;
       t.n0 = n0 + half * kCols;
       t.n_end = (int)p.N;
@@ -407,8 +370,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
               tc_fence_before();
               __syncwarp();
               if (lane == 0) {
-                if constexpr (CG == 1) mbar_arrive(smem_u32(&bar_tmem_empty[acc]));
-                else mbar_arrive_cluster(mapa_u32(smem_u32(&bar_tmem_empty[acc]), 0));
+                mbar_arrive(smem_u32(&bar_tmem_empty[acc]));
               }
               if (!last) {
                 if (!__all_sync(0xffffffffu, early != 0)) ok = mbar_wait_warp(smem_u32(&bar_tmem_full[next]), next_phase, &abort_flag);
@@ -439,7 +401,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         }
       }
       t.ok = ok;
-      if constexpr (CG == 1 && BN == 128 && !GROUPED) {
+      if constexpr (BN == 128 && !GROUPED) {
         if (splits > 1) {
           // [part - 1][column of the tile][row]: a warp stores 128 contiguous bytes
           const int row = q * 32 + lane;
@@ -490,13 +452,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
     __syncthreads();
   }
-  if constexpr (CG == 2) cluster_sync_all();     // neither CTA releases what the pair may still use
   if (warp == 1) {
     tc_fence_after();
-    if constexpr (CG == 1)
-      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
-    else
-      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
   }
 }
 
@@ -674,34 +632,15 @@ struct Fp8WeightedRows {
 // Host side
 // ---------------------------------------------------------------------------------------------
 
-// CTAs (CG = 1) or CTA pairs that run at the same time, asked once per kernel and device
-template <int CG, typename... KArgs>
-inline int fp8_resident(void (*kern)(KArgs...), PerDevice<int>& known) {
+// Prepares a kernel for its shared memory, once per kernel and device
+template <typename... KArgs>
+inline bool fp8_configure(void (*kern)(KArgs...), PerDevice<int>& done) {
   const int dev = current_device_index();
-  int n = known.get(dev);
-  if (n > 0) return n;
+  if (done.get(dev)) return true;
   constexpr int kMost = 227 * 1024 - 3072;     // static shared memory beside it
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess) return 0;
-  if (CG == 1) {
-    n = umma_sm_count();
-  } else {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(umma_sm_count() & ~1);
-    cfg.blockDim = dim3(kFp8Threads);
-    cfg.dynamicSmemBytes = kMost;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CG;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
-      (void)cudaGetLastError();
-      n = umma_sm_count() / CG;
-    }
-  }
-  known.set(dev, n);
-  return n;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess) return false;
+  done.set(dev, 1);
+  return true;
 }
 
 struct Fp8Operand {
@@ -709,36 +648,35 @@ struct Fp8Operand {
   int64_t rows, ld, batch;      // rows per matrix, pitch, distance of matrices (bytes)
 };
 
-// `max_tiles`: row tiles of 128 * CG rows in all
-template <int CG, int BN, bool BROWS, bool GROUPED, class Epi>
+// `max_tiles`: row tiles of 128 rows in all
+template <int BN, bool BROWS, bool GROUPED, class Epi>
 inline int launch_fp8_gemm(const Fp8Operand& a, const Fp8Operand& b, Fp8Params p, const Epi& epi, int64_t max_tiles, bool pdl,
                            cudaStream_t st) {
   if (!umma_available()) return YAMOE_ERR_UNSUPPORTED;
-  using SM = Fp8Smem<CG, BN, BROWS>;
+  using SM = Fp8Smem<BN, BROWS>;
   CUtensorMap tmA, tmB;
   const uint64_t na = GROUPED ? 1 : (uint64_t)p.B;
   const uint64_t da[3] = {(uint64_t)p.K, (uint64_t)a.rows, na}, db[3] = {(uint64_t)p.K, (uint64_t)b.rows, (uint64_t)p.B};
   const uint64_t ga[2] = {(uint64_t)a.ld, (uint64_t)(na > 1 ? a.batch : a.ld)};
   const uint64_t gb[2] = {(uint64_t)b.ld, (uint64_t)(p.B > 1 ? b.batch : b.ld)};
-  const uint32_t boxa[3] = {128, 128, 1}, boxb[3] = {128, BN / CG, 1};
+  const uint32_t boxa[3] = {128, 128, 1}, boxb[3] = {128, BN, 1};
   if (!encode_map(&tmA, a.q, 3, da, ga, boxa, kMapU8) || !encode_map(&tmB, b.q, 3, db, gb, boxb, kMapU8)) return YAMOE_ERR_CUDA;
-  auto kern = fp8_gemm_kernel<CG, BN, BROWS, GROUPED, Epi>;
-  static PerDevice<int> resident;    // per template instantiation and device
-  const int workers = fp8_resident<CG>(kern, resident);
-  if (workers <= 0) return YAMOE_ERR_CUDA;
+  auto kern = fp8_gemm_kernel<BN, BROWS, GROUPED, Epi>;
+  static PerDevice<int> configured;    // per template instantiation and device
+  if (!fp8_configure(kern, configured)) return YAMOE_ERR_CUDA;
   p.NT = (int)ceil_div(p.N, BN);
   const int64_t total = max_tiles * p.NT;
   if (total <= 0) return YAMOE_OK;
-  const bool split = CG == 1 && BN == 128 && !GROUPED && p.splits > 1;
+  const bool split = BN == 128 && !GROUPED && p.splits > 1;
   if (!split) p.splits = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(split ? p.splits * total : CG * std::min<int64_t>(total, workers)));
+  cfg.gridDim = dim3((unsigned)(split ? p.splits * total : std::min<int64_t>(total, umma_sm_count())));
   cfg.blockDim = dim3(kFp8Threads);
   cfg.dynamicSmemBytes = (size_t)fp8_smem_bytes(SM::kTables, GROUPED ? p.B : 0);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CG * p.splits;
+  attr[0].val.clusterDim.x = p.splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled(pdl) ? 1 : 0;

@@ -369,8 +369,7 @@ static int experts_fp8_impl(const void* hidden, const int64_t* ridx, const void*
     rc = fp8_gather<T>(reinterpret_cast<const T*>(hidden), p.x, p.x_scale, p.ld, p.t.max_rows, rt.flat_row, Tn, H, K, st);
   }
   if (rc) return rc;
-  const Fp8Rows rows{rt.pad_off, rt.pair_expert, rt.pair_off, rt.tile_expert, rt.header, rt.row_token, rt.row_flat, rt.row_weight,
-                     p.t.max_rows, p.t.max_tiles, p.t.S};
+  const Fp8Rows rows{rt.pad_off, rt.header, rt.row_token, rt.row_flat, rt.row_weight, p.t.max_rows, p.t.max_tiles};
   {
     StageTimer tm(kStageGateUp, st);
     rc = fp8_gate_up<T>(rows, p.x, p.x_scale, p.ld, gate_up, reinterpret_cast<const T*>(bgu), p.act, p.act_scale, H, E, st);
