@@ -6,9 +6,11 @@
 //                         grid barrier, down, grid barrier, weighted sum of a token's K rows in slot order
 //
 // Bound by HBM where the weights of the experts hit exceed some 50 MB, by latency below.  What carries it:
-//  * The weights do not depend on anything but the routing, so one warp streams the CTA's tiles of 16 KB through a ring (TMA,
-//    192 KB in flight per SM), on across units and across the grid barrier: HBM works through the ends of units, and when
-//    the activations are ready the first third of the down weights of a token already lies in shared memory.
+//  * The weights do not depend on anything but the routing, so one warp streams the CTA's tiles of 32 KB through a ring (TMA,
+//    128 KB in flight per SM; half of that is as fast), on across units and across the grid barrier: HBM works through the
+//    ends of units, and when the activations are ready the first down weights already lie in shared memory.  The rows that
+//    meet a tile come with it, by bulk copies (those of the first down tiles after the barrier); read from global memory by
+//    each of the eight warps they took 40 of 197 us with 16 tokens.
 //  * A unit is 128 output columns of one expert with the whole reduction, 16 columns to each of eight warps: no sums
 //    cross warps (split along the reduction instead, a warp's tiles for itself, they took as long to come together as
 //    the products).
@@ -34,11 +36,15 @@ namespace yb {
 
 constexpr int kLayerMaxT = 32, kLayerMaxS = 256, kLayerMaxK = 32;
 constexpr int kLayerWarps = 8, kLayerThreads = 32 * (kLayerWarps + 1);     // one to issue the copies
-constexpr int kLayerTileBytes = 16384, kLayerStages = 12;
+constexpr int kLayerTileBytes = 32768, kLayerStages = 4;           // a tile: two halves along the reduction
 constexpr int kLayerUnit = 16 * kLayerWarps;                       // output columns of a unit
 constexpr int kLayerParts = 4;                                     // owners of a unit, at most
 constexpr int kLayerRows = 16;                                     // rows of an expert that share a pass over its weights
-constexpr int kLayerSmem = kLayerStages * kLayerTileBytes + 1024;
+// Rows of a tile in shared memory: 16 of 256 fp32 or 16-bit values, or 32 of 128 bf16; 16 bytes more than that apart, so that the
+// rows that eight lanes read lie on different banks
+constexpr int kLayerRowBytes = kLayerRows * (256 * 4 + 16);
+constexpr int kLayerStageRows = kLayerStages * kLayerTileBytes;    // where they begin
+constexpr int kLayerSmem = kLayerStages * (kLayerTileBytes + kLayerRowBytes) + 1024;
 constexpr int kRouterWarps = 8, kRouterThreads = 32 * kRouterWarps;
 constexpr int kLayerStatusBarrier = 8;                             // device status: a grid barrier gave up
 
@@ -194,57 +200,43 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
 template <bool FP8>
 __device__ __forceinline__ int layer_m_row(int g) { return FP8 ? (g >> 1) + 4 * (g & 1) : g; }
 
-// A tile of weights: e4m3 128 rows (output columns) of 128 reduction bytes; bf16 two halves of 64 reduction rows of 64 output
-// columns.  What a lane holds of the rows that it multiplies, 8 * NT of them, for one tile:
+// Half a tile of weights: e4m3 128 rows (output columns) of 128 reduction bytes; bf16 twice 64 reduction rows of 64 output
+// columns.  The operands that a lane holds of the rows that it multiplies, 8 * NT of them, for one half: `row`, the
+// shared memory address of the lane's row of the first eight at the half's first reduction index, the next eight 8 * pitch
+// further.  Rows that do not exist are not defined, nor is what is computed of them.
 template <bool FP8, bool F32, int NT>
-struct LayerRows {
-  static constexpr int kWords = FP8 ? (F32 ? 8 : 4) : 2;      // of 16 bytes, per eight rows
-  uint4 q[NT][kWords];
-
-  // rows[n]: the lane's row of n-tile n at the tile's first reduction index, or null
-  __device__ __forceinline__ void load(const uint8_t* const (&rows)[NT], int c) {
+__device__ __forceinline__ void layer_rows(uint32_t row, uint32_t pitch, int c, const float (&factor)[NT], uint4 (&b)[NT][FP8 ? 4 : 2]) {
+  auto ld16 = [](uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+  };
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+  for (int n = 0; n < NT; ++n) {
+    const uint32_t at = row + n * 8 * pitch;
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) q[n][i] = make_uint4(0, 0, 0, 0);
-      if (rows[n] == nullptr) continue;
-      if constexpr (FP8) {               // 16 neighbours out of each 64 reduction indices
-        constexpr int kBytes = F32 ? 4 : 2, kHalf = kWords / 2;
-#pragma unroll
-        for (int i = 0; i < kWords; ++i)
-          q[n][i] = *reinterpret_cast<const uint4*>(rows[n] + (64 * (i / kHalf) + 16 * c) * kBytes + 16 * (i % kHalf));
-      } else {                           // four neighbours out of each 16
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint2 lo = *reinterpret_cast<const uint2*>(rows[n] + (32 * i + 4 * c) * 2);
-          const uint2 hi = *reinterpret_cast<const uint2*>(rows[n] + (32 * i + 16 + 4 * c) * 2);
-          q[n][i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-        }
+    for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
+      if constexpr (F32) {                 // 16 neighbours out of each 64 reduction indices, eight at a time
+        const uint4 u = ld16(at + (64 * (i >> 1) + 16 * c) * 4 + 32 * (i & 1)), v = ld16(at + (64 * (i >> 1) + 16 * c) * 4 + 32 * (i & 1) + 16);
+        const float f = factor[n];
+        const __half2 h[4] = {__floats2half2_rn(__uint_as_float(u.x) * f, __uint_as_float(u.y) * f),
+                              __floats2half2_rn(__uint_as_float(u.z) * f, __uint_as_float(u.w) * f),
+                              __floats2half2_rn(__uint_as_float(v.x) * f, __uint_as_float(v.y) * f),
+                              __floats2half2_rn(__uint_as_float(v.z) * f, __uint_as_float(v.w) * f)};
+        b[n][i] = *reinterpret_cast<const uint4*>(h);
+      } else if constexpr (FP8) {
+        b[n][i] = ld16(at + (64 * (i >> 1) + 16 * c) * 2 + 16 * (i & 1));
+      } else {                             // four neighbours out of each 16
+        uint2 lo, hi;
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(lo.x), "=r"(lo.y) : "r"(at + (32 * i + 4 * c) * 2));
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(hi.x), "=r"(hi.y) : "r"(at + (32 * i + 16 + 4 * c) * 2));
+        b[n][i] = make_uint4(lo.x, lo.y, hi.x, hi.y);
       }
     }
   }
-  // 16-bit operands; `factor` of fp32 rows
-  __device__ __forceinline__ void operands(const float (&factor)[NT], uint4 (&b)[NT][FP8 ? 4 : 2]) const {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < (FP8 ? 4 : 2); ++i) {
-        if constexpr (F32) {
-          const uint4 u = q[n][2 * i], v = q[n][2 * i + 1];
-          const float f = factor[n];
-          const __half2 h[4] = {__floats2half2_rn(__uint_as_float(u.x) * f, __uint_as_float(u.y) * f),
-                                __floats2half2_rn(__uint_as_float(u.z) * f, __uint_as_float(u.w) * f),
-                                __floats2half2_rn(__uint_as_float(v.x) * f, __uint_as_float(v.y) * f),
-                                __floats2half2_rn(__uint_as_float(v.z) * f, __uint_as_float(v.w) * f)};
-          b[n][i] = *reinterpret_cast<const uint4*>(h);
-        } else {
-          b[n][i] = q[n][i];
-        }
-      }
-  }
-};
+}
 
-// acc += the warp's 16 output columns of the tile times up to 8 * NT rows
+// acc += the warp's 16 output columns of half a tile times up to 8 * NT rows
 template <bool FP8, int NT>
 __device__ __forceinline__ void layer_tile(uint32_t tile, int w, int lane, const uint4 (&b)[NT][FP8 ? 4 : 2], float scale,
                                            float (&acc)[NT][4]) {
@@ -411,9 +403,9 @@ __device__ __forceinline__ int layer_top_k_many(const float* logits, int E, int 
 template <bool FP8>
 __global__ void __launch_bounds__(kLayerThreads, 1)
 layer_experts_kernel(const __grid_constant__ CUtensorMap tm_gu, const __grid_constant__ CUtensorMap tm_dn, const LayerArgs a) {
-  constexpr int kTileK = FP8 ? 128 : 64;
+  constexpr int kHalfK = FP8 ? 128 : 64, kTileK = 2 * kHalfK;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[kLayerStages], bar_empty[kLayerStages];
+  __shared__ __align__(8) uint64_t bar_full[kLayerStages], bar_empty[kLayerStages], bar_act;
   __shared__ int16_t s_e[kLayerMaxS], s_sorted[kLayerMaxS], s_slot_e[kLayerMaxS], s_slot_first[kLayerMaxS + 1], s_slot[kLayerMaxS];
   __shared__ float s_w[kLayerMaxS], s_xs[kLayerMaxT];              
   __shared__ int s_scan[2][kLayerWarps + 1];
@@ -434,6 +426,7 @@ layer_experts_kernel(const __grid_constant__ CUtensorMap tm_gu, const __grid_con
       mbar_init(smem_u32(&bar_full[i]), 1);
       mbar_init(smem_u32(&bar_empty[i]), kLayerWarps);
     }
+    mbar_init(smem_u32(&bar_act), 1);
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -531,14 +524,31 @@ layer_experts_kernel(const __grid_constant__ CUtensorMap tm_gu, const __grid_con
   if (w == kLayerWarps) {
     // ---- the copies, through both phases ----------------------------------------------------------------------------------
     auto copy = [&](const CUtensorMap& map, uint32_t dst, int n, int kt, int e, uint32_t bar) {
-      if constexpr (FP8) {
-        tma_load_3d(dst, &map, kt * kTileK, n * kLayerUnit, e, bar);
-      } else {
-        tma_load_3d(dst, &map, n * kLayerUnit, kt * kTileK, e, bar);
-        tma_load_3d(dst + kLayerTileBytes / 2, &map, n * kLayerUnit + 64, kt * kTileK, e, bar);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = kt * kTileK + h * kHalfK;
+        if constexpr (FP8) {
+          tma_load_3d(dst + h * (kLayerTileBytes / 2), &map, k, n * kLayerUnit, e, bar);
+        } else {
+          tma_load_3d(dst + h * (kLayerTileBytes / 2), &map, n * kLayerUnit, k, e, bar);
+          tma_load_3d(dst + h * (kLayerTileBytes / 2) + kLayerTileBytes / 4, &map, n * kLayerUnit + 64, k, e, bar);
+        }
       }
     };
-    const bool elected = elect_one();
+    // The rows of slot `slot` that meet reduction tile kt, a lane's one or two of them, to the stage whose bytes they are part of
+    auto row_bytes = [&](int i, int kt) { return (uint32_t)min(kTileK, a.Hp - kt * kTileK) * (FP8 && i == 1 ? 4u : 2u); };
+    auto copy_rows = [&](int i, int slot, int kt, int stage) {
+      const bool pairs = i == 1 && !FP8;
+      const int first = s_slot_first[slot], n_rows = s_slot_first[slot + 1] - first, size = FP8 && i == 1 ? 4 : 2;
+      if (lane < (pairs ? 2 * n_rows : n_rows)) {
+        const int p = s_sorted[first + (pairs ? lane >> 1 : lane)];
+        const uint16_t* row = i == 0 ? a.xh + (int64_t)(p / a.K) * a.Hp : a.act + (int64_t)(2 * p + (pairs ? lane & 1 : 0)) * a.Hp;
+        const void* src = reinterpret_cast<const uint8_t*>(row) + (int64_t)kt * kTileK * size;
+        const uint32_t dst = ring + kLayerStageRows + stage * kLayerRowBytes + lane * (kTileK * size + 16);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     ::"r"(dst), "l"(src), "r"(row_bytes(i, kt)), "r"(smem_u32(&bar_full[stage])) : "memory");
+      }
+    };
     bool ok = true;
     int stage = 0;
     uint32_t phase = 0;
@@ -546,22 +556,40 @@ layer_experts_kernel(const __grid_constant__ CUtensorMap tm_gu, const __grid_con
       const int begin = i == 0 ? b0 : b1, end = i == 0 ? e0 : e1;
       const int units_n = i == 0 ? up.units_n : dn.units_n, first_unit = begin / kt_n;
       int kt = begin - first_unit * kt_n, slot = first_unit / units_n, n = first_unit - slot * units_n;
-      int e = begin < end ? s_slot_e[slot] : 0;
-      for (int g = begin; g < end; ++g) {
+      // of the second phase a ring of weights goes out before the activations are there, their rows after
+      int r_kt = kt, r_slot = slot, r_n = n, r_stage = stage, behind = 0;
+      auto step = [&](int& k, int& s_, int& n_) {
+        if (++k == kt_n) {
+          k = 0;
+          if (++n_ == units_n) { n_ = 0; ++s_; }
+        }
+      };
+      bool there = i == 0;
+      for (int g = begin; g < end || (ok && behind > 0); ++g) {
+        if (!there && (g >= end || behind == kLayerStages)) {
+          ok = mbar_wait_warp(smem_u32(&bar_act), 0, &abort_flag);
+          if (!ok) break;
+          asm volatile("fence.proxy.async;" ::: "memory");       // written by ordinary stores, read by copies
+          for (; behind > 0; --behind) {
+            copy_rows(i, r_slot, r_kt, r_stage);
+            step(r_kt, r_slot, r_n);
+            if (++r_stage == kLayerStages) r_stage = 0;
+          }
+          there = true;
+          if (g >= end) break;
+        }
         ok = mbar_wait_warp(smem_u32(&bar_empty[stage]), phase ^ 1u, &abort_flag);
         if (!ok) break;
-        if (elected) {
-          const uint32_t bar = smem_u32(&bar_full[stage]), dst = ring + stage * kLayerTileBytes;
-          mbar_expect_tx(bar, kLayerTileBytes);
-          if (i == 0) copy(tm_gu, dst, n, kt, e, bar); else copy(tm_dn, dst, n, kt, e, bar);
+        const uint32_t bar = smem_u32(&bar_full[stage]), dst = ring + stage * kLayerTileBytes;
+        const int rows = (s_slot_first[slot + 1] - s_slot_first[slot]) * (i == 1 && !FP8 ? 2 : 1);
+        if (lane == 0) {
+          mbar_expect_tx(bar, kLayerTileBytes + rows * row_bytes(i, kt));
+          if (i == 0) copy(tm_gu, dst, n, kt, s_slot_e[slot], bar); else copy(tm_dn, dst, n, kt, s_slot_e[slot], bar);
         }
         __syncwarp();
+        if (there) copy_rows(i, slot, kt, stage); else ++behind;
+        step(kt, slot, n);
         if (++stage == kLayerStages) { stage = 0; phase ^= 1u; }
-        if (++kt == kt_n) {
-          kt = 0;
-          if (++n == units_n) { n = 0; ++slot; }
-          if (g + 1 < end) e = s_slot_e[slot];
-        }
       }
     }
     if (!ok && lane == 0) {
@@ -575,7 +603,7 @@ layer_experts_kernel(const __grid_constant__ CUtensorMap tm_gu, const __grid_con
     // long as all tiles in flight take, some 4 us.
     for (int i = 0; i < 2; ++i) {
       const int begin = i == 0 ? b0 : b1, end = i == 0 ? e0 : e1, N = i == 0 ? 2 * a.H : a.H;
-      const int units_n = i == 0 ? up.units_n : dn.units_n, per_unit = 2 + (FP8 ? kt_n : 0);
+      const int units_n = i == 0 ? up.units_n : dn.units_n, per_unit = 2 + (FP8 ? (a.H + 127) / 128 : 0);
       if (begin == end) continue;
       const int u0 = begin / kt_n, asks = ((end - 1) / kt_n - u0 + 1) * per_unit;
       for (int j = tid; j < asks; j += 32 * kLayerWarps) {
@@ -594,8 +622,10 @@ layer_experts_kernel(const __grid_constant__ CUtensorMap tm_gu, const __grid_con
     uint32_t full_phase = 0;
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
-      if (i == 1 && !layer_grid_barrier(a.counters, ctas, &s_outcome)) {
-        if (tid == 0) atomicMax(a.header + kHdrStatus, kLayerStatusBarrier);
+      if (i == 1) {
+        asm volatile("fence.proxy.async;" ::: "memory");
+        if (!layer_grid_barrier(a.counters, ctas, &s_outcome) && tid == 0) atomicMax(a.header + kHdrStatus, kLayerStatusBarrier);
+        if (tid == 0) mbar_arrive(smem_u32(&bar_act));
       }
       const int begin = i == 0 ? b0 : b1, end = i == 0 ? e0 : e1;
       const int units_n = i == 0 ? up.units_n : dn.units_n, N = i == 0 ? 2 * a.H : a.H;
@@ -631,44 +661,37 @@ layer_experts_kernel(const __grid_constant__ CUtensorMap tm_gu, const __grid_con
         auto work = [&](auto NTC, auto F32C) {
           constexpr int NT = decltype(NTC)::value;
           constexpr bool F32 = decltype(F32C)::value;
-          const uint8_t* rows[NT];
           float factor[NT], inverse[NT];         // of fp32 rows
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const int ci = n * 8 + g8;
-            rows[n] = nullptr;
             factor[n] = inverse[n] = 1.f;
-            if (ci < cols) {
-              const int p = s_sorted[first + (pairs ? ci >> 1 : ci)];
-              rows[n] = reinterpret_cast<const uint8_t*>(i == 0 ? a.xh + (int64_t)(p / a.K) * a.Hp
-                                                                : a.act + (int64_t)(2 * p + (pairs ? ci & 1 : 0)) * a.Hp) +
-                        (int64_t)kt0 * kTileK * (F32 ? 4 : 2);
-              if constexpr (F32) layer_factor(__ldcg(a.act_max + p), factor[n], inverse[n]);
+            if constexpr (F32) {
+              if (n * 8 + g8 < cols) layer_factor(__ldcg(a.act_max + s_sorted[first + n * 8 + g8]), factor[n], inverse[n]);
             }
           }
+          const uint32_t pitch = kTileK * (F32 ? 4 : 2) + 16;
           float acc[NT][4];
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[n][r] = 0.f;
-          // rows and scale of the next tile are on their way while this one is worked on
-          LayerRows<FP8, F32, NT> held;
-          held.load(rows, c4);
-          float scale_next = FP8 ? __ldg(scales + kt0 * scale_step) : 1.f;
+          float scale_next = FP8 ? __ldg(scales + 2 * kt0 * scale_step) : 1.f;      // asked for half a tile ahead
 #pragma unroll 1
           for (int j = 0; j < tiles; ++j) {
-            uint4 b[NT][FP8 ? 4 : 2];
-            held.operands(factor, b);
-            const float scale = scale_next;
-            if (j + 1 < tiles) {
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-                if (rows[n] != nullptr) rows[n] += kTileK * (F32 ? 4 : 2);
-              held.load(rows, c4);
-              if (FP8) scale_next = __ldg(scales + (kt0 + j + 1) * scale_step);
-            }
+            const int halves = (2 * (kt0 + j) + 1) * kHalfK < a.H ? 2 : 1;       // the last tile of a unit may have one
             if (ok) ok = mbar_wait_warp(smem_u32(&bar_full[stage]), full_phase, &abort_flag);
-            if (ok) layer_tile<FP8, NT>(ring + stage * kLayerTileBytes, w, lane, b, scale, acc);
+            const uint32_t row = ring + kLayerStageRows + stage * kLayerRowBytes + g8 * pitch;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (h == halves) break;
+              const float scale = scale_next;
+              if (FP8 && (h + 1 < halves || j + 1 < tiles)) scale_next = __ldg(scales + (2 * (kt0 + j) + h + 1) * scale_step);
+              if (ok) {
+                uint4 b[NT][FP8 ? 4 : 2];
+                layer_rows<FP8, F32, NT>(row + h * kHalfK * (F32 ? 4 : 2), pitch, c4, factor, b);
+                layer_tile<FP8, NT>(ring + stage * kLayerTileBytes + h * (kLayerTileBytes / 2), w, lane, b, scale, acc);
+              }
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bar_empty[stage]));
             if (++stage == kLayerStages) { stage = 0; full_phase ^= 1u; }
