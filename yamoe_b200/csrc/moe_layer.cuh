@@ -133,19 +133,25 @@ layer_router_kernel(const LayerArgs a) {
   for (int i = e * kRouterThreads + threadIdx.x; i < marks; i += (a.E + a.T) * kRouterThreads)
     reinterpret_cast<uint4*>(a.part)[i] = make_uint4(0, 0, 0, 0);
   if (e < a.E) return;
-  // token rows as operands, and the columns behind the activations' H (weights there are zeros, these must be finite)
+  // token rows as operands (eight values at a time), and the columns behind the activations' H (weights there are zeros, these
+  // must be finite)
   const int t = e - a.E;
-  const __nv_bfloat16* xr = a.x + (int64_t)t * a.H;
-  uint16_t* dst = a.xh + (int64_t)t * a.Hp;
+  const uint4* xr = reinterpret_cast<const uint4*>(a.x + (int64_t)t * a.H);
+  uint4* dst = reinterpret_cast<uint4*>(a.xh + (int64_t)t * a.Hp);
   float factor = 1.f;
   if constexpr (FP8) {
     uint32_t most = 0;
-    for (int i = threadIdx.x; i < a.H; i += kRouterThreads) {
-      const uint32_t b = __float_as_uint(__bfloat162float(xr[i])) & 0x7fffffffu;
-      if (b < 0x7f800000u) most = max(most, b);
+    for (int i = threadIdx.x; i < nvec; i += kRouterThreads) {
+      const uint4 q = __ldg(xr + i);
+      const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = (u[j] << 16) & 0x7fffffffu, hi = u[j] & 0x7fff0000u;
+        if (lo < 0x7f800000u) most = max(most, lo);
+        if (hi < 0x7f800000u) most = max(most, hi);
+      }
     }
     most = __reduce_max_sync(0xffffffffu, most);
-    __syncthreads();
     if (lane == 0) s_part[w] = __uint_as_float(most);
     __syncthreads();
     float top = 0.f, inverse;
@@ -155,10 +161,22 @@ layer_router_kernel(const LayerArgs a) {
   } else if (threadIdx.x == 0) {
     a.x_scale[t] = 1.f;
   }
-  for (int i = threadIdx.x; i < a.Hp; i += kRouterThreads) {
-    uint16_t v = 0;
-    if (i < a.H) v = FP8 ? __half_as_ushort(__float2half_rn(__bfloat162float(xr[i]) * factor)) : __bfloat16_as_ushort(xr[i]);
-    dst[i] = v;
+  for (int i = threadIdx.x; i < a.Hp / 8; i += kRouterThreads) {
+    uint4 q = make_uint4(0, 0, 0, 0);
+    if (i < nvec) {
+      q = __ldg(xr + i);
+      if constexpr (FP8) {
+        uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f = bf16x2_to_float2(u[j]);
+          const __half2 h = __floats2half2_rn(f.x * factor, f.y * factor);
+          u[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        q = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+    }
+    dst[i] = q;
   }
   const int pad = a.Hp - a.H, rows = a.T * a.K * 2;          // fp32 rows are as long as two of 16 bits
   for (int i = (e - a.E) * kRouterThreads + threadIdx.x; i < rows * pad; i += a.T * kRouterThreads) {
