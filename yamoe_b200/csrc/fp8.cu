@@ -25,7 +25,7 @@ static int quantize_impl(const T* x, const yamoe_fp8_matrix_t* out, const yamoe_
   if (block_rows == 1 && turned == nullptr) {
     const QuantRows d{reinterpret_cast<uint8_t*>(out->q), out->scale, out->ld, out->q_batch, out->scale_row, out->scale_group,
                       out->scale_batch, nullptr, 0};
-    return launch_quantize_rows<T>(x, d, B, M, (int)K, false, st);
+    return launch_quantize_rows<T>(x, d, B, M, (int)K, st);
   }
   return launch_quantize_tiles<T>(x, B, M, K, block_rows == 128, quant_out(out), quant_out(turned), st);
 }
@@ -34,7 +34,7 @@ template <typename T>
 int fp8_gather(const T* hidden, uint8_t* q, float* scale, int64_t ld, int64_t scale_group, const int32_t* flat_row, int64_t tokens,
                int H, int K, cudaStream_t st) {
   const QuantRows d{q, scale, ld, 0, 1, scale_group, 0, flat_row, K};
-  return launch_quantize_rows<T>(hidden, d, 1, tokens, H, true, st);
+  return launch_quantize_rows<T>(hidden, d, 1, tokens, H, st);
 }
 template int fp8_gather<float>(const float*, uint8_t*, float*, int64_t, int64_t, const int32_t*, int64_t, int, int, cudaStream_t);
 template int fp8_gather<__nv_bfloat16>(const __nv_bfloat16*, uint8_t*, float*, int64_t, int64_t, const int32_t*, int64_t, int, int,
@@ -51,7 +51,7 @@ static int grouped(const Fp8Rows& r, const uint8_t* a, const float* a_scale, int
   p.n_tiles = r.header + kHdrRowTiles;
   p.status = const_cast<int32_t*>(r.header) + kHdrStatus;
   const Fp8Operand A{a, r.max_rows, ld, 0}, B{w.q, N, w.ld, w.q_batch};
-  return launch_fp8_gemm<256, false, true>(A, B, p, epi, r.max_tiles, true, st);
+  return launch_fp8_gemm<256, false, true>(A, B, p, epi, r.max_tiles, st);
 }
 
 template <typename T>
@@ -96,8 +96,8 @@ static int mm_impl(const Fp8Operand& A, const Fp8Operand& B, Fp8Params p, T* out
   p.MT = (int)ceil_div(p.M, 128);
   p.splits = c.splits;
   const int64_t tiles = (int64_t)p.B * p.MT;
-  return c.bn == 256 ? launch_fp8_gemm<256, BROWS, false>(A, B, p, epi, tiles, false, st)
-                     : launch_fp8_gemm<128, BROWS, false>(A, B, p, epi, tiles, false, st);
+  return c.bn == 256 ? launch_fp8_gemm<256, BROWS, false>(A, B, p, epi, tiles, st)
+                     : launch_fp8_gemm<128, BROWS, false>(A, B, p, epi, tiles, st);
 }
 
 }  // namespace yb

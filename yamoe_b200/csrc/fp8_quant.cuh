@@ -7,6 +7,8 @@
 // +-448 whatever way the two divisions are rounded.  A group is 128 neighbours in a row (activations, gradients) or
 // 128 x 128 values (weights), the last ones of a matrix being smaller.
 //
+// The kernels may start before what writes x has ended: x is read by ordinary loads behind the wait for it.
+//
 // Bound by HBM: a value is read once and its code written once, 3 bytes for bf16.  Rows (groups of 1 x 128) need no
 // exchange beyond 16 lanes, which hold a group; blocks and transposed outputs go by tiles of 128 x 128 values held in
 // the registers of a CTA, codes turned around in shared memory.
@@ -41,13 +43,13 @@ template <> struct Eight<__nv_bfloat16> {
   template <bool VEC>
   __device__ __forceinline__ void load(const __nv_bfloat16* p, int n) {
     if (VEC && n >= 8) {
-      q = __ldg(reinterpret_cast<const uint4*>(p));
+      q = ld_written(reinterpret_cast<const uint4*>(p));
     } else {
       const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        w[j] = (2 * j < n ? (uint32_t)__ldg(h + 2 * j) : 0u) | (2 * j + 1 < n ? (uint32_t)__ldg(h + 2 * j + 1) << 16 : 0u);
+        w[j] = (2 * j < n ? (uint32_t)h[2 * j] : 0u) | (2 * j + 1 < n ? (uint32_t)h[2 * j + 1] << 16 : 0u);
       q = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
@@ -71,12 +73,12 @@ template <> struct Eight<float> {
   template <bool VEC>
   __device__ __forceinline__ void load(const float* p, int n) {
     if (VEC && n >= 8) {
-      q[0] = __ldg(reinterpret_cast<const float4*>(p));
-      q[1] = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      q[0] = *reinterpret_cast<const float4*>(p);
+      q[1] = *(reinterpret_cast<const float4*>(p) + 1);
     } else {
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < n ? __ldg(p + j) : 0.f;
+      for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : 0.f;
       q[0] = make_float4(v[0], v[1], v[2], v[3]);
       q[1] = make_float4(v[4], v[5], v[6], v[7]);
     }
@@ -118,7 +120,7 @@ struct QuantRows {
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kQuantWarps * 32)
-quantize_rows_kernel(const T* __restrict__ x, const QuantRows d, int64_t rows, int K) {
+quantize_rows_kernel(const T* x, const QuantRows d, int64_t rows, int K) {
   pdl_trigger();
   const int lane = threadIdx.x & 31, l16 = lane & 15;
   // the pieces of a row are neighbours in the grid
@@ -127,11 +129,13 @@ quantize_rows_kernel(const T* __restrict__ x, const QuantRows d, int64_t rows, i
   const int64_t row = unit / pieces;
   const int k0 = (int)(unit - (unsigned)row * pieces) * (2 * kQuantPairs * kFp8Group) + lane * 8;
   if (row >= rows) return;
-  const T* src = x + ((int64_t)blockIdx.y * rows + row) * K;
+  // Of the expert pass only the tables come from the kernel before this one, which has waited for all that went before itself.
+  if (d.flat_row == nullptr) pdl_wait();
+  const T* src = after_wait(x) + ((int64_t)blockIdx.y * rows + row) * K;
   Eight<T> v[kQuantPairs];
 #pragma unroll
   for (int i = 0; i < kQuantPairs; ++i) v[i].template load<VEC>(src + k0 + i * 2 * kFp8Group, K - k0 - i * 2 * kFp8Group);
-  pdl_wait();
+  if (d.flat_row != nullptr) pdl_wait();
   const int32_t* flat_row = d.flat_row != nullptr ? after_wait(d.flat_row) : nullptr;
 #pragma unroll
   for (int i = 0; i < kQuantPairs; ++i) {
@@ -171,7 +175,7 @@ struct QuantOut {
 // rg ^ (k / 8)), so that neither the writing by columns nor the reading by rows meets bank conflicts.
 template <typename T, bool VEC, bool BLOCK>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 && VEC ? 4 : 2)
-quantize_tile_kernel(const T* __restrict__ x, int64_t batch_stride, int M, int K, const QuantOut out, const QuantOut turned) {
+quantize_tile_kernel(const T* x, int64_t batch_stride, int M, int K, const QuantOut out, const QuantOut turned) {
   constexpr int kWords = sizeof(T) == 2 ? 4 : 8;           // largest magnitudes of eight columns: bf16 two to a word
   __shared__ __align__(16) uint8_t s_codes[128 * 128];
   __shared__ uint32_t s_max[8][16 * kWords];
@@ -180,6 +184,9 @@ quantize_tile_kernel(const T* __restrict__ x, int64_t batch_stride, int M, int K
   const int m0 = blockIdx.y * 128, k0 = blockIdx.x * 128;
   const int64_t b = blockIdx.z;
   const int m = m0 + 8 * rg, k = k0 + 8 * cg;
+  pdl_trigger();
+  pdl_wait();
+  x = after_wait(x);
   Eight<T> v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -286,12 +293,12 @@ inline bool rows_of_16_bytes(const void* x, int64_t K) {
 
 // `batch` matrices of `rows` rows
 template <typename T>
-inline int launch_quantize_rows(const T* x, const QuantRows& d, int64_t batch, int64_t rows, int K, bool pdl, cudaStream_t st) {
+inline int launch_quantize_rows(const T* x, const QuantRows& d, int64_t batch, int64_t rows, int K, cudaStream_t st) {
   const int64_t ctas = ceil_div(rows * ceil_div(K, 2 * kQuantPairs * kFp8Group), kQuantWarps);
   if (ctas == 0 || batch == 0) return YAMOE_OK;
   if (ctas * kQuantWarps > 0x7fffffff || batch > 65535) return YAMOE_ERR_UNSUPPORTED;
   auto kern = rows_of_16_bytes<T>(x, K) ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
-  const cudaError_t rc = launch_pdl_opt(pdl, kern, dim3((unsigned)ctas, (unsigned)batch), dim3(kQuantWarps * 32), 0, st, x, d, rows, K);
+  const cudaError_t rc = launch_pdl_opt(true, kern, dim3((unsigned)ctas, (unsigned)batch), dim3(kQuantWarps * 32), 0, st, x, d, rows, K);
   return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
 }
 
@@ -305,8 +312,8 @@ inline int launch_quantize_tiles(const T* x, int64_t B, int64_t M, int64_t K, bo
   const bool vec = rows_of_16_bytes<T>(x, K);
   auto kern = block ? (vec ? quantize_tile_kernel<T, true, true> : quantize_tile_kernel<T, false, true>)
                     : (vec ? quantize_tile_kernel<T, true, false> : quantize_tile_kernel<T, false, false>);
-  kern<<<grid, 256, 0, st>>>(x, M * K, (int)M, (int)K, out, turned);
-  return cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
+  const cudaError_t rc = launch_pdl_opt(true, kern, grid, dim3(256), 0, st, x, M * K, (int)M, (int)K, out, turned);
+  return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
 }
 
 }  // namespace yb

@@ -337,6 +337,12 @@ at::Tensor fp8_linear_autograd(const at::Tensor& x, const at::Tensor& weight) {
   return fp8_linear_cuda(x, weight);
 }
 
+// contiguous, on the 16-byte boundary that the kernels' wide loads and copies want
+at::Tensor aligned(const at::Tensor& t) {
+  const at::Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
 at::Tensor experts_fp8_cuda(const at::Tensor& hidden_states, const at::Tensor& router_indices, const at::Tensor& routing_weights,
                             const at::Tensor& gate_up, const at::Tensor& gate_up_scale, const at::Tensor& gate_up_bias,
                             const at::Tensor& down, const at::Tensor& down_scale, const at::Tensor& down_bias,
@@ -370,8 +376,8 @@ at::Tensor experts_fp8_cuda(const at::Tensor& hidden_states, const at::Tensor& r
   const c10::cuda::CUDAGuard guard(hidden_states.device());
   const Quantised g = operand("experts_fp8", "gate_up", gate_up, gate_up_scale, 3, true),
                   d = operand("experts_fp8", "down", down, down_scale, 3, true);
-  const at::Tensor hs = hidden_states.contiguous(), ri = router_indices.to(at::kLong).contiguous(),
-                   rw = routing_weights.contiguous(), bg = gate_up_bias.contiguous(), bd = down_bias.contiguous();
+  const at::Tensor hs = aligned(hidden_states), ri = router_indices.to(at::kLong).contiguous(),
+                   rw = routing_weights.contiguous(), bg = aligned(gate_up_bias), bd = aligned(down_bias);
   at::Tensor out = at::empty_like(hs);
   const int code = dtype_of(hs);
   const size_t nbytes = yamoe_b200_experts_fp8_workspace_bytes(T, (int)H, (int)E, (int)K, code);
@@ -384,12 +390,6 @@ at::Tensor experts_fp8_cuda(const at::Tensor& hidden_states, const at::Tensor& r
         "experts_fp8");
   if (T > 0) check_device_status(ws, current_stream(), "experts_fp8");
   return out;
-}
-
-// contiguous, on the 16-byte boundary that the kernels' wide loads and copies want
-at::Tensor aligned(const at::Tensor& t) {
-  const at::Tensor c = t.contiguous();
-  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
 std::tuple<at::Tensor, at::Tensor> moe_layer_cuda(const at::Tensor& hidden_states, const at::Tensor& router_weight,

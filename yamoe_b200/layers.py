@@ -117,3 +117,49 @@ class Yamoe(torch.nn.Module):
         else:
             out = ops.experts(x, router_indices, router_scores, gate_up, gate_up_bias, down, down_bias, int(cap), E, K)
         return out.view(batch, seq, hidden), router_scores
+
+
+class Fp8Yamoe(torch.nn.Module):
+    """The MoE block of `Yamoe` for serving, with expert weights in 8 bits.
+
+        layer = Fp8Yamoe.from_layer(block)          # block: as for `Yamoe`; its bf16 expert weights are not kept
+        out, router_scores = layer(hidden_states)   # [B, S, H] bf16
+
+    Up to 32 tokens with up to 256 assignments (a decode step) run as `moe_layer`, two launches in all, activations at 16
+    bits and the router's logits unrounded.  More tokens run as `router_forward` and `experts_fp8`, which quantises the
+    token rows and the activations too.  `expert_capacity` None: ceil(T K / E), as in `Yamoe`."""
+
+    def __init__(self, router_weight, router_bias, gate_up, gate_up_scale, gate_up_bias, down, down_scale, down_bias,
+                 top_k, expert_capacity=None):
+        super().__init__()
+        for name, t in (("router_weight", router_weight), ("router_bias", router_bias), ("gate_up", gate_up),
+                        ("gate_up_scale", gate_up_scale), ("gate_up_bias", gate_up_bias), ("down", down),
+                        ("down_scale", down_scale), ("down_bias", down_bias)):
+            self.register_buffer(name, t)
+        self.top_k, self.expert_capacity = int(top_k), expert_capacity
+
+    @classmethod
+    def from_layer(cls, block):
+        hidden = block.router.weight.shape[1]
+        e = block.experts
+        gate_up, gate_up_scale, down, down_scale = ops.quantize_experts(e.gate_up_proj[:, :, : 2 * hidden].detach(),
+                                                                        e.down_proj[:, :hidden, :].detach())
+        bias = None if block.router.bias is None else block.router.bias.detach()
+        return cls(block.router.weight.detach(), bias, gate_up, gate_up_scale,
+                   e.gate_up_proj_bias[:, : 2 * hidden].detach(), down, down_scale, e.down_proj_bias.detach(),
+                   getattr(block, "top_k", 4), getattr(block, "expert_capacity", None))
+
+    @torch.no_grad()
+    def forward(self, hidden_states):
+        batch, seq, hidden = hidden_states.shape
+        T, E, K = batch * seq, self.router_weight.shape[0], self.top_k
+        x = hidden_states.reshape(T, hidden)
+        cap = int(self.expert_capacity) if self.expert_capacity is not None else ceil_div(T * K, E)
+        if T <= 32 and T * K <= 256 and x.dtype == torch.bfloat16:
+            out, scores = ops.moe_layer(x, self.router_weight, self.router_bias, self.gate_up, self.gate_up_bias, self.down,
+                                        self.down_bias, cap, E, K, self.gate_up_scale, self.down_scale)
+        else:
+            indices, scores = ops.router_forward(x, self.router_weight, self.router_bias, K)
+            out = ops.experts_fp8(x, indices, scores, self.gate_up, self.gate_up_scale, self.gate_up_bias, self.down,
+                                  self.down_scale, self.down_bias, cap, E, K)
+        return out.view(batch, seq, hidden), scores
