@@ -59,6 +59,7 @@ def main(argv=None):
             print(f"{what} of {T} tokens: bf16 {milliseconds(lambda: block(x)):.3f} ms, 8 bits {milliseconds(lambda: layer(x)):.3f} ms, "
                   f"difference {results[what]:.3f} of the output's norm")
     # a head on the block's outputs, trained with products in 8 bits
+    layer.expert_capacity = a.prompt
     x = layer(torch.randn(1, a.prompt, a.hidden, device="cuda").bfloat16())[0][0].float()
     target = torch.randint(0, a.classes, (a.prompt,), device="cuda")
     head = torch.zeros(a.classes, a.hidden, device="cuda", requires_grad=True)
@@ -68,7 +69,7 @@ def main(argv=None):
         losses.append(loss.item())
         (grad,) = torch.autograd.grad(loss, head)
         with torch.no_grad():
-            head -= grad / grad.norm()
+            head -= grad
     print(f"head: loss {losses[0]:.4f} -> {losses[-1]:.4f}")
     results["loss"] = losses
     return results
