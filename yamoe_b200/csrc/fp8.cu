@@ -42,7 +42,7 @@ template int fp8_gather<__nv_bfloat16>(const __nv_bfloat16*, uint8_t*, float*, i
 
 template <class Epi>
 static int grouped(const Fp8Rows& r, const uint8_t* a, const float* a_scale, int64_t ld, const yamoe_fp8_matrix_t& w, int N, int K,
-                   int E, const Epi& epi, cudaStream_t st) {
+                   int E, const Fp8Out& o, const Epi& epi, cudaStream_t st) {
   Fp8Params p{};
   p.M = r.max_rows; p.N = N; p.K = K; p.B = E;
   p.sa = a_scale; p.sa_m = 1; p.sa_k = r.max_rows;
@@ -51,18 +51,18 @@ static int grouped(const Fp8Rows& r, const uint8_t* a, const float* a_scale, int
   p.n_tiles = r.header + kHdrRowTiles;
   p.status = const_cast<int32_t*>(r.header) + kHdrStatus;
   const Fp8Operand A{a, r.max_rows, ld, 0}, B{w.q, N, w.ld, w.q_batch};
-  return launch_fp8_gemm<256, false, true>(A, B, p, epi, r.max_tiles, st);
+  return launch_fp8_gemm<256, false, true>(A, B, o, p, epi, r.max_tiles, st);
 }
 
 template <typename T>
 int fp8_gate_up(const Fp8Rows& r, const uint8_t* x, const float* x_scale, int64_t ld, const yamoe_fp8_matrix_t& w, const T* bias,
                 uint8_t* act, float* act_scale, int H, int E, cudaStream_t st) {
-  return grouped(r, x, x_scale, ld, w, 2 * H, H, E, Fp8GluQuant<T>{bias, act, act_scale, ld, r.max_rows}, st);
+  return grouped(r, x, x_scale, ld, w, 2 * H, H, E, Fp8Out{}, Fp8GluQuant<T>{bias, act, act_scale, ld, r.max_rows}, st);
 }
 template <typename T>
 int fp8_down(const Fp8Rows& r, const uint8_t* act, const float* act_scale, int64_t ld, const yamoe_fp8_matrix_t& w, const T* bias,
              float* y, int H, int E, cudaStream_t st) {
-  return grouped(r, act, act_scale, ld, w, H, H, E, Fp8WeightedRows<T>{bias, y, r.row_token, r.row_flat, r.row_weight, H}, st);
+  return grouped(r, act, act_scale, ld, w, H, H, E, Fp8Out{y, r.max_rows, H, 1, 4}, Fp8WeightedRows<T>{bias, r.row_token, r.row_weight, H}, st);
 }
 #define YB_INSTANTIATE(T)                                                                                                  \
   template int fp8_gate_up<T>(const Fp8Rows&, const uint8_t*, const float*, int64_t, const yamoe_fp8_matrix_t&, const T*,   \
@@ -76,13 +76,14 @@ YB_INSTANTIATE(__nv_bfloat16)
 // Tiles of a product: estimated clocks of each kind, the least of them.  A block takes a 128 x 256 tile some 1150 clocks, a 128 x 128
 // one 650; a tile's beginning and end 3000; meeting in shared memory 1500 more.
 struct Fp8Choice { int bn, splits; };
+template <bool BROWS, class Epi>
 static Fp8Choice choose_tiles(int64_t B, int64_t M, int64_t N, int64_t K) {
   const int64_t kb = ceil_div(K, kFp8Group), rows = B * ceil_div(M, 128);
   Fp8Choice best{256, 1};
   double least = (double)ceil_div(rows * ceil_div(N, 256), kSMs) * (double)(kb * 1150 + 3000);
   for (int s = 1; s <= kFp8MaxSplits && s <= kb; ++s) {
     const double t =
-        (double)ceil_div(rows * ceil_div(N, 128) * s, kSMs) * (double)(ceil_div(kb, s) * 650 + 3000 + (s > 1 ? 1500 : 0));
+        (double)ceil_div(rows * ceil_div(N, 128), s > 1 ? fp8_clusters<BROWS, Epi>(s) : kSMs) * (double)(ceil_div(kb, s) * 650 + 3000 + (s > 1 ? 1500 : 0));
     if (t < least) { least = t; best = Fp8Choice{128, s}; }
   }
   return best;
@@ -92,12 +93,13 @@ template <typename T, bool BROWS>
 static int mm_impl(const Fp8Operand& A, const Fp8Operand& B, Fp8Params p, T* out, cudaStream_t st) {
   const int vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.N * (int64_t)sizeof(T) % 16 == 0;
   const Fp8Store<T> epi{out, p.N, p.M * p.N, vec};
-  const Fp8Choice c = choose_tiles(p.B, p.M, p.N, p.K);
+  const Fp8Choice c = choose_tiles<BROWS, Fp8Store<T>>(p.B, p.M, p.N, p.K);
   p.MT = (int)ceil_div(p.M, 128);
   p.splits = c.splits;
   const int64_t tiles = (int64_t)p.B * p.MT;
-  return c.bn == 256 ? launch_fp8_gemm<256, BROWS, false>(A, B, p, epi, tiles, st)
-                     : launch_fp8_gemm<128, BROWS, false>(A, B, p, epi, tiles, st);
+  const Fp8Out o{vec ? out : nullptr, p.M, p.N, p.B, (int)sizeof(T)};
+  return c.bn == 256 ? launch_fp8_gemm<256, BROWS, false>(A, B, o, p, epi, tiles, st)
+                     : launch_fp8_gemm<128, BROWS, false>(A, B, o, p, epi, tiles, st);
 }
 
 }  // namespace yb

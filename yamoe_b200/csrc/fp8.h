@@ -19,7 +19,7 @@ int fp8_gather(const T* hidden, uint8_t* q, float* scale, int64_t ld, int64_t sc
 struct Fp8Rows {
   const int32_t* pad_off;
   const int32_t* header;        // row tiles, status
-  const int32_t *row_token, *row_flat;
+  const int32_t* row_token;
   const float* row_weight;
   int64_t max_rows, max_tiles;
 };

@@ -56,21 +56,28 @@ struct Fp8Params {
 constexpr int kFp8MaxSplits = 4;
 
 constexpr int kFp8ScaleBlocks = 4, kFp8ScaleSlots = 2;     // blocks of 128 whose scales come together, such groups on their way
-constexpr int kFp8ParkBytes = 32 * 64;                     // per epilogue warp: 64 bytes of each of its rows
+
+constexpr int kFp8BoxBytes = 32 * 128;
+constexpr int kFp8ShareBytes = 128 * 64 * 4;               // the most that a CTA of a cluster has of a tile's sums in the end
 
 template <int BN, bool BROWS>
 struct Fp8Smem {
   static constexpr int kABytes = 128 * 128;
   static constexpr int kBBytes = BN * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = 196608 / kStageBytes;     // 4 (256 columns) or 6
-  static_assert(kStages * kStageBytes >= (kFp8MaxSplits - 1) * 128 * 128 * 4, "the sums of the others of a cluster");
+  // 128 columns: the last of the six stages is where rows park, unless a cluster shares the tile, whose CTAs have one each
+  // and park when the stages are done with
+  static constexpr int kStages = BN == 256 ? 3 : 6;
+  static constexpr int kBoxes = BN / 128;                  // of 32 rows of 128 bytes, of a warp, on their way out
+  static constexpr int kParkBytes = kBoxes * kFp8BoxBytes;
   static constexpr int kScaleFloats = 128 + (BROWS ? BN : 4);                    // of a block: rows, columns or column blocks
-  static constexpr int kPark = kStages * kStageBytes;                            // from the 1024-byte boundary on
-  static constexpr int kScales = kPark + kFp8EpiWarps * kFp8ParkBytes;
+  static constexpr int kPark = (BN == 256 ? kStages : kStages - 1) * kStageBytes;     // from the 1024-byte boundary on
+  static constexpr int kScales = kPark + kFp8EpiWarps * kParkBytes;
+  static_assert(kScales >= kStages * kStageBytes, "a stage is as large as what the warps park");
+  static_assert(BN != 128 || kPark >= kFp8MaxSplits * kFp8ShareBytes, "the sums of a cluster's parts");
   static constexpr int kTables = kScales + kFp8ScaleSlots * kFp8ScaleBlocks * kScaleFloats * 4 + 1024;
 };
-inline int fp8_smem_bytes(int tables, int experts) { return tables + (experts > 0 ? 2 * (experts + 1) * 4 : 0); }
+inline int fp8_smem_bytes(int tables, int experts) { return tables + (experts > 0 ? (experts + 1) * 4 : 0); }
 
 __device__ __forceinline__ void tc_mma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -108,18 +115,23 @@ struct Fp8Tile {
   int64_t row_end;     // rows from here on are another's
   int n0, n_end;       // n_end: columns of the matrix
   int q, half, lane;   // lane quarter and column half of the warp
-  uint32_t park;       // kFp8ParkBytes of shared memory of the warp's own
+  uint32_t park;       // shared memory of the warp's own (kParkBytes)
   bool ok;             // false: take part in barriers only
+  const CUtensorMap* out;      // where boxes of 32 rows of 128 bytes go
 };
+// The four groups of 16 columns of a half of a tile of 128, shared out to `splits` CTAs
+__device__ __forceinline__ int fp8_owner(int g, int splits) { return g * splits / 4; }
+__device__ __forceinline__ int fp8_first_group(int part, int splits) { return (4 * part + splits - 1) / splits; }
 
 template <int BN, bool BROWS, bool GROUPED, class Epi>
 __global__ void __launch_bounds__(kFp8Threads, 1)
-fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Fp8Params p,
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const __grid_constant__ CUtensorMap tmOut, const Fp8Params p,
                 const Epi epi) {
   using SM = Fp8Smem<BN, BROWS>;
-  constexpr int kStages = SM::kStages, kAccs = 512 / BN, kCols = BN / 2;
+  constexpr int kAccs = 512 / BN, kCols = BN / 2;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[kStages], bar_empty[kStages], bar_tmem_full[kAccs], bar_tmem_empty[kAccs];
+  __shared__ __align__(8) uint64_t bar_full[SM::kStages], bar_empty[SM::kStages], bar_tmem_full[kAccs], bar_tmem_empty[kAccs];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
   __shared__ __align__(8) uint64_t bar_scale_full[kFp8ScaleSlots], bar_scale_empty[kFp8ScaleSlots];
@@ -127,15 +139,15 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = BN == 128 && !GROUPED ? p.splits : 1;
+  const int stages = BN == 256 || splits > 1 ? SM::kStages : SM::kStages - 1;
   const int part = splits > 1 ? (int)cluster_ctarank() : 0;       // of the tile's blocks
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const aligned = smem_raw + (smem_base - smem_u32(smem_raw));
   float* const s_scale = reinterpret_cast<float*>(aligned + SM::kScales);
-  int32_t* s_first = reinterpret_cast<int32_t*>(smem_raw + SM::kTables);   // grouped: first tile of each expert
-  int32_t* s_pad = s_first + p.B + 1;                                      // first padded row of each expert
+  int32_t* s_pad = reinterpret_cast<int32_t*>(smem_raw + SM::kTables);     // grouped: first padded row of each expert
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
       mbar_init(smem_u32(&bar_empty[s]), 1);
     }
@@ -162,10 +174,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   pdl_trigger();
   pdl_wait();
   if constexpr (GROUPED) {
-    for (int i = threadIdx.x; i <= p.B; i += kFp8Threads) {
-      s_pad[i] = p.pad_off[i];
-      s_first[i] = p.pad_off[i] / kTileM;
-    }
+    for (int i = threadIdx.x; i <= p.B; i += kFp8Threads) s_pad[i] = p.pad_off[i];
     __syncthreads();
   }
   if (p.clear_status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = kStatusOk;   // waits give up after seconds at the earliest
@@ -177,15 +186,15 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   // work item -> matrix or expert, first row of the tile, first column
   auto decode = [&](int64_t id, int& b, int64_t& m0, int& n0) {
     if constexpr (GROUPED) {
-      const int tile = (int)(id / p.NT);
+      const int row = (int)((uint32_t)id / (uint32_t)p.NT) * kTileM;
       int lo = 0, hi = p.B;                      // the last expert whose first tile is not behind this one
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (s_first[mid] <= tile) lo = mid; else hi = mid;
+        if (s_pad[mid] <= row) lo = mid; else hi = mid;
       }
       b = lo;
-      const int cnt = s_first[b + 1] - s_first[b];
-      const int local = (int)(id - (int64_t)s_first[b] * p.NT);
+      const int first = s_pad[b] / kTileM, cnt = s_pad[b + 1] / kTileM - first;
+      const int local = (int)id - first * p.NT;
       const int nt = local / cnt;
       m0 = s_pad[b] + (int64_t)(local - nt * cnt) * kTileM;
       n0 = nt * BN;
@@ -222,11 +231,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             tma_load_3d(sa + SM::kABytes, &tmB, kb * kFp8Group, n0, b, full);
           }
           __syncwarp();
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          if (++stage == stages) { stage = 0; phase ^= 1u; }
         }
       }
       // the commits that free the last stages must have arrived here before this CTA ends
-      for (int s = 0; s < kStages && ok; ++s)
+      for (int s = 0; s < stages && ok; ++s)
         ok = mbar_wait_warp(smem_u32(&bar_empty[s]), s < stage ? phase : phase ^ 1u, &abort_flag);
       if (!ok && lane == 0) {
         abort_flag = 1;
@@ -262,7 +271,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             tc_commit(smem_u32(&bar_empty[stage]));
           }
           __syncwarp();
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          if (++stage == stages) { stage = 0; phase ^= 1u; }
           if (++acc == kAccs) { acc = 0; acc_phase ^= 1u; }
         }
       }
@@ -335,7 +344,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       t.n0 = n0 + half * kCols;
       t.n_end = (int)p.N;
       t.q = q; t.half = half; t.lane = lane;
-      t.park = smem_base + SM::kPark + (warp - kFp8FirstEpiWarp) * kFp8ParkBytes;
+      t.out = &tmOut;
+      t.park = smem_base + SM::kPark + (warp - kFp8FirstEpiWarp) * SM::kParkBytes;
       const bool row_ok = t.row < t.row_end;
       const auto pre = epi.begin(t, row_ok);
       uint64_t sum[kCols / 2];
@@ -406,40 +416,54 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       t.ok = ok;
       if constexpr (BN == 128 && !GROUPED) {
         if (splits > 1) {
-          // [part - 1][four columns of the tile][row]: a warp stores 512 contiguous bytes
-          const int row = q * 32 + lane;
-          const uint32_t at = (uint32_t)((half * (kCols / 4) * 128 + row) * 16);
-          cluster_sync_all();                    // the first CTA's copies and instructions are done with its shared memory
-          if (part > 0 && row_ok) {
-            const uint32_t dst = mapa_u32(smem_base, 0) + (uint32_t)(part - 1) * (128 * 128 * 4) + at;
+          // Each CTA gets all parts' sums of its own share of the columns, its own among them, so that no register is
+          // picked by part: [part][half][four columns][row], a warp stores 512 contiguous bytes.
+          const uint32_t at = (uint32_t)(half * (kFp8ShareBytes / 2) + (q * 32 + lane) * 16);
+          cluster_sync_all();                    // everyone's copies and instructions are done with their shared memory
+          if (row_ok) {
 #pragma unroll
-            for (int i = 0; i < kCols / 4; ++i) {
-              float v[4];
-              unpack_f32x2(sum[2 * i], v[0], v[1]);
-              unpack_f32x2(sum[2 * i + 1], v[2], v[3]);
-              asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t)i * 2048u), "f"(v[0]), "f"(v[1]),
-                           "f"(v[2]), "f"(v[3]) : "memory");
+            for (int g = 0; g < kCols / 16; ++g) {
+              const int owner = fp8_owner(g, splits);
+              const uint32_t dst = mapa_u32(smem_base, owner) + part * kFp8ShareBytes + at + (g - fp8_first_group(owner, splits)) * 8192;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                float v[4];
+                unpack_f32x2(sum[8 * g + 2 * i], v[0], v[1]);
+                unpack_f32x2(sum[8 * g + 2 * i + 1], v[2], v[3]);
+                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t)i * 2048u), "f"(v[0]), "f"(v[1]),
+                             "f"(v[2]), "f"(v[3]) : "memory");
+              }
             }
           }
           cluster_sync_all();
-          if (part > 0) break;
-          for (int o = 1; o < splits; ++o) {
-            const uint32_t src = smem_base + (uint32_t)(o - 1) * (128 * 128 * 4) + at;
+          if (ok && t.row - lane < t.row_end) {
+            const int g0 = fp8_first_group(part, splits), g1 = fp8_first_group(part + 1, splits);
+#pragma unroll 1
+            for (int g = g0; g < g1 && t.n0 + 16 * g < t.n_end; ++g) {
+              float v[16];
 #pragma unroll
-            for (int i = 0; i < kCols / 4; ++i) {
-              float v[4], x[4];
-              unpack_f32x2(sum[2 * i], v[0], v[1]);
-              unpack_f32x2(sum[2 * i + 1], v[2], v[3]);
-              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
-                           : "r"(src + (uint32_t)i * 2048u));
-              sum[2 * i] = pack_f32x2(v[0] + x[0], v[1] + x[1]);
-              sum[2 * i + 1] = pack_f32x2(v[2] + x[2], v[3] + x[3]);
+              for (int i = 0; i < 16; ++i) v[i] = 0.f;
+#pragma unroll 1
+              for (int o = 0; o < splits; ++o) {
+                const uint32_t src = smem_base + o * kFp8ShareBytes + at + (g - g0) * 8192;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  float x[4];
+                  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3])
+                               : "r"(src + (uint32_t)i * 2048u) : "memory");
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) v[4 * i + j] += x[j];
+                }
+              }
+              epi.store_group(t, v, 16 * g);
             }
           }
+          break;
         }
       }
-      epi.template finish<kCols>(t, row_ok, pre, sum, s_epi, parity);
+      epi.template finish<kCols, SM::kBoxes>(t, row_ok, pre, sum, s_epi, parity);
     }
+    tma_store_wait_all();
     if (!ok) {
       abort_flag = 1;
       atomicMax(p.status, (int)kStatusEpilogueTimeout);
@@ -492,6 +516,30 @@ __device__ __forceinline__ void store_rows_64(uint32_t park, int lane, const uin
   __syncwarp();
 }
 
+// 16 bytes (piece k) of the lane's row of a box, as TMA with 128-byte swizzle wants them
+__device__ __forceinline__ void park_row(const Fp8Tile& t, int box, int k, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(t.park + box * kFp8BoxBytes + t.lane * 128 + ((k ^ (t.lane & 7)) << 4)),
+               "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// The warp's boxes on their way: rows that exist only in part, and columns, are cut off by the tensor map.  One instruction for 4 KB:
+// a bulk copy for each row took 95 clocks apiece to issue, 3000 for a tile, as long as 16-byte stores of its rows by the lanes.
+template <int BOXES>
+__device__ __forceinline__ void send_boxes(const Fp8Tile& t, int col, int box_cols) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if (t.lane == 0 && t.row < t.row_end) {
+#pragma unroll
+    for (int x = 0; x < BOXES; ++x)
+      if (col + x * box_cols < t.n_end)
+        tma_store_3d(t.out, col + x * box_cols, (int)t.row, t.b, t.park + x * kFp8BoxBytes);
+    tma_store_commit();
+  }
+}
+__device__ __forceinline__ void boxes_free(int lane) {
+  if (lane == 0) tma_store_wait_read();
+  __syncwarp();
+}
+
 // C[b, m, n] rounded to T
 template <typename T>
 struct Fp8Store {
@@ -502,36 +550,87 @@ struct Fp8Store {
   int vec;                 // rows start on 16-byte boundaries
 
   __device__ __forceinline__ Pre begin(const Fp8Tile&, bool) const { return {}; }
-  template <int COLS>
-  __device__ __forceinline__ void finish(const Fp8Tile& t, bool row_ok, const Pre&, const uint64_t (&sum)[COLS / 2], Shared&,
-                                         uint32_t) const {
-    if (!t.ok) return;
-    constexpr int VE = 16 / (int)sizeof(T), kCols = 64 / (int)sizeof(T);     // columns of 16 and of 64 bytes
-    T* c = C + t.b * batch + t.row * ld + t.n0;
+
+  // 16 columns of the warp's rows from n0 + i on, the lane's in `v`, as far as they exist
+  __device__ __forceinline__ void store_group(const Fp8Tile& t, const float (&v)[16], int i) const {
+    constexpr int kPieces = (int)sizeof(T), kPitch = 16 * kPieces + 16;      // 16-byte pieces of a row
+    const uint32_t mine = t.park + t.lane * kPitch;
 #pragma unroll
-    for (int i = 0; i < COLS; i += kCols) {
-      const int cols = t.n_end - t.n0 - i;
-      if (cols <= 0) break;
-      float v[kCols];
+    for (int k = 0; k < kPieces; ++k) {
+      uint4 w;
+      if constexpr (sizeof(T) == 2)
+        w = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                       pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+      else
+        w = make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
+                       __float_as_uint(v[4 * k + 3]));
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + 16 * k), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+    }
+    __syncwarp();
+    const int rows = (int)min((int64_t)32, t.row_end - (t.row - t.lane));
+    const int cols = min(16, t.n_end - t.n0 - i);
+    T* const first = C + t.b * batch + (t.row - t.lane) * ld + t.n0 + i;      // the warp's first row
+    if (vec) {
+      constexpr int kRows = 32 / kPieces;              // at a time
+      const int k = t.lane % kPieces;
 #pragma unroll
-      for (int j = 0; j < kCols; j += 2) unpack_f32x2(sum[(i + j) / 2], v[j], v[j + 1]);
-      if (vec) {
-        uint4 w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if constexpr (sizeof(T) == 2)
-            w[k] = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                              pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
-          else
-            w[k] = make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
-                              __float_as_uint(v[4 * k + 3]));
-        }
-        store_rows_64(t.park, t.lane, w, row_ok ? reinterpret_cast<char*>(c + i) : nullptr, cols / VE);
-      } else if (row_ok) {
-#pragma unroll
-        for (int j = 0; j < kCols; ++j)
-          if (j < cols) DT<T>::st(c + i + j, v[j]);
+      for (int p = 0; p < kPieces; ++p) {
+        const int r = p * kRows + t.lane / kPieces;
+        uint4 x;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                     : "r"(t.park + r * kPitch + 16 * k) : "memory");
+        if (r < rows && k * (16 / kPieces) < cols) *reinterpret_cast<uint4*>(first + r * ld + k * (16 / kPieces)) = x;
       }
+    } else {
+      using U = typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type;
+      const int j = t.lane & 15;
+      U x[16];
+#pragma unroll
+      for (int p = 0; p < 16; ++p) {
+        const uint32_t at = t.park + (2 * p + (t.lane >> 4)) * kPitch + j * (int)sizeof(T);
+        if constexpr (sizeof(T) == 2) asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x[p]) : "r"(at) : "memory");
+        else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x[p]) : "r"(at) : "memory");
+      }
+#pragma unroll
+      for (int p = 0; p < 16; ++p) {
+        const int r = 2 * p + (t.lane >> 4);
+        if (r < rows && j < cols) reinterpret_cast<U*>(first + r * ld)[j] = x[p];
+      }
+    }
+    __syncwarp();
+  }
+
+  template <int COLS, int BOXES>
+  __device__ __forceinline__ void finish(const Fp8Tile& t, bool, const Pre&, const uint64_t (&sum)[COLS / 2], Shared&, uint32_t) const {
+    if (!t.ok) return;
+    if (vec) {
+      constexpr int kBoxCols = 128 / (int)sizeof(T);
+#pragma unroll
+      for (int i = 0; i < COLS; i += BOXES * kBoxCols) {
+        if (t.n0 + i >= t.n_end) break;
+        boxes_free(t.lane);
+#pragma unroll
+        for (int k = 0; k < 8 * BOXES; ++k) {
+          constexpr int VE = 16 / (int)sizeof(T);
+          float v[VE];
+#pragma unroll
+          for (int j = 0; j < VE; j += 2) unpack_f32x2(sum[(i + k * VE + j) / 2], v[j], v[j + 1]);
+          if constexpr (sizeof(T) == 2)
+            park_row(t, k / 8, k % 8, pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+          else
+            park_row(t, k / 8, k % 8, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        }
+        send_boxes<BOXES>(t, t.n0 + i, kBoxCols);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < COLS; i += 16) {
+      if (t.n0 + i >= t.n_end) break;
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) unpack_f32x2(sum[(i + j) / 2], v[j], v[j + 1]);
+      store_group(t, v, i);
     }
   }
 };
@@ -549,7 +648,7 @@ struct Fp8GluQuant {
   int64_t ld, scale_group;
 
   __device__ __forceinline__ Pre begin(const Fp8Tile&, bool) const { return {}; }
-  template <int COLS>
+  template <int COLS, int BOXES>
   __device__ __forceinline__ void finish(const Fp8Tile& t, bool row_ok, const Pre&, const uint64_t (&sum)[COLS / 2], Shared& s,
                                          uint32_t parity) const {
     static_assert(COLS == 128, "a group of 128 activations is a tile of 256 columns");
@@ -586,51 +685,46 @@ struct Fp8GluQuant {
   }
 };
 
-// down of the expert pass: y = w_row * (v + bias) in fp32 at the flat position of the row, or (fp32 calls) at the padded row
-// itself, as combine_padded_kernel wants the K rows of a token that it sums.  Padding rows have no position and no weight.
+// down of the expert pass: y = w_row * (v + bias) in fp32 at the padded row, as combine_padded_kernel wants the K rows of a
+// token that it sums.  What padding rows get is not read.
 template <typename T>
 struct Fp8WeightedRows {
-  static constexpr bool kFlat = sizeof(T) != sizeof(float);
   struct Shared {};
-  struct Pre { float w; int64_t at; };
+  struct Pre { float w; };
   const T* bias;           // [E, N]
-  float* y;                // [S, N] or [rows, N]
   const int32_t* row_token;
-  const int32_t* row_flat;
   const float* row_weight;
   int64_t N;
 
   __device__ __forceinline__ Pre begin(const Fp8Tile& t, bool row_ok) const {
-    Pre p{0.f, -1};
-    if (row_ok && row_token[t.row] >= 0) {
-      p.at = kFlat ? (int64_t)row_flat[t.row] : t.row;
-      p.w = row_weight[t.row];
-    }
-    return p;
+    const int token = row_ok ? row_token[t.row] : -1;
+    const float w = row_ok ? row_weight[t.row] : 0.f;          // (padding rows have none)
+    return Pre{token >= 0 ? w : 0.f};
   }
-  template <int COLS>
+  template <int COLS, int BOXES>
   __device__ __forceinline__ void finish(const Fp8Tile& t, bool, const Pre& p, const uint64_t (&sum)[COLS / 2], Shared&,
                                          uint32_t) const {
     if (!t.ok) return;
-    float* dst = y + p.at * N + t.n0;
     const T* bs = bias + t.b * N + t.n0;
+    Fp8Tile o = t;
+    o.b = 0;                                         // the rows of all experts are one matrix
 #pragma unroll
-    for (int i = 0; i < COLS; i += 16) {
-      const int cols = t.n_end - t.n0 - i;         // a multiple of 8
+    for (int i = 0; i < COLS; i += 32 * BOXES) {
+      const int cols = t.n_end - t.n0 - i;           // a multiple of 8
       if (cols <= 0) break;
-      float b[16];
-      load_vec<T, 8>(bs + i, *reinterpret_cast<float(*)[8]>(b));
-      if (cols > 8) load_vec<T, 8>(bs + i + 8, *reinterpret_cast<float(*)[8]>(b + 8));
-      uint4 w[4];
+      boxes_free(t.lane);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float v[4];
-        unpack_f32x2(sum[(i + 4 * k) / 2], v[0], v[1]);
-        unpack_f32x2(sum[(i + 4 * k) / 2 + 1], v[2], v[3]);
-        w[k] = make_uint4(__float_as_uint(p.w * (v[0] + b[4 * k])), __float_as_uint(p.w * (v[1] + b[4 * k + 1])),
-                          __float_as_uint(p.w * (v[2] + b[4 * k + 2])), __float_as_uint(p.w * (v[3] + b[4 * k + 3])));
+      for (int k = 0; k < 4 * BOXES; ++k) {
+        float b[8] = {}, v[8];
+        if (8 * k < cols) load_vec<T, 8>(bs + i + 8 * k, b);
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) unpack_f32x2(sum[(i + 8 * k + j) / 2], v[j], v[j + 1]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = p.w * (v[j] + b[j]);
+        park_row(t, k / 4, 2 * (k % 4), __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        park_row(t, k / 4, 2 * (k % 4) + 1, __float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
       }
-      store_rows_64(t.park, t.lane, w, p.at >= 0 ? reinterpret_cast<char*>(dst + i) : nullptr, cols / 4);
+      send_boxes<BOXES>(o, t.n0 + i, 32);
     }
   }
 };
@@ -640,12 +734,13 @@ struct Fp8WeightedRows {
 // ---------------------------------------------------------------------------------------------
 
 // Prepares a kernel for its shared memory, once per kernel and device
-template <typename... KArgs>
+template <class Epi>
+constexpr int kFp8MostSmem = 227 * 1024 - 1024 - (int)sizeof(typename Epi::Shared);     // static shared memory lies beside it
+template <class Epi, typename... KArgs>
 inline bool fp8_configure(void (*kern)(KArgs...), PerDevice<int>& done) {
   const int dev = current_device_index();
   if (done.get(dev)) return true;
-  constexpr int kMost = 227 * 1024 - 3072;     // static shared memory beside it
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess) return false;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8MostSmem<Epi>) != cudaSuccess) return false;
   done.set(dev, 1);
   return true;
 }
@@ -654,31 +749,69 @@ struct Fp8Operand {
   const void* q;
   int64_t rows, ld, batch;      // rows per matrix, pitch, distance of matrices (bytes)
 };
+// Where the boxes of a tile go; null: the epilogue sends none
+struct Fp8Out {
+  void* c;
+  int64_t rows, cols, batch;    // rows of a matrix; matrices
+  int size;                     // of a value: 2 bf16, 4 fp32
+};
+
+// Clusters of `splits` CTAs that are on the GPU at the same time
+template <bool BROWS, class Epi>
+inline int fp8_clusters(int splits) {
+  static PerDevice<int> most[kFp8MaxSplits + 1], configured;
+  const int dev = current_device_index();
+  int n = most[splits].get(dev);
+  if (n > 0) return n;
+  auto kern = fp8_gemm_kernel<128, BROWS, false, Epi>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(splits);
+  cfg.blockDim = dim3(kFp8Threads);
+  cfg.dynamicSmemBytes = (size_t)fp8_smem_bytes(Fp8Smem<128, BROWS>::kTables, 0);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (!fp8_configure<Epi>(kern, configured) || cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+    (void)cudaGetLastError();
+    n = umma_sm_count() / splits;
+  }
+  most[splits].set(dev, n);
+  return n;
+}
 
 // `max_tiles`: row tiles of 128 rows in all
 template <int BN, bool BROWS, bool GROUPED, class Epi>
-inline int launch_fp8_gemm(const Fp8Operand& a, const Fp8Operand& b, Fp8Params p, const Epi& epi, int64_t max_tiles,
+inline int launch_fp8_gemm(const Fp8Operand& a, const Fp8Operand& b, const Fp8Out& o, Fp8Params p, const Epi& epi, int64_t max_tiles,
                            cudaStream_t st) {
   if (!umma_available()) return YAMOE_ERR_UNSUPPORTED;
   using SM = Fp8Smem<BN, BROWS>;
-  CUtensorMap tmA, tmB;
+  static_assert(SM::kTables + (GROUPED ? 1025 * 4 : 0) <= kFp8MostSmem<Epi>, "up to 1024 experts");
+  CUtensorMap tmA, tmB, tmOut{};
   const uint64_t na = GROUPED ? 1 : (uint64_t)p.B;
   const uint64_t da[3] = {(uint64_t)p.K, (uint64_t)a.rows, na}, db[3] = {(uint64_t)p.K, (uint64_t)b.rows, (uint64_t)p.B};
   const uint64_t ga[2] = {(uint64_t)a.ld, (uint64_t)(na > 1 ? a.batch : a.ld)};
   const uint64_t gb[2] = {(uint64_t)b.ld, (uint64_t)(p.B > 1 ? b.batch : b.ld)};
   const uint32_t boxa[3] = {128, 128, 1}, boxb[3] = {128, BN, 1};
   if (!encode_map(&tmA, a.q, 3, da, ga, boxa, kMapU8) || !encode_map(&tmB, b.q, 3, db, gb, boxb, kMapU8)) return YAMOE_ERR_CUDA;
+  if (o.c != nullptr) {
+    const uint64_t dim[3] = {(uint64_t)o.cols, (uint64_t)o.rows, (uint64_t)o.batch};
+    const uint64_t pitch[2] = {(uint64_t)(o.cols * o.size), (uint64_t)(o.cols * o.size * (o.batch > 1 ? o.rows : 1))};
+    const uint32_t box[3] = {128u / o.size, 32, 1};
+    if (!encode_map(&tmOut, o.c, 3, dim, pitch, box, o.size == 2 ? kMapBf16 : kMapF32Swizzled)) return YAMOE_ERR_CUDA;
+  }
   auto kern = fp8_gemm_kernel<BN, BROWS, GROUPED, Epi>;
   static PerDevice<int> configured;    // per template instantiation and device
-  if (!fp8_configure(kern, configured)) return YAMOE_ERR_CUDA;
+  if (!fp8_configure<Epi>(kern, configured)) return YAMOE_ERR_CUDA;
   p.NT = (int)ceil_div(p.N, BN);
   const int64_t total = max_tiles * p.NT;
   if (total <= 0) return YAMOE_OK;
   const bool split = BN == 128 && !GROUPED && p.splits > 1;
   if (!split) p.splits = 1;
   // Clusters that start early, on SMs that the launch before leaves free, take places from those that cannot: 45 clusters of three
-  // took 16.6 us instead of 12.6.  Where there is no room for more than one they gain (48 of three: 28.8 -> 26.2).
-  const bool early = !split || p.splits * (total + 2) > umma_sm_count();
+  // took 16.6 us instead of 12.6.
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(split ? p.splits * total : std::min<int64_t>(total, umma_sm_count())));
   cfg.blockDim = dim3(kFp8Threads);
@@ -689,10 +822,10 @@ inline int launch_fp8_gemm(const Fp8Operand& a, const Fp8Operand& b, Fp8Params p
   attr[0].val.clusterDim.x = p.splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled(true) && early ? 1 : 0;
+  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled(true) && !split ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, kern, tmA, tmB, p, epi) != cudaSuccess) return YAMOE_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmOut, p, epi) != cudaSuccess) return YAMOE_ERR_CUDA;
   return cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
 }
 

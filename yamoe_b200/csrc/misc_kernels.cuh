@@ -386,14 +386,13 @@ __device__ __forceinline__ void unpack_vec(const uint4& q, float (&v)[16 / sizeo
 // other: 30 us at T = 64 and 512 with H = 2880, now 3 to 5), HBM the others.  The pieces of a row are neighbours in
 // the grid, so that its 512-byte parts are read at about the same time (T = 4096 44 us with the tokens as
 // neighbours, 30 with the pieces, 24 since the loads wait unconverted; T = 1531, K = 8, H = 2048 23 and 11).
-// Rows of another type than the output (fp32 rows of a bf16 call) lie at their flat positions p = t*K + k.
-template <typename TY, typename T, int KB>
+// FLAT: the rows lie at their flat positions p = t*K + k (fp32 rows of a decode-sized bf16 call).
+template <typename TY, typename T, int KB, bool FLAT>
 __global__ void __launch_bounds__(kRowWarps * 32, KB > 4 ? 4 : 5)
 combine_padded_kernel(const TY* y, const int32_t* flat_row, T* __restrict__ out, int64_t Tn, int H, int K) {
   pdl_wait();
   y = after_wait(y);
   flat_row = after_wait(flat_row);
-  constexpr bool kFlat = !std::is_same<TY, T>::value;
   constexpr int VE = 16 / (int)sizeof(TY);
   const unsigned chunks = (unsigned)(H / VE + 31) / 32;
   const unsigned piece = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
@@ -412,7 +411,7 @@ combine_padded_kernel(const TY* y, const int32_t* flat_row, T* __restrict__ out,
     for (int k = 0; k < KB; ++k) {
       q[k] = make_uint4(0, 0, 0, 0);
       if (r[k] >= 0)
-        q[k] = ld_written(reinterpret_cast<const uint4*>(y + (kFlat ? (size_t)(t * K + k0 + k) : (size_t)r[k]) * H) + i);
+        q[k] = ld_written(reinterpret_cast<const uint4*>(y + (FLAT ? (size_t)(t * K + k0 + k) : (size_t)r[k]) * H) + i);
     }
 #pragma unroll
     for (int k = 0; k < KB; ++k)
@@ -426,10 +425,10 @@ combine_padded_kernel(const TY* y, const int32_t* flat_row, T* __restrict__ out,
   store_vec<T, VE>(out + (size_t)t * H + (size_t)i * VE, acc);
 }
 
-template <typename TY, typename T>
+template <bool FLAT, typename TY, typename T>
 inline int launch_combine(const TY* y, const int32_t* flat_row, T* out, int64_t Tn, int H, int K, cudaStream_t st) {
   const dim3 grid((unsigned)ceil_div(Tn * ceil_div(H, 32 * (16 / (int)sizeof(TY))), kRowWarps));
-  auto kern = K <= 4 ? combine_padded_kernel<TY, T, 4> : combine_padded_kernel<TY, T, 8>;
+  auto kern = K <= 4 ? combine_padded_kernel<TY, T, 4, FLAT> : combine_padded_kernel<TY, T, 8, FLAT>;
   const cudaError_t rc = launch_pdl_opt(true, kern, grid, dim3(kRowWarps * 32), 0, st, y, flat_row, out, Tn, H, K);
   return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
 }

@@ -230,7 +230,7 @@ static int forward_f32_split(const Plan& p, const float* hidden, const float* wg
   }
   if (rc) return rc;
   StageTimer tm(kStageCombine, st);
-  return launch_combine(reinterpret_cast<const float*>(p.yrows), p.rt.flat_row, out, Tn, H, K, st);
+  return launch_combine<false>(reinterpret_cast<const float*>(p.yrows), p.rt.flat_row, out, Tn, H, K, st);
 }
 
 template <typename T>
@@ -303,8 +303,8 @@ static int forward_impl(const void* hidden, const int64_t* ridx, const void* rw,
       if (rc) return rc;
       StageTimer tm(kStageCombine, st);
       if (flat)
-        return launch_combine(reinterpret_cast<const float*>(p.yrows), p.rt.flat_row, reinterpret_cast<T*>(out), Tn, H, K, st);
-      return launch_combine(reinterpret_cast<const T*>(p.yrows), p.rt.flat_row, reinterpret_cast<T*>(out), Tn, H, K, st);
+        return launch_combine<true>(reinterpret_cast<const float*>(p.yrows), p.rt.flat_row, reinterpret_cast<T*>(out), Tn, H, K, st);
+      return launch_combine<false>(reinterpret_cast<const T*>(p.yrows), p.rt.flat_row, reinterpret_cast<T*>(out), Tn, H, K, st);
     }
   } else {
     {
@@ -326,18 +326,18 @@ static int forward_impl(const void* hidden, const int64_t* ridx, const void* rw,
 
 // ---------------------------------------------------------------------------------------------
 // Expert forward on 8-bit operands: routing tables as above, codes and scales of the gathered token rows, of the
-// activations, and fp32 result rows at their flat positions.
+// activations, and fp32 result rows.
 // ---------------------------------------------------------------------------------------------
 struct Fp8Plan {
   Plan t;                        // tables
   int64_t ld = 0;                // pitch of the codes
   uint8_t *x = nullptr, *act = nullptr;
   float *x_scale = nullptr, *act_scale = nullptr;   // [groups, max_rows]
-  float* y = nullptr;            // bf16: [S, H], fp32: [max_rows, H] (see Fp8WeightedRows)
+  float* y = nullptr;            // [max_rows, H]
   size_t bytes = 0;
 };
 
-static Fp8Plan plan_experts_fp8(void* ws, int64_t T, int H, int E, int K, int dtype) {
+static Fp8Plan plan_experts_fp8(void* ws, int64_t T, int H, int E, int K) {
   Fp8Plan p;
   Bump b(ws);
   carve_tables(b, p.t, T, E, K, true);
@@ -347,7 +347,7 @@ static Fp8Plan plan_experts_fp8(void* ws, int64_t T, int H, int E, int K, int dt
   p.act = b.take<uint8_t>((size_t)p.t.max_rows * p.ld);
   p.x_scale = b.take<float>(groups * p.t.max_rows);
   p.act_scale = b.take<float>(groups * p.t.max_rows);
-  p.y = b.take<float>((size_t)(dtype == YAMOE_F32 ? p.t.max_rows : p.t.S) * H);
+  p.y = b.take<float>((size_t)p.t.max_rows * H);
   p.bytes = b.off + 256;
   return p;
 }
@@ -356,7 +356,7 @@ template <typename T>
 static int experts_fp8_impl(const void* hidden, const int64_t* ridx, const void* rw, int rcols, const yamoe_fp8_matrix_t& gate_up,
                             const void* bgu, const yamoe_fp8_matrix_t& down, const void* bd, void* out, int64_t Tn, int H, int E,
                             int K, int64_t cap, void* ws, cudaStream_t st) {
-  const Fp8Plan p = plan_experts_fp8(ws, Tn, H, E, K, sizeof(T) == 4 ? YAMOE_F32 : YAMOE_BF16);
+  const Fp8Plan p = plan_experts_fp8(ws, Tn, H, E, K);
   const RouteTables& rt = p.t.rt;
   int rc;
   {
@@ -369,7 +369,7 @@ static int experts_fp8_impl(const void* hidden, const int64_t* ridx, const void*
     rc = fp8_gather<T>(reinterpret_cast<const T*>(hidden), p.x, p.x_scale, p.ld, p.t.max_rows, rt.flat_row, Tn, H, K, st);
   }
   if (rc) return rc;
-  const Fp8Rows rows{rt.pad_off, rt.header, rt.row_token, rt.row_flat, rt.row_weight, p.t.max_rows, p.t.max_tiles};
+  const Fp8Rows rows{rt.pad_off, rt.header, rt.row_token, rt.row_weight, p.t.max_rows, p.t.max_tiles};
   {
     StageTimer tm(kStageGateUp, st);
     rc = fp8_gate_up<T>(rows, p.x, p.x_scale, p.ld, gate_up, reinterpret_cast<const T*>(bgu), p.act, p.act_scale, H, E, st);
@@ -381,7 +381,7 @@ static int experts_fp8_impl(const void* hidden, const int64_t* ridx, const void*
   }
   if (rc) return rc;
   StageTimer tm(kStageCombine, st);
-  return launch_combine(p.y, rt.flat_row, reinterpret_cast<T*>(out), Tn, H, K, st);
+  return launch_combine<false>(p.y, rt.flat_row, reinterpret_cast<T*>(out), Tn, H, K, st);
 }
 
 // Forward pass that leaves what the backward pass needs in a workspace with the BACKWARD layout:
@@ -413,7 +413,7 @@ static int forward_train_impl(const void* hidden, const int64_t* ridx, const voi
       if ((rc = launch_umma_f32<kFwd>(pair_args(p, act.p, H, wd, H, (int64_t)H * H, 0, H, H, E), act.stride, wrows,
                                       p.max_rows, 16, st)))
         return rc;
-      return launch_combine(yrows, p.rt.flat_row, reinterpret_cast<T*>(out), Tn, H, K, st);
+      return launch_combine<false>(yrows, p.rt.flat_row, reinterpret_cast<T*>(out), Tn, H, K, st);
     }
   }
   const bool convert = saves_planes(dtype, H);
@@ -449,7 +449,7 @@ static int forward_train_impl(const void* hidden, const int64_t* ridx, const voi
       split_rows_kernel<<<row_blocks, kRowWarps * 32, 0, st>>>(actw, p.planes(p.actw, Hp), p.rt.header);
     }
   }
-  return launch_combine(yrows, p.rt.flat_row, reinterpret_cast<T*>(out), Tn, H, K, st);
+  return launch_combine<false>(yrows, p.rt.flat_row, reinterpret_cast<T*>(out), Tn, H, K, st);
 }
 
 // Input, weight and bias gradients in fp32 (the routing-weight gradients are left in p.gw_row).
@@ -1182,7 +1182,7 @@ int yamoe_b200_experts_forward(const void* hidden_states, const int64_t* router_
 
 size_t yamoe_b200_experts_fp8_workspace_bytes(int64_t T, int H, int E, int K, int dtype) {
   if (check_common(T, H, E, K, dtype)) return 0;
-  return plan_experts_fp8(nullptr, T, H, E, K, dtype).bytes;
+  return plan_experts_fp8(nullptr, T, H, E, K).bytes;
 }
 
 int yamoe_b200_experts_fp8_forward(const void* hidden_states, const int64_t* router_indices, const void* routing_weights,
