@@ -57,7 +57,7 @@ def test_experts_refusals(lib):
     f, n = lib.yamoe_b200_experts_fp8_forward, lib.yamoe_b200_experts_fp8_workspace_bytes
     T, H, E, K = 16, 128, 8, 2
     ws = n(T, H, E, K, BF16)
-    assert ws > 0 and n(T, H, E, K, F32) > ws
+    assert ws > 0 and n(T, H, E, K, F32) >= ws
     assert n(T, 130, E, K, BF16) == n(T, H, 2000, K, BF16) == n(T, H, E, K, 5) == 0
 
     def call(x=4096, cols=E, gate_up=matrix(), down=matrix(), cap=4, h=H, dtype=BF16, work=4096, size=ws, out=4096, experts=E):

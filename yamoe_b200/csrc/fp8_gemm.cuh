@@ -8,15 +8,18 @@
 // number per thread and accumulator, and the whole addition is one packed multiply-add for two elements.  With a scale per
 // row of B too (BROWS: weight gradients) the columns' scales go through shared memory.
 //
-// What bounds it are the adding warps, two on each scheduler, and the round trip of an accumulator: instructions, commit, loads
-// and additions, the arrivals, the issuer's wait.  So an accumulator has the whole width of the tile (one wait and one arrival
-// per block and warp), a load of 32 columns is always on its way while those before it are added, across blocks too, and
-// the scales are brought to shared memory by a warp of their own, four blocks at a time.
+// What bounds it, in clocks per block of a 128 x 256 tile (8192 x 5760 x 2880; its four instructions need 512): the
+// instructions alone 623, with the copies of their operands (48 KB) 735, with the additions 1000, of which a third is
+// waiting for loads from TMEM; a tile's end and beginning take another 90.  So an accumulator has the whole width of the
+// tile (one wait and one arrival per block and warp), a load of 32 columns is always on its way while those before it are
+// added, across blocks too (64 columns at a time, refilled half by half, took 5 % longer), the scales are brought to
+// shared memory by a warp of their own, four blocks at a time, and a tile leaves by TMA while the next one is begun.
+// 1.83 PFLOP/s at that size (148 us, 1.1 of what cuBLAS reaches in bf16).
 //
 // Both operands are K-major with 128-byte swizzle: a block of 128 is one swizzle row.  A CTA has tiles of 128 x 256 (CTA pairs
-// with tiles of 256 x 256 were no faster, 150.5 and 151.2 us for 8192 x 5760 x 2880: L2's bytes are not what bounds it, and
-// tiles of 256 rows fit experts' rows less well).  Few tiles: 128 x 128, and a cluster of up to four CTAs shares a
-// tile's blocks (split), the sums of the others meeting in the first one's shared memory, added in order.
+// with tiles of 256 x 256 were no faster, 150.5 and 151.2 us at that size when additions and stores took longer, and tiles
+// of 256 rows fit experts' rows less well).  Few tiles: 128 x 128, and a cluster of up to four CTAs shares a tile's blocks
+// (split); each CTA ends with a share of the columns, to whose sums the others send theirs, added in order.
 //
 // Rows come as they are (B matrices of M rows) or (GROUPED) sorted by expert in the padded layout of the
 // expert pass, an expert's tiles following each other with the row tile varying fastest.
@@ -494,9 +497,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 // ---------------------------------------------------------------------------------------------
 
 // 64 bytes of each of the warp's 32 rows (a lane's own, in `v`) to `dst` (null: nowhere), of which `pieces` of 16 bytes
-// exist.  By way of shared memory, so that four lanes write a row's bytes side by side: straight from the lanes that hold
-// them, 16 bytes to 32 rows at a time, the stores of a 256 x 256 tile of bf16 took 6000 clocks, during which no
-// accumulator is taken up.
+// exist.  By way of shared memory, so that four lanes write a row's bytes side by side.
 __device__ __forceinline__ void store_rows_64(uint32_t park, int lane, const uint4 (&v)[4], char* dst, int pieces) {
 #pragma unroll
   for (int k = 0; k < 4; ++k)
@@ -521,8 +522,9 @@ __device__ __forceinline__ void park_row(const Fp8Tile& t, int box, int k, uint3
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(t.park + box * kFp8BoxBytes + t.lane * 128 + ((k ^ (t.lane & 7)) << 4)),
                "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-// The warp's boxes on their way: rows that exist only in part, and columns, are cut off by the tensor map.  One instruction for 4 KB:
-// a bulk copy for each row took 95 clocks apiece to issue, 3000 for a tile, as long as 16-byte stores of its rows by the lanes.
+// The warp's boxes on their way; rows and columns that do not exist are cut off by the tensor map.  While a tile is stored no
+// accumulator is taken up: 128 x 256 values of bf16 took 6000 clocks by 16-byte stores straight from the lanes that hold
+// the rows, 3450 with four lanes to a row, as long with a bulk copy per row (95 clocks apiece to issue), 1300 as boxes.
 template <int BOXES>
 __device__ __forceinline__ void send_boxes(const Fp8Tile& t, int col, int box_cols) {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
