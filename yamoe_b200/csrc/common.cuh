@@ -160,6 +160,12 @@ inline cudaError_t launch_pdl_opt(bool default_on, void (*kern)(KArgs...), dim3 
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
 }
 
+// The same for kernels without dynamic shared memory that always start early.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_early(void (*kern)(KArgs...), dim3 grid, dim3 block, cudaStream_t st, Args&&... args) {
+  return launch_pdl_opt(true, kern, grid, block, 0, st, std::forward<Args>(args)...);
+}
+
 // Routing tables kept at the head of every workspace (all int32 unless noted).
 struct RouteTables {
   int32_t* header = nullptr;       // [16]: 0 ticket, 1 n_row_tiles, 2 rows_used, 3 dropped, 4 device status, 5 tile pairs

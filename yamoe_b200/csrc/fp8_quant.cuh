@@ -298,7 +298,7 @@ inline int launch_quantize_rows(const T* x, const QuantRows& d, int64_t batch, i
   if (ctas == 0 || batch == 0) return YAMOE_OK;
   if (ctas * kQuantWarps > 0x7fffffff || batch > 65535) return YAMOE_ERR_UNSUPPORTED;
   auto kern = rows_of_16_bytes<T>(x, K) ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
-  const cudaError_t rc = launch_pdl_opt(true, kern, dim3((unsigned)ctas, (unsigned)batch), dim3(kQuantWarps * 32), 0, st, x, d, rows, K);
+  const cudaError_t rc = launch_early(kern, dim3((unsigned)ctas, (unsigned)batch), dim3(kQuantWarps * 32), st, x, d, rows, K);
   return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
 }
 
@@ -312,7 +312,7 @@ inline int launch_quantize_tiles(const T* x, int64_t B, int64_t M, int64_t K, bo
   const bool vec = rows_of_16_bytes<T>(x, K);
   auto kern = block ? (vec ? quantize_tile_kernel<T, true, true> : quantize_tile_kernel<T, false, true>)
                     : (vec ? quantize_tile_kernel<T, true, false> : quantize_tile_kernel<T, false, false>);
-  const cudaError_t rc = launch_pdl_opt(true, kern, grid, dim3(256), 0, st, x, M * K, (int)M, (int)K, out, turned);
+  const cudaError_t rc = launch_early(kern, grid, dim3(256), st, x, M * K, (int)M, (int)K, out, turned);
   return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
 }
 
