@@ -12,6 +12,8 @@
 // Bound by HBM: a value is read once and its code written once, 3 bytes for bf16.  Rows (groups of 1 x 128) need no
 // exchange beyond 16 lanes, which hold a group; blocks and transposed outputs go by tiles of 128 x 128 values held in
 // the registers of a CTA, codes turned around in shared memory.
+// Rows: 4096 x 2880 of bf16 8.6 us (4.1 TB/s, 3 us of it the launch).  Tiles: the transposed codes of the bf16 weights of
+// 32 experts (2880 x 5760), 1.6 GB read and written, 238 us (6.7 TB/s), 252 as one of many calls in a row.
 #pragma once
 #include "common.cuh"
 

@@ -22,6 +22,9 @@
 //    is far from busy, and a weight costs the same number of instructions for one row as for eight.  Within a tile the
 //    reduction index is permuted (the same way for both operands), so that the rows come by 8- or 16-byte loads.
 //
+// 128 experts, H = 2880, K = 4: one token 55 us with bf16 weights (200 MB, 0.55 of copy rate: 23 us are router, launches, first
+// copies, barriers and combine), 43 with e4m3 (100 MB); 16 tokens, 64 experts, H = 2048, K = 8: 167 (712 MB, 0.65).
+//
 // Roundings: logits, softmax, sums and GLU are fp32.  e4m3 weights become f16 exactly, and what they multiply becomes f16
 // times a power of two that brings the largest value of its row to 2^14: token rows exactly but for values under 2^-29 of
 // the largest, activations to 11 bits (under 2^-28 of the largest, 2^-39 of it).  With bf16 weights an activation is

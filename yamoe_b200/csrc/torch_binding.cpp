@@ -305,6 +305,7 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight) {
     check_linear(x, weight);
     const c10::cuda::CUDAGuard guard(x.device());
+    const at::AutoDispatchBelowADInplaceOrView below;      // of what is made here nothing is recorded
     const bool dx = x.requires_grad(), dw = weight.requires_grad();
     Quantised xq, wq, xt, wt;
     quantise(as_matrices(x, weight), 1, &xq, dw ? &xt : nullptr);
@@ -321,6 +322,7 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
     at::Tensor dy = grads[0];
     if (!dy.defined() || !(want_x || want_w)) return {at::Tensor(), at::Tensor()};
     const c10::cuda::CUDAGuard guard(dy.device());
+    const at::AutoDispatchBelowADInplaceOrView below;
     dy = (ctx->saved_data["rank"].toInt() == 3 || dy.dim() == 2 ? dy : dy.reshape({-1, dy.size(-1)})).contiguous();
     Quantised g, gt;
     quantise(dy, 1, want_x ? &g : nullptr, want_w ? &gt : nullptr);
