@@ -9,7 +9,7 @@
 // row of B too (BROWS: weight gradients) the columns' scales go through shared memory.
 //
 // What bounds it, in clocks per block of a 128 x 256 tile (8192 x 5760 x 2880; its four instructions need 512): the
-// instructions alone 623, with the copies of their operands (48 KB) 735, with the additions 1000, of which a third is
+// instructions alone 623, with the copies of their operands (48 KB) 735, with the additions 930, of which a third is
 // waiting for loads from TMEM; a tile's end and beginning take another 90.  So an accumulator has the whole width of the
 // tile (one wait and one arrival per block and warp), a load of 32 columns is always on its way while those before it are
 // added, across blocks too (64 columns at a time, refilled half by half, took 5 % longer), the scales are brought to
