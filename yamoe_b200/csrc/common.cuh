@@ -52,10 +52,22 @@ __device__ __forceinline__ int covered_rows(int count, int padded, int row_round
   return (min(count, padded) + row_round - 1) / row_round * row_round;
 }
 
+// Clamps of the GLU.  NaN stays NaN, as in torch; fminf and fmaxf would make it a bound.
+__device__ __forceinline__ float clamp_gate(float g) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(g), "f"(kLimit));
+  return r;
+}
+__device__ __forceinline__ float clamp_up(float u) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(u), "f"(-kLimit));
+  return clamp_gate(r);
+}
+
 // Clamped SwiGLU of one (gate, up) pre-activation pair.  reference: csrc/moe.cpp:167-180.
 __device__ __forceinline__ float glu_act(float g, float u) {
-  g = fminf(g, kLimit);
-  u = fminf(fmaxf(u, -kLimit), kLimit);
+  g = clamp_gate(g);
+  u = clamp_up(u);
   const float s = __fdividef(1.0f, 1.0f + __expf(-kAlpha * g));
   return (u + 1.0f) * (g * s);
 }

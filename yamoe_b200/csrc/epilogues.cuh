@@ -285,8 +285,8 @@ struct EpiGluBackward {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const float pg = p[2 * i], pu = p[2 * i + 1];
-        const float gc = fminf(pg, kLimit);
-        const float uc = fminf(fmaxf(pu, -kLimit), kLimit);
+        const float gc = clamp_gate(pg);
+        const float uc = clamp_up(pu);
         const float s = __fdividef(1.0f, 1.0f + __expf(-kAlpha * gc));
         const float gate_act = gc * s;
         dot += v[i] * (uc + 1.0f) * gate_act;

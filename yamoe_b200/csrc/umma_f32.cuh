@@ -380,8 +380,8 @@ struct F32GluBackward {             // see PairGluBackward; the gradient leaves 
       const float2 q = ok ? ld_written(src + (size_t)i * H) : make_float2(0.f, 0.f);
       const float w = __shfl_sync(0xffffffffu, w_lane, i);
       const float pg = q.x, pu = q.y;
-      const float gc = fminf(pg, kLimit);
-      const float uc = fminf(fmaxf(pu, -kLimit), kLimit);
+      const float gc = clamp_gate(pg);
+      const float uc = clamp_up(pu);
       const float s = __fdividef(1.0f, 1.0f + __expf(-kAlpha * gc));
       const float gate_act = gc * s;
       dot[i] = ok ? v[i] * (uc + 1.0f) * gate_act : 0.f;

@@ -286,8 +286,8 @@ struct PairGluBackward {
     for (int i = 0; i < 32; ++i) {
       const float w = __shfl_sync(0xffffffffu, w_lane, i);
       const float pg = __uint_as_float(p[i] << 16), pu = __uint_as_float(p[i] & 0xffff0000u);
-      const float gc = fminf(pg, kLimit);
-      const float uc = fminf(fmaxf(pu, -kLimit), kLimit);
+      const float gc = clamp_gate(pg);
+      const float uc = clamp_up(pu);
       const float s = __fdividef(1.0f, 1.0f + __expf(-kAlpha * gc));
       const float gate_act = gc * s;
       const bool ok = (have >> i) & 1u;
