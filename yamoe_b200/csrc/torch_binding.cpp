@@ -333,7 +333,16 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
   }
 };
 
+// Forward mode: a tangent that nobody takes up would count as zero.
+void check_no_tangent(const at::Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), "fp8_linear: forward-mode differentiation is not supported");
+}
+
 at::Tensor fp8_linear_autograd(const at::Tensor& x, const at::Tensor& weight) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
+    check_no_tangent(x);
+    check_no_tangent(weight);
+  }
   if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad())) return Fp8Linear::apply(x, weight);
   at::AutoDispatchBelowAutograd below;
   return fp8_linear_cuda(x, weight);
