@@ -29,3 +29,39 @@ def test_forward_mode_is_refused(which, grad, no_grad):
             yamoe_b200.fp8_linear(*pair)
         primal = [fwAD.unpack_dual(t).primal for t in pair]
         assert torch.equal(yamoe_b200.fp8_linear(*primal), yamoe_b200.fp8_linear(*[t.detach() for t in primal]))
+
+
+@pytest.mark.parametrize("wants", [(True, True), (True, False), (False, True)])
+def test_second_order_is_refused(wants):
+    """Gradients of a gradient do not exist: whoever asks for them gets an error, whoever does not is not disturbed by
+    create_graph."""
+    import yamoe_b200
+    x, w, dy = tensors()
+    x.requires_grad_(wants[0])
+    w.requires_grad_(wants[1])
+    leaves = [t for t in (x, w) if t.requires_grad]
+    plain = torch.autograd.grad(yamoe_b200.fp8_linear(x, w), leaves, dy)
+    first = torch.autograd.grad(yamoe_b200.fp8_linear(x, w), leaves, dy, create_graph=True)
+    for a, b in zip(plain, first):
+        assert torch.equal(a, b) and b.requires_grad
+    # in a loss of its own, and beside a term that has a gradient
+    for extra in (0.0, 1.0):
+        y = yamoe_b200.fp8_linear(x, w)
+        first = torch.autograd.grad(y, leaves, dy, create_graph=True)
+        loss = sum((g.float() ** 2).sum() for g in first) + extra * sum((t.float() ** 2).sum() for t in leaves)
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(loss, leaves, retain_graph=True)
+        with pytest.raises(RuntimeError, match="once"):
+            loss.backward()
+    # in the upstream gradient
+    up = dy.clone().requires_grad_(True)
+    first = torch.autograd.grad(yamoe_b200.fp8_linear(x, w), leaves, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(first[0].float().sum(), up)
+    # a graph that other parts of a model need
+    scale = torch.ones((), device="cuda", requires_grad=True)
+    y = yamoe_b200.fp8_linear(x, w)
+    loss = (y.float() * scale ** 2).sum()
+    (ds,) = torch.autograd.grad(loss, scale, create_graph=True)
+    (dds,) = torch.autograd.grad(ds, scale)
+    assert torch.allclose(dds, 2 * y.detach().float().sum())

@@ -12,6 +12,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <cstdlib>
@@ -300,6 +301,16 @@ at::Tensor fp8_linear_cuda(const at::Tensor& x, const at::Tensor& weight) {
   return mm(xq, wq, x.scalar_type()).view(linear_shape(x, weight));
 }
 
+// Backward computes on codes, below the autograd layer: what it returns has no derivative.  Where a graph of it is asked for
+// (create_graph), it leads through a node that raises when it is differentiated, on to all that it depends on.
+void differentiate_no_further(const at::Tensor& dy, at::Tensor& dx, at::Tensor& dw) {
+  torch::autograd::edge_list on = torch::autograd::get_current_node()->next_edges();
+  for (const torch::autograd::Edge& e : torch::autograd::collect_next_edges(dy)) on.push_back(e);
+  const auto node = std::make_shared<torch::autograd::Error>("fp8_linear can be differentiated once only", std::move(on));
+  for (at::Tensor* t : {&dx, &dw})
+    if (t->defined()) torch::autograd::create_gradient_edge(*t, node);
+}
+
 // y = Q(x) Q(w)^T with dx = Q(dy) Q(w) and dw = Q(dy^T) Q(x^T)^T; what backward needs of x and w is kept as codes.
 struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight) {
@@ -319,16 +330,20 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
     const auto saved = ctx->get_saved_variables();
     const Quantised xt{saved[0], saved[1]}, wt{saved[2], saved[3]};
     const bool want_x = ctx->needs_input_grad(0) && wt.defined(), want_w = ctx->needs_input_grad(1) && xt.defined();
-    at::Tensor dy = grads[0];
+    const at::Tensor dy = grads[0];
     if (!dy.defined() || !(want_x || want_w)) return {at::Tensor(), at::Tensor()};
     const c10::cuda::CUDAGuard guard(dy.device());
-    const at::AutoDispatchBelowADInplaceOrView below;
-    dy = (ctx->saved_data["rank"].toInt() == 3 || dy.dim() == 2 ? dy : dy.reshape({-1, dy.size(-1)})).contiguous();
-    Quantised g, gt;
-    quantise(dy, 1, want_x ? &g : nullptr, want_w ? &gt : nullptr);
     at::Tensor dx, dw;
-    if (want_x) dx = mm(g, wt, dy.scalar_type()).view(ctx->saved_data["x_shape"].toIntVector());
-    if (want_w) dw = mm(gt, xt, dy.scalar_type());
+    {
+      const at::AutoDispatchBelowADInplaceOrView below;
+      const at::Tensor d =
+          (ctx->saved_data["rank"].toInt() == 3 || dy.dim() == 2 ? dy : dy.reshape({-1, dy.size(-1)})).contiguous();
+      Quantised g, gt;
+      quantise(d, 1, want_x ? &g : nullptr, want_w ? &gt : nullptr);
+      if (want_x) dx = mm(g, wt, d.scalar_type()).view(ctx->saved_data["x_shape"].toIntVector());
+      if (want_w) dw = mm(gt, xt, d.scalar_type());
+    }
+    if (at::GradMode::is_enabled()) differentiate_no_further(dy, dx, dw);
     return {dx, dw};
   }
 };
