@@ -65,3 +65,40 @@ def test_second_order_is_refused(wants):
     (ds,) = torch.autograd.grad(loss, scale, create_graph=True)
     (dds,) = torch.autograd.grad(ds, scale)
     assert torch.allclose(dds, 2 * y.detach().float().sum())
+
+
+@pytest.mark.parametrize("M,N,K", [(20, 40, 72), (17, 33, 50), (1, 129, 9), (130, 1, 1)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_saved_tensors_may_come_back_in_another_layout(M, N, K, dtype):
+    import yamoe_b200
+    x, w, dy = tensors(M, N, K, dtype)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    want = torch.autograd.grad(yamoe_b200.fp8_linear(x, w), (x, w), dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = yamoe_b200.fp8_linear(x, w)
+    got = torch.autograd.grad(y, (x, w), dy)
+
+    def shifted(t):                        # one byte off
+        if t.dtype != torch.float8_e4m3fn:
+            return t.contiguous()
+        room = torch.empty(t.numel() + 1, dtype=torch.uint8, device=t.device)[1:].view(t.shape)
+        room.copy_(t.view(torch.uint8) if t.is_contiguous() else t.contiguous().view(torch.uint8))
+        return room.view(t.dtype)
+    with torch.autograd.graph.saved_tensors_hooks(shifted, lambda t: t):
+        y = yamoe_b200.fp8_linear(x, w)
+    odd = torch.autograd.grad(y, (x, w), dy)
+    for a, b, c in zip(want, got, odd):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_saved_tensors_of_several_matrices():
+    import yamoe_b200
+    x, w, dy = (randn(3, *s, seed=i).cuda() for i, s in enumerate(((20, 72), (40, 72), (20, 40))))
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    want = torch.autograd.grad(yamoe_b200.fp8_linear(x, w), (x, w), dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = yamoe_b200.fp8_linear(x, w)
+    for a, b in zip(want, torch.autograd.grad(y, (x, w), dy)):
+        assert torch.equal(a, b)

@@ -328,7 +328,7 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Quantised xt{saved[0], saved[1]}, wt{saved[2], saved[3]};
+    Quantised xt{saved[0], saved[1]}, wt{saved[2], saved[3]};
     const bool want_x = ctx->needs_input_grad(0) && wt.defined(), want_w = ctx->needs_input_grad(1) && xt.defined();
     const at::Tensor dy = grads[0];
     if (!dy.defined() || !(want_x || want_w)) return {at::Tensor(), at::Tensor()};
@@ -336,6 +336,9 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
     at::Tensor dx, dw;
     {
       const at::AutoDispatchBelowADInplaceOrView below;
+      // hooks on saved tensors may give the codes back in a layout of their own
+      if (want_w) xt = operand("fp8_linear", "codes of x", xt.q, xt.scale, (int)xt.q.dim(), false);
+      if (want_x) wt = operand("fp8_linear", "codes of weight", wt.q, wt.scale, (int)wt.q.dim(), true);
       const at::Tensor d =
           (ctx->saved_data["rank"].toInt() == 3 || dy.dim() == 2 ? dy : dy.reshape({-1, dy.size(-1)})).contiguous();
       Quantised g, gt;
