@@ -261,13 +261,13 @@ at::Tensor fp8_mm_cuda(const at::Tensor& a, const at::Tensor& a_scale, const at:
                        at::ScalarType out_dtype) {
   TORCH_CHECK(a.dim() == 2 || a.dim() == 3, "fp8_mm: a must be 2D [M, K] or 3D [B, M, K]");
   TORCH_CHECK(out_dtype == at::kFloat || out_dtype == at::kBFloat16, "fp8_mm: out_dtype must be float32 or bfloat16");
+  TORCH_CHECK(b.device() == a.device() && a_scale.device() == a.device() && b_scale.device() == a.device(),
+              "fp8_mm: tensors must be on one device");
   const c10::cuda::CUDAGuard guard(a.device());
   const Quantised qa = operand("fp8_mm", "a", a, a_scale, a.dim(), false), qb = operand("fp8_mm", "b", b, b_scale, a.dim(), false);
   TORCH_CHECK(a_scale.size(-2) == a.size(-2), "fp8_mm: a must have a scale per row and group of 128");
   TORCH_CHECK(a.size(-1) == b.size(-1), "fp8_mm: a is [.., M, K] and b [.., N, K]: K is ", a.size(-1), " and ", b.size(-1));
   TORCH_CHECK(a.dim() == 2 || a.size(0) == b.size(0), "fp8_mm: a and b must hold the same number of matrices");
-  TORCH_CHECK(b.device() == a.device() && a_scale.device() == a.device() && b_scale.device() == a.device(),
-              "fp8_mm: tensors must be on one device");
   return mm(qa, qb, out_dtype);
 }
 
@@ -446,11 +446,12 @@ std::tuple<at::Tensor, at::Tensor> moe_layer_cuda(const at::Tensor& hidden_state
               "moe_layer: gate_up_bias must be [E, 2*H]");
   TORCH_CHECK(down_bias.dim() == 2 && down_bias.size(0) == E && down_bias.size(1) == H, "moe_layer: down_bias must be [E, H]");
   TORCH_CHECK(K >= 1 && K <= E, "moe_layer: top_k must be between 1 and the number of experts");
-  TORCH_CHECK(gate_up.device() == hidden_states.device() && down.device() == hidden_states.device(),
-              "moe_layer: weights must be on the device of hidden_states");
   const bool fp8 = gate_up.scalar_type() == at::kFloat8_e4m3fn;
   TORCH_CHECK(gate_up_scale.has_value() == fp8 && down_scale.has_value() == fp8,
               "moe_layer: scales belong to float8_e4m3fn weights, and to both of them");
+  TORCH_CHECK(gate_up.device() == hidden_states.device() && down.device() == hidden_states.device() &&
+                  (!fp8 || (gate_up_scale->device() == hidden_states.device() && down_scale->device() == hidden_states.device())),
+              "moe_layer: weights and scales must be on the device of hidden_states");
   const c10::cuda::CUDAGuard guard(hidden_states.device());
   Quantised g, d;
   at::Tensor gu = gate_up, dn = down;
