@@ -1,10 +1,10 @@
-"""`fp8_linear` under autograd beyond one backward pass.
+"""`fp8_linear` under autograd beyond one backward pass, and with nothing to multiply.
 (Its values and gradients: test_gpu_fp8.py.)"""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
-from test_gpu_fp8 import randn
+from test_gpu_fp8 import check_product, dequantised, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +102,26 @@ def test_saved_tensors_of_several_matrices():
         y = yamoe_b200.fp8_linear(x, w)
     for a, b in zip(want, torch.autograd.grad(y, (x, w), dy)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("lead", [(), (5,), (2, 3), (0,), (2, 0), (0, 0), (2, 0, 3)])
+@pytest.mark.parametrize("N,K", [(24, 40), (0, 40), (24, 0), (0, 0)])
+def test_empty_sizes(lead, N, K):
+    """No rows, outputs or inputs: what torch's linear gives, zeros where nothing is summed."""
+    import yamoe_b200
+    x, w = randn(*lead, K, seed=1).cuda().requires_grad_(True), randn(N, K, seed=2).cuda().requires_grad_(True)
+    y = yamoe_b200.fp8_linear(x, w)
+    assert y.shape == (*lead, N)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    assert dx.shape == x.shape and dw.shape == w.shape
+    with torch.no_grad():
+        assert torch.equal(yamoe_b200.fp8_linear(x, w), y)
+    if K == 0:
+        assert not y.any()
+    if N == 0:
+        assert not dx.any()
+    if x.numel() == 0:
+        assert not dw.any()
+    elif N > 0:
+        flat = x.detach().reshape(-1, K).cpu()
+        check_product(y.detach().reshape(-1, N), dequantised(flat, 1), dequantised(w.detach().cpu(), 128), "y")

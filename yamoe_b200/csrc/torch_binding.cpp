@@ -282,9 +282,12 @@ void check_linear(const at::Tensor& x, const at::Tensor& w) {
   TORCH_CHECK(x.size(-1) == w.size(-1), "fp8_linear: x is [.., K] and weight [.., N, K]: K is ", x.size(-1), " and ", w.size(-1));
 }
 
-// x as the matrices that a weight of this rank multiplies
-at::Tensor as_matrices(const at::Tensor& x, const at::Tensor& w) {
-  return (w.dim() == 3 || x.dim() == 2 ? x : x.reshape({-1, x.size(-1)})).contiguous();
+// x (or dy) as the matrices that a weight of this rank multiplies
+at::Tensor as_matrices(const at::Tensor& x, int64_t rank) {
+  if (rank == 3 || x.dim() == 2) return x.contiguous();
+  int64_t rows = 1;                        // (reshape cannot tell it where a row has no values)
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
+  return x.reshape({rows, x.size(-1)}).contiguous();
 }
 std::vector<int64_t> linear_shape(const at::Tensor& x, const at::Tensor& w) {
   std::vector<int64_t> s = x.sizes().vec();
@@ -296,7 +299,7 @@ at::Tensor fp8_linear_cuda(const at::Tensor& x, const at::Tensor& weight) {
   check_linear(x, weight);
   const c10::cuda::CUDAGuard guard(x.device());
   Quantised xq, wq;
-  quantise(as_matrices(x, weight), 1, &xq, nullptr);
+  quantise(as_matrices(x, weight.dim()), 1, &xq, nullptr);
   quantise(weight.contiguous(), kGroup, &wq, nullptr);
   return mm(xq, wq, x.scalar_type()).view(linear_shape(x, weight));
 }
@@ -319,7 +322,7 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
     const at::AutoDispatchBelowADInplaceOrView below;      // of what is made here nothing is recorded
     const bool dx = x.requires_grad(), dw = weight.requires_grad();
     Quantised xq, wq, xt, wt;
-    quantise(as_matrices(x, weight), 1, &xq, dw ? &xt : nullptr);
+    quantise(as_matrices(x, weight.dim()), 1, &xq, dw ? &xt : nullptr);
     quantise(weight.contiguous(), kGroup, &wq, dx ? &wt : nullptr);
     ctx->save_for_backward({xt.q, xt.scale, wt.q, wt.scale});
     ctx->saved_data["x_shape"] = x.sizes().vec();
@@ -339,8 +342,7 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
       // hooks on saved tensors may give the codes back in a layout of their own
       if (want_w) xt = operand("fp8_linear", "codes of x", xt.q, xt.scale, (int)xt.q.dim(), false);
       if (want_x) wt = operand("fp8_linear", "codes of weight", wt.q, wt.scale, (int)wt.q.dim(), true);
-      const at::Tensor d =
-          (ctx->saved_data["rank"].toInt() == 3 || dy.dim() == 2 ? dy : dy.reshape({-1, dy.size(-1)})).contiguous();
+      const at::Tensor d = as_matrices(dy, ctx->saved_data["rank"].toInt());
       Quantised g, gt;
       quantise(d, 1, want_x ? &g : nullptr, want_w ? &gt : nullptr);
       if (want_x) dx = mm(g, wt, d.scalar_type()).view(ctx->saved_data["x_shape"].toIntVector());
