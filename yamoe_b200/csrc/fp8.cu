@@ -187,6 +187,7 @@ int yamoe_b200_moe_layer(const void* hidden_states, const void* router_weight, c
   for (const void* q : wide)
     if (reinterpret_cast<uintptr_t>(q) & 15) return YAMOE_ERR_BAD_ARG;
   if ((reinterpret_cast<uintptr_t>(gate_up_bias) | reinterpret_cast<uintptr_t>(down_bias)) & 3) return YAMOE_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(router_bias) | reinterpret_cast<uintptr_t>(router_scores)) & 1) return YAMOE_ERR_BAD_ARG;
   if (fp8 && (!fp8_matrix_ok(gate_up_fp8, E, H) || !fp8_matrix_ok(down_fp8, E, H))) return YAMOE_ERR_BAD_ARG;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
       workspace_bytes < yamoe_b200_moe_layer_workspace_bytes(T, H, E, K))

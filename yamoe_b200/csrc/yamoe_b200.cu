@@ -1197,7 +1197,11 @@ int yamoe_b200_experts_fp8_forward(const void* hidden_states, const int64_t* rou
   if (T > 0 && (!hidden_states || !router_indices || !routing_weights || !out)) return YAMOE_ERR_BAD_ARG;
   if (!gate_up || !gate_up_bias || !down || !down_bias) return YAMOE_ERR_BAD_ARG;
   if (!fp8_matrix_ok(gate_up, E, H) || !fp8_matrix_ok(down, E, H)) return YAMOE_ERR_BAD_ARG;
-  if ((reinterpret_cast<uintptr_t>(hidden_states) | reinterpret_cast<uintptr_t>(out)) & 15) return YAMOE_ERR_BAD_ARG;
+  const void* wide[] = {hidden_states, out, gate_up_bias, down_bias};
+  for (const void* q : wide)
+    if (reinterpret_cast<uintptr_t>(q) & 15) return YAMOE_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(router_indices) & 7) || (reinterpret_cast<uintptr_t>(routing_weights) & (dtype == YAMOE_F32 ? 3 : 1)))
+    return YAMOE_ERR_BAD_ARG;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
       workspace_bytes < yamoe_b200_experts_fp8_workspace_bytes(T, H, E, K, dtype))
     return YAMOE_ERR_WORKSPACE;
