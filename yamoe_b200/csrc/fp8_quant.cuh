@@ -111,6 +111,10 @@ __device__ __forceinline__ uint2 fp8_codes(const E& e, float inv) {
 // are in flight together.  With `flat_row` a row is a token and goes to the rows of its K assignments (negative: dropped),
 // read once.
 constexpr int kQuantWarps = 8, kQuantPairs = 4;
+// What a warp takes of a row.  A row may have up to 2^31 - 1 values: rounding up passes 31 bits.
+constexpr int kQuantPiece = 2 * kQuantPairs * kFp8Group;
+__host__ __device__ constexpr unsigned quant_pieces(int K) { return ((unsigned)K + kQuantPiece - 1) / kQuantPiece; }
+static_assert(quant_pieces(0x7fffffff) == 1u << 21 && quant_pieces(1) == 1, "");
 
 struct QuantRows {
   uint8_t* q;          // [.., ldq]
@@ -126,10 +130,10 @@ quantize_rows_kernel(const T* x, const QuantRows d, int64_t rows, int K) {
   pdl_trigger();
   const int lane = threadIdx.x & 31, l16 = lane & 15;
   // the pieces of a row are neighbours in the grid
-  const unsigned pieces = (unsigned)((K + 2 * kQuantPairs * kFp8Group - 1) / (2 * kQuantPairs * kFp8Group));
+  const unsigned pieces = quant_pieces(K);
   const unsigned unit = blockIdx.x * kQuantWarps + (threadIdx.x >> 5);
   const int64_t row = unit / pieces;
-  const int k0 = (int)(unit - (unsigned)row * pieces) * (2 * kQuantPairs * kFp8Group) + lane * 8;
+  const int k0 = (int)(unit - (unsigned)row * pieces) * kQuantPiece + lane * 8;
   if (row >= rows) return;
   // Of the expert pass only the tables come from the kernel before this one, which has waited for all that went before itself.
   if (d.flat_row == nullptr) pdl_wait();
@@ -296,7 +300,7 @@ inline bool rows_of_16_bytes(const void* x, int64_t K) {
 // `batch` matrices of `rows` rows
 template <typename T>
 inline int launch_quantize_rows(const T* x, const QuantRows& d, int64_t batch, int64_t rows, int K, cudaStream_t st) {
-  const int64_t ctas = ceil_div(rows * ceil_div(K, 2 * kQuantPairs * kFp8Group), kQuantWarps);
+  const int64_t ctas = ceil_div(rows * quant_pieces(K), kQuantWarps);
   if (ctas == 0 || batch == 0) return YAMOE_OK;
   if (ctas * kQuantWarps > 0x7fffffff || batch > 65535) return YAMOE_ERR_UNSUPPORTED;
   auto kern = rows_of_16_bytes<T>(x, K) ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>;
