@@ -336,7 +336,8 @@ int yamoe_b200_experts_backward_saved(const void *grad_out, int grad_out_per_slo
  *
  * yamoe_fp8_matrix_t describes `batch` matrices of R rows and C columns (given by the call):
  *   q       codes, row pitch `ld` and matrix pitch `q_batch` bytes; q 16-byte aligned, both pitches
- *           multiples of 16, ld >= C.  Bytes between C and ld may be written.
+ *           multiples of 16, ld >= C.  Bytes between C and ld may be written.  Where products read several matrices,
+ *           q_batch is a multiple of ld and at least R * ld.
  *   scale   of (matrix b, row or row block r, column group g) at b * scale_batch + r * scale_row + g * scale_group
  *           (in floats)
  * ------------------------------------------------------------------------------------------- */

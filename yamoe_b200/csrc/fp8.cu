@@ -14,6 +14,10 @@ bool fp8_matrix_ok(const yamoe_fp8_matrix_t* m, int64_t batch, int64_t cols) {
   return batch <= 1 || (m->q_batch > 0 && m->q_batch % 16 == 0 && m->q_batch < (int64_t)1 << 40);
 }
 
+bool fp8_maps_ok(const yamoe_fp8_matrix_t* m, int64_t batch, int64_t rows) {
+  return batch <= 1 || (m->q_batch % m->ld == 0 && m->q_batch / m->ld >= rows);
+}
+
 static QuantOut quant_out(const yamoe_fp8_matrix_t* m) {
   if (m == nullptr) return QuantOut{};
   return QuantOut{reinterpret_cast<uint8_t*>(m->q), m->scale, m->ld, m->q_batch, m->scale_row, m->scale_group, m->scale_batch};
@@ -149,6 +153,7 @@ int yamoe_b200_fp8_mm(const yamoe_fp8_matrix_t* a, const yamoe_fp8_matrix_t* b, 
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
       workspace_bytes < yamoe_b200_fp8_mm_workspace_bytes(batch, M, N, K))
     return YAMOE_ERR_WORKSPACE;
+  if (!fp8_maps_ok(a, batch, M) || !fp8_maps_ok(b, batch, N)) return YAMOE_ERR_BAD_ARG;
   Fp8Params p{};
   p.M = M; p.N = N; p.K = (int)K; p.B = (int)batch;
   p.sa = a->scale; p.sa_b = a->scale_batch; p.sa_m = a->scale_row; p.sa_k = a->scale_group;
@@ -193,6 +198,7 @@ int yamoe_b200_moe_layer(const void* hidden_states, const void* router_weight, c
       workspace_bytes < yamoe_b200_moe_layer_workspace_bytes(T, H, E, K))
     return YAMOE_ERR_WORKSPACE;
   if (T == 0) return YAMOE_OK;
+  if (fp8 && (!fp8_maps_ok(gate_up_fp8, E, 2 * (int64_t)H) || !fp8_maps_ok(down_fp8, E, H))) return YAMOE_ERR_BAD_ARG;
   if (!umma_available()) return YAMOE_ERR_UNSUPPORTED;
   using bf = __nv_bfloat16;
   LayerArgs a{};
@@ -213,7 +219,7 @@ int yamoe_b200_moe_layer(const void* hidden_states, const void* router_weight, c
     a.scale_gu = g.scale; a.gu_b = g.scale_batch; a.gu_r = g.scale_row; a.gu_g = g.scale_group;
     a.scale_dn = d.scale; a.dn_b = d.scale_batch; a.dn_r = d.scale_row; a.dn_g = d.scale_group;
     const uint64_t dg[3] = {h, 2 * h, n}, dd[3] = {h, h, n};
-    const uint64_t sg[2] = {(uint64_t)g.ld, (uint64_t)(E > 1 ? g.q_batch : g.ld)}, sd[2] = {(uint64_t)d.ld, (uint64_t)(E > 1 ? d.q_batch : d.ld)};
+    const uint64_t sg[2] = {(uint64_t)g.ld, E > 1 ? (uint64_t)g.q_batch : 2 * h * g.ld}, sd[2] = {(uint64_t)d.ld, E > 1 ? (uint64_t)d.q_batch : h * d.ld};
     const uint32_t box[3] = {128, kLayerUnit, 1};
     if (!encode_map(&gu, g.q, 3, dg, sg, box, kMapU8) || !encode_map(&dn, d.q, 3, dd, sd, box, kMapU8)) return YAMOE_ERR_CUDA;
     return launch_moe_layer<true>(a, gu, dn, st);

@@ -9,6 +9,8 @@ namespace yb {
 
 // A matrix that the calls of this library read or write: pitches and alignment as the header asks
 bool fp8_matrix_ok(const yamoe_fp8_matrix_t* m, int64_t batch, int64_t cols);
+// The same as tensor maps want it besides: the matrices of `rows` rows one behind the other, a whole number of pitches apart
+bool fp8_maps_ok(const yamoe_fp8_matrix_t* m, int64_t batch, int64_t rows);
 
 // hidden [T, H] -> codes [rows, ld] and scales [groups, scale_group] at the rows of each token's K assignments
 template <typename T>

@@ -794,13 +794,13 @@ inline int launch_fp8_gemm(const Fp8Operand& a, const Fp8Operand& b, const Fp8Ou
   CUtensorMap tmA, tmB, tmOut{};
   const uint64_t na = GROUPED ? 1 : (uint64_t)p.B;
   const uint64_t da[3] = {(uint64_t)p.K, (uint64_t)a.rows, na}, db[3] = {(uint64_t)p.K, (uint64_t)b.rows, (uint64_t)p.B};
-  const uint64_t ga[2] = {(uint64_t)a.ld, (uint64_t)(na > 1 ? a.batch : a.ld)};
-  const uint64_t gb[2] = {(uint64_t)b.ld, (uint64_t)(p.B > 1 ? b.batch : b.ld)};
+  const uint64_t ga[2] = {(uint64_t)a.ld, (uint64_t)(na > 1 ? a.batch : a.ld * a.rows)};
+  const uint64_t gb[2] = {(uint64_t)b.ld, (uint64_t)(p.B > 1 ? b.batch : b.ld * b.rows)};
   const uint32_t boxa[3] = {128, 128, 1}, boxb[3] = {128, BN, 1};
   if (!encode_map(&tmA, a.q, 3, da, ga, boxa, kMapU8) || !encode_map(&tmB, b.q, 3, db, gb, boxb, kMapU8)) return YAMOE_ERR_CUDA;
   if (o.c != nullptr) {
     const uint64_t dim[3] = {(uint64_t)o.cols, (uint64_t)o.rows, (uint64_t)o.batch};
-    const uint64_t pitch[2] = {(uint64_t)(o.cols * o.size), (uint64_t)(o.cols * o.size * (o.batch > 1 ? o.rows : 1))};
+    const uint64_t pitch[2] = {(uint64_t)(o.cols * o.size), (uint64_t)(o.cols * o.size * o.rows)};
     const uint32_t box[3] = {128u / o.size, 32, 1};
     if (!encode_map(&tmOut, o.c, 3, dim, pitch, box, o.size == 2 ? kMapBf16 : kMapF32Swizzled)) return YAMOE_ERR_CUDA;
   }

@@ -161,8 +161,10 @@ yamoe_fp8_matrix_t matrix_of(const Quantised& m) {
   yamoe_fp8_matrix_t r{};
   r.q = m.q.data_ptr();
   r.scale = m.scale.data_ptr<float>();
-  r.ld = m.q.size(-2) > 1 ? m.q.stride(-2) : ceil_div(m.q.size(-1), 16) * 16;
-  r.q_batch = batched && m.q.size(0) > 1 ? m.q.stride(0) : m.q.size(-2) * r.ld;
+  const bool several = batched && m.q.size(0) > 1;
+  // (one row: its pitch is that of the matrices)
+  r.ld = m.q.size(-2) > 1 ? m.q.stride(-2) : several ? m.q.stride(0) : ceil_div(m.q.size(-1), 16) * 16;
+  r.q_batch = several ? m.q.stride(0) : m.q.size(-2) * r.ld;
   r.scale_row = m.scale.stride(-2);
   r.scale_group = m.scale.stride(-1);
   r.scale_batch = batched ? m.scale.stride(0) : 0;
@@ -232,7 +234,9 @@ Quantised operand(const char* op, const char* name, const at::Tensor& q, const a
               op, ": the scale of ", name, " must hold one value per group of ", blocks_only ? "128 x 128" : "1 or 128 x 128");
   const bool ok = q.stride(-1) == 1 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 &&
                   (rows <= 1 || (q.stride(-2) % 16 == 0 && q.stride(-2) >= q.size(-1))) &&
-                  (dim == 2 || q.size(0) <= 1 || (q.stride(0) % 16 == 0 && q.stride(0) > 0));
+                  (dim == 2 || q.size(0) <= 1 ||
+                   (rows <= 1 ? q.stride(0) % 16 == 0 && q.stride(0) >= q.size(-1)
+                              : q.stride(-2) > 0 && q.stride(0) % q.stride(-2) == 0 && q.stride(0) / q.stride(-2) >= rows));
   // one row of a width that is no multiple of 16 may end where its memory ends
   if (ok || q.numel() == 0) return {q, scale};
   Quantised m = empty_quantised(dim == 3, dim == 3 ? q.size(0) : 1, rows, q.size(-1), kGroup, q);

@@ -1206,6 +1206,7 @@ int yamoe_b200_experts_fp8_forward(const void* hidden_states, const int64_t* rou
       workspace_bytes < yamoe_b200_experts_fp8_workspace_bytes(T, H, E, K, dtype))
     return YAMOE_ERR_WORKSPACE;
   if (T == 0) return YAMOE_OK;
+  if (!fp8_maps_ok(gate_up, E, 2 * (int64_t)H) || !fp8_maps_ok(down, E, H)) return YAMOE_ERR_BAD_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == YAMOE_BF16
              ? experts_fp8_impl<__nv_bfloat16>(hidden_states, router_indices, routing_weights, routing_cols, *gate_up, gate_up_bias,
