@@ -7,7 +7,9 @@
 // +-448 whatever way the two divisions are rounded.  A group is 128 neighbours in a row (activations, gradients) or
 // 128 x 128 values (weights), the last ones of a matrix being smaller.
 //
-// The kernels may start before what writes x has ended: x is read by ordinary loads behind the wait for it.
+// The kernels may start before what writes x has ended: x is read by ordinary loads behind the wait for it.  The one exception
+// is the gather of the expert pass, which reads the token rows before its wait: the kernel before it is the routing's, a
+// plain launch, which began when all that went before it had ended; only its tables are waited for.
 //
 // Bound by HBM: a value is read once and its code written once, 3 bytes for bf16.  Rows (groups of 1 x 128) need no
 // exchange beyond 16 lanes, which hold a group; blocks and transposed outputs go by tiles of 128 x 128 values held in
@@ -135,7 +137,7 @@ quantize_rows_kernel(const T* x, const QuantRows d, int64_t rows, int K) {
   const int64_t row = unit / pieces;
   const int k0 = (int)(unit - (unsigned)row * pieces) * kQuantPiece + lane * 8;
   if (row >= rows) return;
-  // Of the expert pass only the tables come from the kernel before this one, which has waited for all that went before itself.
+  // Of the expert pass only the tables come from the kernel before this one, a plain launch: x was there when that one began.
   if (d.flat_row == nullptr) pdl_wait();
   const T* src = after_wait(x) + ((int64_t)blockIdx.y * rows + row) * K;
   Eight<T> v[kQuantPairs];
