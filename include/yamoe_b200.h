@@ -355,8 +355,9 @@ int yamoe_b200_fp8_quantize(const void *x, const yamoe_fp8_matrix_t *out, const 
                             int64_t batch, int64_t M, int64_t K, int block_rows, int dtype, void *stream);
 
 /* out[b] [M, N] = A[b] [M, K] @ B[b] [N, K]^T of quantised matrices, A with groups of 1 x 128, B with
- * groups of b_block_rows (1 or 128) x 128.  Products are summed in fp32, exactly scaled block by block, and
- * rounded once to out_dtype; rows of out are N elements apart, matrices M * N.  The workspace holds the status word. */
+ * groups of b_block_rows (1 or 128) x 128.  Products of a block of 128 are summed in fp32, times the product of the block's two
+ * scales (an fp32 number: it loses bits where it is under 2^-126) added to the other blocks' in fp32, and rounded once
+ * to out_dtype; rows of out are N elements apart, matrices M * N.  The workspace holds the status word. */
 size_t yamoe_b200_fp8_mm_workspace_bytes(int64_t batch, int64_t M, int64_t N, int64_t K);
 int yamoe_b200_fp8_mm(const yamoe_fp8_matrix_t *a, const yamoe_fp8_matrix_t *b, int b_block_rows, void *out,
                       int64_t batch, int64_t M, int64_t N, int64_t K, int out_dtype, void *workspace,
@@ -378,8 +379,9 @@ int yamoe_b200_experts_fp8_forward(const void *hidden_states, const int64_t *rou
  *   the K largest of a token (equal ones: lower id first; NaN above all) and the softmax over them are its experts and
  *   their weights, of which router_scores [T,E] is the dense matrix; out = the expert forward with expert_capacity.
  * bf16 tensors; the weights are either bf16 (gate_up [E,H,2H], down [E,H,H]; gate_up_fp8 and down_fp8 NULL) or quantised as
- * yamoe_b200_experts_fp8_forward takes them (gate_up and down NULL); activations are not quantised.  Sums and weights are
- * fp32, nothing depends on the order in which CTAs finish.
+ * yamoe_b200_experts_fp8_forward takes them (gate_up and down NULL).  Activations are not brought to 8 bits: beside bf16 weights they
+ * are multiplied with 16 bits (the sum of two bf16 numbers), beside e4m3 weights with 11 (f16 times a power of two per row, token rows
+ * too).  Sums and weights are fp32, nothing depends on the order in which CTAs finish.
  * T <= 32, T*K <= 256, K <= 32, K <= E <= 1024, H a multiple of 8 up to 65536: otherwise YAMOE_ERR_UNSUPPORTED, and 0
  * workspace bytes.  The second launch is cooperative: its CTAs, one per SM, wait for one another. */
 size_t yamoe_b200_moe_layer_workspace_bytes(int64_t T, int H, int E, int K);

@@ -15,7 +15,7 @@
 // exchange beyond 16 lanes, which hold a group; blocks and transposed outputs go by tiles of 128 x 128 values held in
 // the registers of a CTA, codes turned around in shared memory.
 // Rows: 4096 x 2880 of bf16 8.6 us (4.1 TB/s, 3 us of it the launch).  Tiles: the transposed codes of the bf16 weights of
-// 32 experts (2880 x 5760), 1.6 GB read and written, 238 us (6.7 TB/s), 252 as one of many calls in a row.
+// 32 experts (2880 x 5760), 1.6 GB read and written, 246 us (6.5 TB/s).
 #pragma once
 #include "common.cuh"
 

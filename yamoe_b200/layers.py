@@ -125,9 +125,10 @@ class Fp8Yamoe(torch.nn.Module):
         layer = Fp8Yamoe.from_layer(block)          # block: as for `Yamoe`; its bf16 expert weights are not kept
         out, router_scores = layer(hidden_states)   # [B, S, H] bf16
 
-    Up to 32 tokens with up to 256 assignments (a decode step) run as `moe_layer`, two launches in all, activations at 16
-    bits and the router's logits unrounded.  More tokens run as `router_forward` and `experts_fp8`, which quantises the
-    token rows and the activations too.  `expert_capacity` None: ceil(T K / E), as in `Yamoe`."""
+    Up to 32 tokens with up to 256 assignments (a decode step) run as `moe_layer`, two launches in
+    all, activations at 11 bits and the router's logits unrounded.  Others run as `router_forward`, whose logits are bf16
+    numbers, and `experts_fp8`, which quantises the token rows and the activations too; so where two logits of a token round to the
+    same number its experts may depend on how many tokens come with it.  `expert_capacity` None: ceil(T K / E), as in `Yamoe`."""
 
     def __init__(self, router_weight, router_bias, gate_up, gate_up_scale, gate_up_bias, down, down_scale, down_bias,
                  top_k, expert_capacity=None):
