@@ -391,6 +391,74 @@ int yamoe_b200_moe_layer(const void *hidden_states, const void *router_weight, c
                          void *router_scores, int64_t T, int H, int E, int K, int64_t expert_capacity, int dtype,
                          void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * The steps of the expert layer, for expert networks that a caller puts together (no counterpart in the reference, whose
+ * gather and scatter are above).  All of them may be captured; their workspaces belong to one call at a time.
+ *
+ * Tokens sorted by expert: assignment p = t*K + k of token t gets row row_of[p], those of expert e in the order of p.
+ *   capacity < 0    rows [T*K, H]: expert e has rows offsets[e] .. offsets[e+1]-1
+ *   capacity C      rows [E, C, H]: expert e has rows e*C .. e*C + n-1, n = offsets[e+1]-offsets[e]; what is behind its first C
+ *                   assignments gets row_of = -1
+ *   row_of  int32 [T*K], -1 for ids outside [0,E) too;  offsets int32 [E+1]: rows given before each expert's
+ * rows[row_of[p]] = hidden_states[t]; the other rows are zero.  H, K >= 0, E <= 1024, fewer than 2^30 assignments, fewer than 2^31 rows.  Elements
+ * need no alignment beyond their own; rows of a multiple of 16 bytes on 16-byte boundaries are moved fastest. */
+size_t yamoe_b200_sort_tokens_workspace_bytes(int64_t T, int E, int K);
+int yamoe_b200_sort_tokens(const void *hidden_states, const int64_t *router_indices, void *rows, int32_t *row_of,
+                           int32_t *offsets, int64_t T, int64_t H, int E, int K, int64_t capacity, int dtype,
+                           void *workspace, size_t workspace_bytes, void *stream);
+
+/* out[t,:] = sum_k w[t,k] rows[row_of[t*K+k],:] in fp32 and in the order of k; entries of row_of outside [0, n_rows) are left out.
+ *   weights   NULL: 1;  [T,K] with router_indices NULL;  [T,E] with router_indices int64 [T,K]: w[t,k] = weights[t, router_indices[t,k]],
+ *             0 for a column that does not exist.  weight_dtype: dtype, or YAMOE_F32.
+ * Without weights this is the gradient of yamoe_b200_sort_tokens. */
+int yamoe_b200_combine_tokens(const void *rows, int64_t n_rows, const int32_t *row_of, const void *weights,
+                              int weight_dtype, const int64_t *router_indices, void *out, int64_t T, int64_t H, int E,
+                              int K, int dtype, void *stream);
+
+/* Its gradients; either output may be NULL (d_weights: has to be without weights).
+ *   d_rows[r,:] = sum of w[p] d_out[t(p),:] over the assignments p with row_of[p] = r, zero without any.  A row of several is summed in
+ *   an order that is not fixed beyond two; the rows of yamoe_b200_sort_tokens have one at most.
+ *   d_weights   like weights: <d_out[t], rows[row_of[t*K+k]]>, 0 where there is no row; with router_indices the sum over the slots of
+ *   a column, 0 for those of none.  K <= 1024. */
+size_t yamoe_b200_combine_tokens_backward_workspace_bytes(int64_t n_rows, int64_t T, int K);
+int yamoe_b200_combine_tokens_backward(const void *d_out, const void *rows, int64_t n_rows, const int32_t *row_of,
+                                       const void *weights, int weight_dtype, const int64_t *router_indices,
+                                       void *d_rows, void *d_weights, int64_t T, int64_t H, int E, int K, int dtype,
+                                       void *workspace, size_t workspace_bytes, void *stream);
+
+/* 8-bit integers with one fp32 scale per row: scale = a / 127 with a = max(max |x|, 2^-100) over the row, codes x * (127 / a) to the nearest
+ * integer (ties to even), every step in fp32.  A row with a NaN or an infinity gets codes 0 and the scale NaN.
+ * yamoe_int8_matrix_t describes `batch` matrices of R rows and C columns (given by the call): codes with row pitch `ld` and matrix
+ * pitch `q_batch` in bytes, q 16-byte aligned, both multiples of 16, ld >= C; bytes between C and ld may be read and written.
+ * Where products read several matrices, q_batch is a multiple of ld and at least R * ld.  The scale of (matrix b, row r) lies at
+ * b * scale_batch + r * scale_row (in floats). */
+typedef struct {
+  void *q;
+  float *scale;
+  int64_t ld, q_batch, scale_row, scale_batch;
+} yamoe_int8_matrix_t;
+
+/* x, dtype [batch, M, K] contiguous -> out: its M rows of K codes, or with `transpose` the K rows of M codes of x^T. */
+int yamoe_b200_int8_quantize(const void *x, const yamoe_int8_matrix_t *out, int64_t batch, int64_t M, int64_t K,
+                             int transpose, int dtype, void *stream);
+
+/* out[b] [M,N] = A[b] [M,K] @ B[b] [N,K]^T of quantised matrices: the sums are exact (K < 2^17), as fp32 times A's scale, times B's, rounded
+ * once to out_dtype.  With offsets (int32 [batch+1], ascending) A is ONE matrix [M,K], rows offsets[e] .. offsets[e+1]-1 of which
+ * are multiplied by B[e]; the other rows of out [M,N] are zero.  batch <= 1024 then.  M, N < 2^30.  The workspace holds the status word. */
+size_t yamoe_b200_int8_mm_workspace_bytes(int64_t batch, int64_t M, int64_t N, int64_t K);
+int yamoe_b200_int8_mm(const yamoe_int8_matrix_t *a, const yamoe_int8_matrix_t *b, const int32_t *offsets, void *out,
+                       int64_t batch, int64_t M, int64_t N, int64_t K, int out_dtype, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/* The clamped GLU of the expert forward on pre-activations [M, 2N] (even columns gate, odd ones up): out [M, N].  With `codes` also the
+ * checkpoint of its backward pass: e4m3 codes of the pre-activations in groups of 1 x 128 (yamoe_b200_fp8_quantize has the definition),
+ * rows of `ld` bytes, 16-byte aligned, ld a multiple of 16 and at least 2N; `scales` fp32 [M, ceil(2N / 128)].  2N < 2^31.
+ * The backward pass is the GLU's derivative at the values of the codes, times d_out [M, N]. */
+int yamoe_b200_glu_forward(const void *pre, void *out, void *codes, float *scales, int64_t ld, int64_t M, int64_t N,
+                           int dtype, void *stream);
+int yamoe_b200_glu_backward(const void *d_out, const void *codes, const float *scales, int64_t ld, void *d_pre,
+                            int64_t M, int64_t N, int dtype, void *stream);
+
 /* Device status word of the last forward/backward call that used `workspace`: 0 when every
  * bounded device-side wait completed, otherwise a code naming the wait that gave up.  Reads
  * 4 bytes from the device with cudaMemcpyAsync on `stream` and synchronises that stream. */

@@ -34,8 +34,15 @@ class Fp8Matrix(ctypes.Structure):
                 [(n, c_int64) for n in ("ld", "q_batch", "scale_row", "scale_group", "scale_batch")])
 
 
+class Int8Matrix(ctypes.Structure):
+    """yamoe_int8_matrix_t of include/yamoe_b200.h."""
+    _fields_ = ([(n, c_void_p) for n in ("q", "scale")] +
+                [(n, c_int64) for n in ("ld", "q_batch", "scale_row", "scale_batch")])
+
+
 _ctx_p = ctypes.POINTER(EpCtx)
 _fp8_p = ctypes.POINTER(Fp8Matrix)
+_int8_p = ctypes.POINTER(Int8Matrix)
 PATH_AUTO, PATH_SIMT, PATH_TCGEN05, PATH_GEMV = 0, 1, 2, 3
 
 # name -> (restype, argtypes); mirrors include/yamoe_b200.h one to one
@@ -91,6 +98,18 @@ SIGNATURES = {
     "yamoe_b200_moe_layer_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
     "yamoe_b200_moe_layer": (c_int, [c_void_p] * 4 + [_fp8_p, c_void_p, c_void_p, _fp8_p, c_void_p, c_void_p, c_void_p] +
                              [c_int64, c_int, c_int, c_int, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
+    "yamoe_b200_sort_tokens_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "yamoe_b200_sort_tokens": (c_int, [c_void_p] * 5 + [c_int64, c_int64, c_int, c_int, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
+    "yamoe_b200_combine_tokens": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64, c_int,
+                                          c_int, c_int, c_void_p]),
+    "yamoe_b200_combine_tokens_backward_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int]),
+    "yamoe_b200_combine_tokens_backward": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                                   c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "yamoe_b200_int8_quantize": (c_int, [c_void_p, _int8_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p]),
+    "yamoe_b200_int8_mm_workspace_bytes": (c_size_t, [c_int64] * 4),
+    "yamoe_b200_int8_mm": (c_int, [_int8_p, _int8_p, c_void_p, c_void_p] + [c_int64] * 4 + [c_int, c_void_p, c_size_t, c_void_p]),
+    "yamoe_b200_glu_forward": (c_int, [c_void_p] * 4 + [c_int64] * 3 + [c_int, c_void_p]),
+    "yamoe_b200_glu_backward": (c_int, [c_void_p] * 3 + [c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
     "yamoe_b200_mbar_wait_probe": (c_int, [c_void_p, ctypes.c_uint64, c_void_p]),
     "yamoe_b200_device_status": (c_int, [c_void_p, c_void_p, ctypes.POINTER(ctypes.c_int32)]),
 }

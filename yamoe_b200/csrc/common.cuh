@@ -178,6 +178,34 @@ inline cudaError_t launch_early(void (*kern)(KArgs...), dim3 grid, dim3 block, c
   return launch_pdl_opt(true, kern, grid, block, 0, st, std::forward<Args>(args)...);
 }
 
+// For the kernels of the expert layer's steps (steps.cu), all of which wait for the one before them before they touch memory.
+template <typename... KArgs, typename... Args>
+inline int launch_behind(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
+  const cudaError_t rc = launch_pdl_opt(true, kern, grid, block, smem, st, std::forward<Args>(args)...);
+  return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
+}
+
+// The same with clusters of `cluster` CTAs; `early`: may start before the kernel in front of it has ended.
+template <typename... KArgs, typename... Args>
+inline int launch_clusters(void (*kern)(KArgs...), int cluster, bool early, dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                           Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled(early) ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t rc = cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+  return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
+}
+
 // Routing tables kept at the head of every workspace (all int32 unless noted).
 struct RouteTables {
   int32_t* header = nullptr;       // [16]: 0 ticket, 1 n_row_tiles, 2 rows_used, 3 dropped, 4 device status, 5 tile pairs

@@ -1,0 +1,666 @@
+// Product of two matrices of 8-bit integers with a scale per row of either (tcgen05 kind::i8, cta_group::2, sm_100a):
+//
+//   C[m, n] = sa[m] * sb[n] * (sum over k of qa[m, k] * qb[n, k])
+//
+// The sum is exact in 32 bits (K < 2^17), so neither tiles nor splits change a result; it is brought to fp32 once, then times sa, times sb
+// (a product of the two scales first could leave the range), and rounded once to the output's type.
+//
+// Three arrangements: one or several pairs of matrices, and rows sorted by expert (offsets[e] .. offsets[e + 1] - 1 times matrix e).
+//
+// int8_pair_kernel.  As in umma_pair.cuh, CTA pairs with the weights' rows (output columns) in the instruction's M dimension, 256 to a pair, and
+// the tokens' rows in its N dimension, any multiple of 32 up to 256: an expert's rows are cut into tiles of equal width wherever they
+// begin, so nothing is padded in memory, and few rows cost few clocks.  A k-block is 128 bytes wide, one swizzle row, 32 KB per CTA; six
+// stages, freed two at a time; two accumulators, so that a tile is scaled and stored while the next is multiplied.  Scales are met in the
+// epilogue alone, unlike the e4m3 products with a scale per 128 (fp8_gemm.cuh), whose sums leave TMEM after every block.
+// Few tiles: a cluster of up to four pairs shares a tile's k-blocks; the chunks of 32 rows are dealt out among the pairs, each of which gets
+// the others' sums of its chunks through distributed shared memory.
+//
+// int8_rows_kernel.  A handful of rows: bound by the bytes of the weights and by latency.  A CTA has 16 output columns and all rows, its eight
+// warps take 64-byte blocks of k in turn, straight from global memory to mma.sync m16n8k32; their sums meet in shared memory.
+//
+// Every wait is bounded as in umma_gemm.cuh.
+#pragma once
+#include <algorithm>
+
+#include "tcgen05.cuh"
+
+namespace yb {
+
+constexpr int kInt8StageBytes = 2 * 128 * 128;           // this CTA's 128 rows of weights and up to 128 of tokens, 128 bytes each
+constexpr int kInt8Stages = 6, kInt8Groups = kInt8Stages / 2;
+constexpr int kInt8EpiWarps = 8, kInt8Threads = 32 * (3 + kInt8EpiWarps);
+constexpr int kInt8RingBytes = kInt8Stages * kInt8StageBytes + 1024;     // + slack for 1024-byte alignment
+constexpr int kInt8MaxSplits = 4;
+constexpr int kInt8ChunkBytes = 128 * 32 * 4;            // sums of 128 columns and 32 rows
+// a pair's chunks of a tile and, for each, the sums of every pair of the cluster
+constexpr int int8_exchange_slots(int splits) { return (8 + splits - 1) / splits * splits; }
+static_assert(int8_exchange_slots(2) * kInt8ChunkBytes <= kInt8Stages * kInt8StageBytes &&
+              int8_exchange_slots(3) * kInt8ChunkBytes <= kInt8Stages * kInt8StageBytes &&
+              int8_exchange_slots(4) * kInt8ChunkBytes <= kInt8Stages * kInt8StageBytes, "the exchange takes the ring's place");
+constexpr int kInt8MaxExperts = 1024;
+
+template <typename T>
+struct Int8Params {
+  int64_t M;                    // rows per matrix, or of all experts
+  int N, K, B;                  // columns, reduction length, matrices (experts)
+  int width;                    // rows of a tile at most, a multiple of 32
+  int MT, NT;                   // tiles of `width` rows per matrix (not grouped), of 256 columns
+  const float* sa;              // scale of (matrix b, row m) at b * sa_b + m * sa_m
+  const float* sb;
+  int64_t sa_b, sa_m, sb_b, sb_n;
+  const int32_t* offsets;       // grouped: [B + 1]
+  T* out;                       // rows N apart, matrices M * N
+  int vec;                      // columns may be stored two at a time
+  int32_t* status;
+  int splits;                   // pairs of a cluster that share a tile's k-blocks; a cluster has one tile then
+};
+
+__device__ __forceinline__ void tc2_mma_int8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// arrives on the barrier at this shared-memory offset in the CTAs of `mask` once every MMA issued so far is done
+__device__ __forceinline__ void tc2_commit_to(uint32_t bar, uint16_t mask) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(bar), "h"(mask) : "memory");
+}
+
+// Row `e` of the experts' table, kept within the rows that there are
+__device__ __forceinline__ int int8_offset(const int32_t* offsets, int e, int64_t M) {
+  return (int)max((int64_t)0, min((int64_t)offsets[e], M));
+}
+
+template <typename T>
+__device__ __forceinline__ void int8_zero_row(T* row, int N, int first, int step) {
+  for (int n = first; n < N; n += step) DT<T>::st(row + n, 0.f);
+}
+
+// 32 rows of this lane's column m as sums v: scaled and stored, rows `row` .. row + nvalid - 1 of `out`.
+template <typename T>
+__device__ __forceinline__ void int8_store(const Int8Params<T>& p, T* out, const float* sa, float sb, int m, int64_t row, int nvalid, int lane,
+                                           const uint32_t (&v)[32]) {
+  const float sa_lane = lane < nvalid ? sa[(row + lane) * p.sa_m] : 0.f;
+  float x[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) x[i] = (float)(int)v[i] * __shfl_sync(0xffffffffu, sa_lane, i) * sb;
+  T* at = out + row * p.N + m;
+  if (sizeof(T) == 2 && p.vec) {
+    // neighbouring lanes hold neighbouring columns: the even one stores both of the first sixteen rows, the odd one of the others
+    const bool odd = lane & 1;
+    const int t0 = odd ? 16 : 0;
+    at -= odd;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float got = __shfl_xor_sync(0xffffffffu, odd ? x[i] : x[16 + i], 1);
+      const __nv_bfloat162 two = __floats2bfloat162_rn(odd ? got : x[i], odd ? x[16 + i] : got);
+      if (t0 + i < nvalid && m < p.N) *reinterpret_cast<__nv_bfloat162*>(at + (int64_t)(t0 + i) * p.N) = two;
+    }
+  } else if (m < p.N) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < nvalid) DT<T>::st(at + (int64_t)i * p.N, x[i]);
+  }
+}
+
+template <typename T, bool GROUPED>
+__global__ void __launch_bounds__(kInt8Threads, 1)
+int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                 const __grid_constant__ CUtensorMap tmXsmall, const Int8Params<T> p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_full[kInt8Stages];       // used in the leader CTA of the pair
+  __shared__ __align__(8) uint64_t bar_empty[kInt8Groups];      // per CTA
+  __shared__ __align__(8) uint64_t bar_tmem_full[2];            // per CTA
+  __shared__ __align__(8) uint64_t bar_tmem_empty[2];           // used in the leader CTA
+  __shared__ uint32_t tmem_base_slot;
+  __shared__ int abort_flag;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t cta = cluster_ctarank(), rank = cta & 1, lead = cta & ~1u;
+  const bool leader = rank == 0;
+  const uint16_t pair_mask = (uint16_t)(3u << lead);
+  const int splits = GROUPED ? 1 : p.splits, part = (int)(cta >> 1);
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  int32_t* s_row = reinterpret_cast<int32_t*>(smem_raw + kInt8RingBytes);      // grouped: [B + 1] first row of each expert
+  int32_t* s_tile = s_row + p.B + 1;                                           // grouped: [B + 1] row tiles before each expert's
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kInt8Stages; ++s) mbar_init(smem_u32(&bar_full[s]), 2);   // arrive.expect_tx of both CTAs
+    for (int s = 0; s < kInt8Groups; ++s) mbar_init(smem_u32(&bar_empty[s]), 1);
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&bar_tmem_full[a]), 1);
+      mbar_init(smem_u32(&bar_tmem_empty[a]), 2 * kInt8EpiWarps);
+    }
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_base_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();          // the peers' barriers exist before any remote signal is sent
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_slot;
+  pdl_trigger();
+  pdl_wait();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = kStatusOk;        // waits give up after seconds at the earliest
+  if constexpr (GROUPED) {
+    const int32_t* offsets = after_wait(p.offsets);
+    for (int i = threadIdx.x; i <= p.B; i += kInt8Threads) s_row[i] = int8_offset(offsets, i, p.M);
+    __syncthreads();
+    if (warp == 0) {
+      int before = 0;
+      for (int e0 = 0; e0 < p.B; e0 += 32) {
+        const int e = e0 + lane;
+        int tiles = e < p.B ? (max(0, s_row[e + 1] - s_row[e]) + p.width - 1) / p.width : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, tiles, o);
+          if (lane >= o) tiles += up;
+        }
+        if (e < p.B) s_tile[e + 1] = before + tiles;
+        before += __shfl_sync(0xffffffffu, tiles, 31);
+      }
+      if (lane == 0) s_tile[0] = 0;
+    }
+    __syncthreads();
+  }
+  const int64_t total = (GROUPED ? (int64_t)s_tile[p.B] : (int64_t)p.B * p.MT) * p.NT;
+  const int64_t first_id = blockIdx.x / (2 * splits), n_workers = gridDim.x / (2 * splits);
+  const int kblocks_all = (p.K + 127) >> 7;
+  const int kb_first = part * kblocks_all / splits, kb_end = (part + 1) * kblocks_all / splits;
+
+  // work item -> matrix or expert, first column, first row, its end, width (a multiple of 32)
+  auto decode = [&](int64_t id, int& b, int& m0, int64_t& row0, int64_t& row_end, int& width) {
+    int local, tiles;
+    int64_t first, rows;
+    if constexpr (GROUPED) {
+      const int tile = (int)(id / p.NT);                // experts' tiles follow each other, NT items to each
+      int lo = 0, hi = p.B;                             // the last expert whose first tile is not behind this one
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_tile[mid] <= tile) lo = mid; else hi = mid;
+      }
+      b = lo;
+      tiles = s_tile[b + 1] - s_tile[b];
+      local = (int)(id - (int64_t)s_tile[b] * p.NT);
+      first = s_row[b];
+      rows = s_row[b + 1] - first;
+    } else {
+      const int64_t per = (int64_t)p.MT * p.NT;
+      b = (int)(id / per);
+      local = (int)(id - b * per);
+      tiles = p.MT;
+      first = 0;
+      rows = p.M;
+    }
+    // the row tile varies fastest, so that the pairs running at a time share weights in L2
+    const int nt = local / tiles;
+    const int step = (int)(((rows + tiles - 1) / tiles + 31) & ~31);
+    m0 = nt * 256;
+    row0 = first + (int64_t)(local - nt * tiles) * step;
+    row_end = min(first + rows, row0 + step);
+    width = (int)((row_end - row0 + 31) & ~31);          // (tiles of at most 256 rows, rounded up to 32: none is left without rows)
+  };
+
+  if (warp == 0 || warp == 2 + kInt8EpiWarps) {
+    // =========================== TMA producers (both CTAs) ===================================
+    // one warp for the weights, which also announces the bytes of both, and one for the tokens
+    const bool for_w = warp == 0;
+    const bool elected = elect_one();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int64_t id = first_id; id < total && ok; id += n_workers) {
+      int b, m0, width;
+      int64_t row0, row_end;
+      decode(id, b, m0, row0, row_end, width);
+      const int half = width >> 1, my_m = m0 + (int)rank * 128, my_row = (int)row0 + (int)rank * half;
+      const bool load_w = my_m < p.N;      // nothing of this CTA's columns exists: its results are not read
+      const bool big = half > 96;
+      const int small = (half + 31) >> 5;
+      const uint32_t bytes = (load_w ? 128 * 128 : 0) + (big ? 128 * 128 : small * 4096);
+      for (int kb = kb_first; kb < kb_end; ++kb) {
+        if ((stage & 1) == 0) {
+          ok = mbar_wait_warp(smem_u32(&bar_empty[stage >> 1]), phase ^ 1u, &abort_flag);
+          if (!ok) break;
+        }
+        if (elected) {
+          const uint32_t full = mapa_u32(smem_u32(&bar_full[stage]), lead);
+          const uint32_t sw = smem_base + stage * kInt8StageBytes, sx = sw + 128 * 128;
+          const int k0 = kb * 128;
+          if (for_w) {
+            mbar_expect_tx_cluster(full, bytes);
+            if (load_w) tma2_load_3d(sw, &tmW, k0, my_m, b, full);
+          } else if (big) {
+            tma2_load_3d(sx, &tmX, k0, my_row, GROUPED ? 0 : b, full);
+          } else {
+            for (int i = 0; i < small; ++i) tma2_load_3d(sx + i * 4096, &tmXsmall, k0, my_row + 32 * i, GROUPED ? 0 : b, full);
+          }
+        }
+        __syncwarp();
+        if (++stage == kInt8Stages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    // the commits that free the last stages must have arrived here before this CTA ends
+    for (int g = 0; g < kInt8Groups && ok; ++g)
+      ok = mbar_wait_warp(smem_u32(&bar_empty[g]), 2 * g < stage ? phase : phase ^ 1u, &abort_flag);
+    if (!ok && lane == 0) {
+      abort_flag = 1;
+      atomicMax(p.status, (int)kStatusProducerTimeout);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // =========================== MMA issuer (leader CTA only) ================================
+    if (leader) {
+      // s8 x s8 -> s32, both K-major; without its N field (bits 17..22 = N / 8), which depends on the tile
+      constexpr uint32_t idesc_base = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(256 >> 4) << 24);
+      const uint64_t wdesc0 = make_smem_desc(smem_base, 16, 1024), xdesc0 = make_smem_desc(smem_base + 128 * 128, 16, 1024);
+      const bool elected = elect_one();
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int64_t id = first_id; id < total && ok; id += n_workers) {
+        int b, m0, width;
+        int64_t row0, row_end;
+        decode(id, b, m0, row0, row_end, width);
+        const uint32_t idesc = idesc_base | ((uint32_t)(width >> 3) << 17);
+        ok = mbar_wait_warp(smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, &abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        for (int kb = kb_first; kb < kb_end; ++kb) {
+          ok = mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          if (elected) {
+            const uint64_t wdesc = wdesc0 + (uint64_t)(stage * (kInt8StageBytes >> 4));
+            const uint64_t xdesc = xdesc0 + (uint64_t)(stage * (kInt8StageBytes >> 4));
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tc2_mma_int8(tmem_base + acc * 256, wdesc + (uint64_t)(2 * k), xdesc + (uint64_t)(2 * k), idesc, (uint32_t)(kb != kb_first || k != 0));
+            if (stage & 1) tc2_commit_to(smem_u32(&bar_empty[stage >> 1]), pair_mask);
+            if (kb == kb_end - 1) tc2_commit_to(smem_u32(&bar_tmem_full[acc]), pair_mask);
+          }
+          __syncwarp();
+          if (++stage == kInt8Stages) { stage = 0; phase ^= 1u; }
+        }
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1u;
+      }
+      if (ok && (stage & 1) && elected) tc2_commit_to(smem_u32(&bar_empty[stage >> 1]), pair_mask);   // a group that is half used
+      if (!ok && lane == 0) {
+        abort_flag = 1;
+        atomicMax(p.status, (int)kStatusMmaTimeout);
+      }
+    }
+    __syncwarp();
+  } else {
+    // =========================== epilogue (warps 2 .. 9 of both CTAs) ========================
+    const int q = warp & 3;                    // TMEM lane quarter this warp may read
+    const int turn = (warp - 2) >> 2;          // takes every other chunk of 32 rows
+    const float* sa = after_wait(p.sa);
+    const float* sb = after_wait(p.sb);
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int64_t id = first_id; id < total; id += n_workers) {
+      int b, m0, width;
+      int64_t row0, row_end;
+      decode(id, b, m0, row0, row_end, width);
+      const int m = m0 + (int)rank * 128 + q * 32 + lane;
+      const bool mine = m - lane < p.N;
+      const int chunks = width >> 5;
+      const float scale = m < p.N ? sb[b * p.sb_b + m * p.sb_n] : 0.f;
+      const float* sa_b = sa + (GROUPED ? 0 : b * p.sa_b);
+      T* out = p.out + (GROUPED ? 0 : (int64_t)b * p.M * p.N);
+      const bool ok = mbar_wait_warp(smem_u32(&bar_tmem_full[acc]), acc_phase, &abort_flag);
+      if (!ok) {
+        abort_flag = 1;
+        atomicMax(p.status, (int)kStatusEpilogueTimeout);
+      }
+      const uint32_t t_row = tmem_base + acc * 256 + ((uint32_t)(q * 32) << 16);
+      if (splits > 1) {
+        const uint32_t at = (uint32_t)(q * 32 + lane) * 16;
+        tc_fence_after();
+        cluster_sync_all();                    // everyone's copies and instructions are done with their shared memory
+        if (ok && mine) {
+          for (int c = turn; c < chunks; c += 2) {
+            const int owner = c % splits;
+            if (owner == part) continue;
+            uint32_t v[32];
+            tc_ld_32x32_issue(t_row + c * 32, v);
+            tc_ld_wait(v);
+            const uint32_t dst = mapa_u32(smem_base, 2 * owner + rank) + (c / splits * splits + part) * kInt8ChunkBytes + at;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (uint32_t)i * 2048u), "r"(v[4 * i]), "r"(v[4 * i + 1]),
+                           "r"(v[4 * i + 2]), "r"(v[4 * i + 3]) : "memory");
+          }
+        }
+        cluster_sync_all();
+        if (ok && mine) {
+          for (int c = turn; c < chunks; c += 2) {
+            if (c % splits != part) continue;
+            uint32_t v[32];
+            tc_ld_32x32_issue(t_row + c * 32, v);
+            tc_ld_wait(v);
+            for (int o = 0; o < splits; ++o) {
+              if (o == part) continue;
+              const uint32_t src = smem_base + (c / splits * splits + o) * kInt8ChunkBytes + at;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                uint32_t x[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                             : "r"(src + (uint32_t)i * 2048u) : "memory");
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[4 * i + j] += x[j];
+              }
+            }
+            int8_store(p, out, sa_b, scale, m, row0 + c * 32, (int)min((int64_t)32, row_end - row0 - c * 32), lane, v);
+          }
+        }
+        break;
+      }
+      if (!ok) break;
+      tc_fence_after();
+      if (mine) {
+#pragma unroll 1
+        for (int c = turn; c < chunks; c += 2) {
+          uint32_t v[32];
+          tc_ld_32x32_issue(t_row + c * 32, v);
+          tc_ld_wait(v);
+          int8_store(p, out, sa_b, scale, m, row0 + c * 32, (int)min((int64_t)32, row_end - row0 - c * 32), lane, v);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&bar_tmem_empty[acc]), lead));
+      acc ^= 1;
+      if (acc == 0) acc_phase ^= 1u;
+    }
+    if constexpr (GROUPED) {                   // rows of no expert
+      const int64_t step = (int64_t)gridDim.x * kInt8EpiWarps;
+      for (int64_t r = (int64_t)blockIdx.x * kInt8EpiWarps + warp - 2; r < p.M; r += step) {
+        if (r >= s_row[0] && r < s_row[p.B]) {
+          r += (s_row[p.B] - 1 - r) / step * step;         // on to the last one of its own among the experts' rows
+          continue;
+        }
+        int8_zero_row(p.out + r * p.N, p.N, lane, 32);
+      }
+    }
+  }
+  if (splits > 1 && (warp < 2 || warp >= 2 + kInt8EpiWarps)) {      // what the epilogue's warps meet in
+    cluster_sync_all();
+    cluster_sync_all();
+  }
+
+  // ---- teardown ---------------------------------------------------------------------------
+  tc_fence_before();
+  __syncthreads();
+  if (abort_flag != 0) {
+    // give copies that may still be in flight time to land before the shared memory is released
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  cluster_sync_all();          // no CTA releases shared memory or TMEM that another may still use
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+// ---- a handful of rows ----------------------------------------------------------------------------------------------------
+constexpr int kInt8RowsThreads = 256;
+
+__device__ __forceinline__ void mma_int8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the first `n` bytes of a word
+__device__ __forceinline__ uint32_t first_bytes(uint32_t w, int n) { return n >= 4 ? w : n <= 0 ? 0u : w & ((1u << (8 * n)) - 1u); }
+
+struct Int8Rows {
+  const uint8_t* x;             // codes of the tokens [B, M, ldx]
+  const uint8_t* w;             // of the weights [B, N, ldw]
+  int64_t ldx, x_batch, ldw, w_batch;
+};
+
+// blockIdx.x: 16 columns; blockIdx.y: matrix, or (GROUPED) the experts that have rows, one after the other.  8 * NT rows at a time; U blocks
+// of 64 bytes of each row are on their way together.
+//
+// A sum does not depend on the order of its terms: lane (g, t) takes 16 neighbouring bytes of rows g and g + 8, words 0 and 1 of which are one
+// instruction's k, 2 and 3 the next one's, of weights and tokens alike.
+template <typename T, int NT, int U, bool GROUPED>
+__global__ void __launch_bounds__(kInt8RowsThreads)
+int8_rows_kernel(const Int8Rows d, const Int8Params<T> p) {
+  constexpr int kRows = 8 * NT;
+  __shared__ int s_sum[8][kRows][17];
+  __shared__ int s_count[8], s_expert;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16;
+  pdl_trigger();
+  pdl_wait();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.status = kStatusOk;
+  int b = blockIdx.y;
+  int64_t row0 = 0, row_end = p.M;
+  if constexpr (GROUPED) {
+    const int32_t* offsets = after_wait(p.offsets);
+    unsigned have[4];
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {              // 128 experts to a warp
+      const int e = warp * 128 + i * 32 + lane;
+      have[i] = __ballot_sync(0xffffffffu, e < p.B && int8_offset(offsets, min(e, p.B - 1) + 1, p.M) > int8_offset(offsets, min(e, p.B - 1), p.M));
+      count += __popc(have[i]);
+    }
+    if (lane == 0) s_count[warp] = count;
+    if (threadIdx.x == 0) s_expert = -1;
+    __syncthreads();
+    int index = b;
+    for (int w = 0; w < warp; ++w) index -= s_count[w];
+    if (index >= 0 && index < count) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = __popc(have[i]);
+        if (index >= 0 && index < c && lane == 0) s_expert = warp * 128 + i * 32 + (int)__fns(have[i], 0, index + 1);
+        index -= c;
+      }
+    }
+    __syncthreads();
+    if (blockIdx.y == 0) {                     // rows of no expert
+      const int first = int8_offset(offsets, 0, p.M), end = int8_offset(offsets, p.B, p.M), n = n0 + (threadIdx.x & 15);
+      if (n < p.N)
+        for (int64_t r = threadIdx.x >> 4; r < p.M; r += kInt8RowsThreads / 16)
+          if (r < first || r >= end) DT<T>::st(p.out + r * p.N + n, 0.f);
+    }
+    b = s_expert;
+    if (b < 0) return;
+    row0 = int8_offset(offsets, b, p.M);
+    row_end = int8_offset(offsets, b + 1, p.M);
+  }
+  const uint8_t* w = after_wait(d.w) + b * d.w_batch + 16 * t;
+  const uint8_t* x = after_wait(d.x) + (GROUPED ? 0 : b * d.x_batch) + 16 * t;
+  const float* sa = after_wait(p.sa) + (GROUPED ? 0 : b * p.sa_b);
+  const float* sb = after_wait(p.sb) + b * p.sb_b;
+  T* out = p.out + (GROUPED ? 0 : (int64_t)b * p.M * p.N);
+  const uint8_t* w0 = w + (int64_t)min(n0 + g, p.N - 1) * d.ldw;           // columns that do not exist: computed and not stored
+  const uint8_t* w1 = w + (int64_t)min(n0 + g + 8, p.N - 1) * d.ldw;
+  const int blocks = (p.K + 63) >> 6;
+  for (; row0 < row_end; row0 += kRows) {
+    int c[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[j][i] = 0;
+    const uint8_t* xr[NT];
+    bool there[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      there[j] = row0 + 8 * j + g < row_end;
+      xr[j] = x + (there[j] ? row0 + 8 * j + g : row0) * d.ldx;
+    }
+    for (int blk = warp; blk < blocks; blk += 8 * U) {
+      uint4 a0[U], a1[U], v[U][NT];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        // bytes of this lane's sixteen that exist; those of a row's end are read with it, as pitches are multiples of 16, and masked
+        const int k = (blk + 8 * u) * 64, left = p.K - k - 16 * t;
+        a0[u] = a1[u] = make_uint4(0, 0, 0, 0);
+        if (left > 0) {
+          a0[u] = ld_written(reinterpret_cast<const uint4*>(w0 + k));
+          a1[u] = ld_written(reinterpret_cast<const uint4*>(w1 + k));
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          v[u][j] = make_uint4(0, 0, 0, 0);
+          if (left > 0 && there[j]) v[u][j] = ld_written(reinterpret_cast<const uint4*>(xr[j] + k));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int left = p.K - (blk + 8 * u) * 64 - 16 * t;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          uint4 z = v[u][j];
+          if (left < 16) z = make_uint4(first_bytes(z.x, left), first_bytes(z.y, left - 4), first_bytes(z.z, left - 8), first_bytes(z.w, left - 12));
+          mma_int8(c[j], a0[u].x, a1[u].x, a0[u].y, a1[u].y, z.x, z.y);
+          mma_int8(c[j], a0[u].z, a1[u].z, a0[u].w, a1[u].w, z.z, z.w);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s_sum[warp][8 * j + 2 * t + (i & 1)][g + 8 * (i >> 1)] = c[j][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kRows * 16; i += kInt8RowsThreads) {
+      const int r = i >> 4, n = n0 + (i & 15);
+      if (row0 + r < row_end && n < p.N) {
+        int sum = 0;
+#pragma unroll
+        for (int v = 0; v < 8; ++v) sum += s_sum[v][r][i & 15];
+        DT<T>::st(out + (row0 + r) * p.N + n, (float)sum * sa[(row0 + r) * p.sa_m] * sb[n * p.sb_n]);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+struct Int8Operand {
+  const void* q;
+  int64_t rows, ld, batch;
+};
+
+inline bool int8_map(CUtensorMap* m, const Int8Operand& o, int K, int B, uint32_t box_rows) {
+  const uint64_t dims[3] = {(uint64_t)K, (uint64_t)o.rows, (uint64_t)B};
+  const uint64_t strides[2] = {(uint64_t)o.ld, B > 1 ? (uint64_t)o.batch : (uint64_t)(o.ld * o.rows)};
+  const uint32_t box[3] = {128, box_rows, 1};
+  return encode_map(m, o.q, 3, dims, strides, box, kMapU8);
+}
+
+inline int int8_pair_smem(int experts) { return kInt8RingBytes + (experts > 0 ? 2 * (experts + 1) * 4 : 0); }
+
+// Clusters of `cluster` CTAs of a kernel that run at the same time (asked once per kernel, size and device).
+template <auto kern>
+inline int int8_resident(int cluster, int smem) {
+  static PerDevice<int> known[2 * kInt8MaxSplits + 1];
+  const int dev = current_device_index();
+  int n = known[cluster].get(dev);
+  if (n > 0) return n;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(umma_sm_count() / cluster * cluster));
+  cfg.blockDim = dim3(kInt8Threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+    (void)cudaGetLastError();
+    n = std::max(1, umma_sm_count() / cluster);
+  }
+  known[cluster].set(dev, n);
+  return n;
+}
+
+// Tiles of a product that is not grouped, by estimated clocks.  A k-block takes a pair 2 clocks per row of the tile, or as long as
+// its operands take to come, 128 rows of weights and half of the tile's rows at 64 bytes per clock and CTA; a tile's beginning and end some
+// 2500, meeting in shared memory 1500 more.
+struct Int8Choice { int width, splits; };
+template <auto kern>
+inline Int8Choice int8_choose(int64_t B, int64_t M, int64_t N, int64_t K, int smem) {
+  const int64_t kb = ceil_div(K, 128), NT = ceil_div(N, 256);
+  Int8Choice best{256, 1};
+  double least = 1e30;
+  for (int width = 32; width <= 256; width += 32) {
+    const int64_t MT = ceil_div(M, width);
+    const int even = (int)round_up(ceil_div(M, MT), 32);           // what the tiles come to
+    if (even != width) continue;
+    for (int s = 1; s <= kInt8MaxSplits && s <= kb; ++s) {
+      const int64_t tiles = B * MT * NT, room = std::max(1, int8_resident<kern>(2 * s, smem));
+      if (s > 1 && tiles > room) break;                            // a cluster has one tile
+      const double block = std::max(2.0 * width, 256.0 + width);
+      const double t = (double)ceil_div(tiles, room) * ((double)ceil_div(kb, s) * block + 2500) + (s > 1 ? 1500 : 0);
+      if (t < least) { least = t; best = Int8Choice{width, s}; }
+    }
+  }
+  return best;
+}
+
+template <typename T, bool GROUPED>
+inline int launch_int8_pair(const Int8Operand& X, const Int8Operand& W, Int8Params<T> p, cudaStream_t st) {
+  if (!umma_available()) return YAMOE_ERR_UNSUPPORTED;
+  CUtensorMap tmW, tmX, tmXs;
+  if (!int8_map(&tmW, W, p.K, p.B, 128) || !int8_map(&tmX, X, p.K, GROUPED ? 1 : p.B, 128) || !int8_map(&tmXs, X, p.K, GROUPED ? 1 : p.B, 32))
+    return YAMOE_ERR_CUDA;
+  constexpr auto kern = int8_pair_kernel<T, GROUPED>;
+  const int most = int8_pair_smem(GROUPED ? kInt8MaxExperts : 0), smem = int8_pair_smem(GROUPED ? p.B : 0);
+  p.NT = (int)ceil_div(p.N, 256);
+  const int pairs = int8_resident<kern>(2, most);
+  if (pairs <= 0) return YAMOE_ERR_CUDA;
+  if constexpr (GROUPED) {
+    p.width = 256;
+    p.splits = 1;
+    const int64_t tiles = (ceil_div(p.M, p.width) + std::min<int64_t>(p.B, p.M)) * p.NT;       // at most
+    return launch_clusters(kern, 2, true, dim3((unsigned)(2 * std::min<int64_t>(tiles, pairs))), dim3(kInt8Threads), smem, st, tmW, tmX, tmXs, p);
+  } else {
+    const Int8Choice c = int8_choose<kern>(p.B, p.M, p.N, p.K, most);
+    p.width = c.width;
+    p.splits = c.splits;
+    p.MT = (int)ceil_div(p.M, c.width);
+    const int64_t tiles = (int64_t)p.B * p.MT * p.NT;
+    const int64_t grid = c.splits > 1 ? 2 * c.splits * tiles : 2 * std::min<int64_t>(tiles, pairs);
+    // (clusters of four and more start behind the kernel before them: while that one holds SMs they would be placed badly)
+    return launch_clusters(kern, 2 * c.splits, c.splits == 1, dim3((unsigned)grid), dim3(kInt8Threads), smem, st, tmW, tmX, tmXs, p);
+  }
+}
+
+template <typename T, bool GROUPED>
+inline int launch_int8_rows(const Int8Rows& d, const Int8Params<T>& p, cudaStream_t st) {
+  const dim3 grid((unsigned)ceil_div(p.N, 16), (unsigned)(GROUPED ? std::min<int64_t>(p.B, p.M) : p.B));
+  auto kern = p.M <= 8 ? int8_rows_kernel<T, 1, 6, GROUPED> : p.M <= 16 ? int8_rows_kernel<T, 2, 4, GROUPED> : int8_rows_kernel<T, 4, 2, GROUPED>;
+  return launch_behind(kern, grid, dim3(kInt8RowsThreads), 0, st, d, p);
+}
+
+// Few rows go by int8_rows_kernel.
+inline bool int8_few_rows(int64_t M, int64_t B, bool grouped) { return B <= 65535 && M <= (grouped ? 32 : 16); }
+
+template <typename T>
+inline int launch_int8_mm(const Int8Operand& X, const Int8Operand& W, const Int8Params<T>& p, cudaStream_t st) {
+  const bool grouped = p.offsets != nullptr;
+  if (int8_few_rows(p.M, p.B, grouped)) {
+    const Int8Rows d{reinterpret_cast<const uint8_t*>(X.q), reinterpret_cast<const uint8_t*>(W.q), X.ld, X.batch, W.ld, W.batch};
+    return grouped ? launch_int8_rows<T, true>(d, p, st) : launch_int8_rows<T, false>(d, p, st);
+  }
+  return grouped ? launch_int8_pair<T, true>(X, W, p, st) : launch_int8_pair<T, false>(X, W, p, st);
+}
+
+}  // namespace yb

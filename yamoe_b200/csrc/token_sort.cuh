@@ -1,0 +1,612 @@
+// Tokens sorted by expert and back, as operators of their own.
+//
+//   sort      row_of[t, k] = first row of expert e + number of assignments p' < p = t K + k of the same expert e
+//             rows[row_of[t, k]] = hidden[t]; rows without an assignment are zero
+//   combine   out[t] = sum over k of w[t, k] rows[row_of[t, k]]
+//   its gradients   d_rows[r] = sum over p with row_of[p] = r of w[p] d_out[t(p)],   d_w[t, k] = <d_out[t], rows[row_of[t, k]]>
+//
+// Without a capacity an expert's rows follow those of the expert before it; with one, expert e has rows e C .. e C + C - 1 and
+// assignments behind its first C are dropped (row_of = -1), as are ids outside [0, E).
+//
+// Bound by HBM for a prompt and by latency for a batch of single tokens.  A token's row is read once and written K times (a warp per
+// 512-byte piece of a token, the pieces of a token side by side in the grid).  Up to kSortSmallMax assignments every CTA ranks all of them
+// for itself and goes on to copy: one launch.  Above, blocks count, rank and copy in three launches; a block takes what lies before it from the
+// table of all blocks' counts, so that no CTA waits for another and nothing has to be zeroed.
+#pragma once
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace yb {
+
+constexpr int kSortMaxExperts = 1024;
+constexpr int kSortSmallThreads = 1024, kSortSmallWarps = 32, kSortSmallRounds = 4;
+constexpr int kSortSmallMax = kSortSmallThreads * kSortSmallRounds;
+constexpr int kSortThreads = 256, kSortWarps = 8, kSortRounds = 8;
+constexpr int kSortPart = kSortThreads * kSortRounds;         // assignments that a block ranks at a time
+constexpr int kSortMaxBlocks = 256;
+
+struct SortArgs {
+  const int64_t* indices;       // [S]
+  const uint8_t* hidden;        // [T, row_bytes]
+  uint8_t* rows;                // [R, row_bytes]
+  int32_t* row_of;              // [S]
+  int32_t* offsets;             // [E + 1] rows kept before each expert's
+  int64_t T, R, row_bytes;
+  int S, E, K;
+  int capacity;                 // -1: none
+  int32_t* counts;              // [blocks, E] (large sorts)
+  int parts;                    // of kSortPart assignments that a block takes
+};
+
+__device__ __forceinline__ int sort_kept(int total, int capacity) { return capacity < 0 ? total : min(total, capacity); }
+
+// Inclusive scan of one number per thread over a CTA of whole warps; `part` has a place for each warp.
+template <int WARPS>
+__device__ __forceinline__ int block_scan(int v, int* part) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  if (lane == 31) part[w] = v;
+  __syncthreads();
+  int before = 0;
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) before += i < w ? part[i] : 0;
+  __syncthreads();
+  return v + before;
+}
+
+// Number of items of the same key in lower lanes, and `base[key]` raised by all of this warp's: the place of each.
+__device__ __forceinline__ int take_places(int key, int32_t* base, int lane) {
+  const unsigned mask = __match_any_sync(0xffffffffu, key);
+  int place = 0;
+  if (key >= 0) place = base[key] + __popc(mask & ((1u << lane) - 1u));
+  __syncwarp();
+  if (key >= 0 && (__ffs(mask) - 1) == lane) base[key] += __popc(mask);
+  __syncwarp();
+  return place;
+}
+
+__device__ __forceinline__ int load_expert(const int64_t* indices, int j, int end, int E, int lane) {
+  if (j < end) {
+    const int64_t v = indices[j];
+    if (v >= 0 && v < E) return (int)v;
+  }
+  return -1 - lane;            // a key that no other lane has
+}
+
+// One 32-lane piece of a token's row to the rows of its K assignments.
+template <typename P>
+__device__ __forceinline__ void copy_piece(const SortArgs& a, int64_t t, int i, int n, const int32_t* row_of) {
+  if (i >= n) return;
+  const P v = reinterpret_cast<const P*>(a.hidden + t * a.row_bytes)[i];
+  for (int k = 0; k < a.K; ++k) {
+    const int r = row_of[k];
+    if (r >= 0) reinterpret_cast<P*>(a.rows + r * a.row_bytes)[i] = v;
+  }
+}
+template <typename P>
+__device__ __forceinline__ void zero_row(const SortArgs& a, int64_t r, int n, int lane) {
+  P* d = reinterpret_cast<P*>(a.rows + r * a.row_bytes);
+  for (int i = lane; i < n; i += 32) d[i] = P{};
+}
+// Rows without an assignment, 32 to a warp: lanes look, the warp writes.
+template <typename P>
+__device__ __forceinline__ void zero_unused(const SortArgs& a, int64_t first, int n, int lane, const int32_t* offsets) {
+  const int64_t r = first + lane;
+  bool unused = false;
+  if (r < a.R) {
+    if (a.capacity < 0) {
+      unused = r >= offsets[a.E];
+    } else {
+      const int e = (int)(r / a.capacity);
+      unused = r - (int64_t)e * a.capacity >= offsets[e + 1] - offsets[e];
+    }
+  }
+  for (unsigned todo = __ballot_sync(0xffffffffu, unused); todo != 0; todo &= todo - 1) zero_row<P>(a, first + (__ffs(todo) - 1), n, lane);
+}
+
+// ---- small: everything in one launch ------------------------------------------------------------------------------------
+inline size_t sort_small_smem(int S, int E) {
+  return ((size_t)kSortSmallWarps * E + E + 1 + S) * sizeof(int32_t);
+}
+
+template <typename P>
+__global__ void __launch_bounds__(kSortSmallThreads)
+sort_small_kernel(SortArgs a, int rounds) {
+  extern __shared__ int32_t smem_i[];
+  int32_t* base = smem_i;                              // [warps][E] counts, then first row of a warp's assignments of an expert
+  int32_t* offsets = smem_i + kSortSmallWarps * a.E;   // [E + 1]
+  int32_t* row_of = offsets + a.E + 1;                 // [S]
+  __shared__ int s_part[kSortSmallWarps];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  for (int i = tid; i < kSortSmallWarps * a.E; i += kSortSmallThreads) base[i] = 0;
+  pdl_trigger();
+  pdl_wait();
+  const int64_t* indices = after_wait(a.indices);
+  a.hidden = after_wait(a.hidden);
+  const int first = w * 32 * rounds;
+  int ex[kSortSmallRounds];
+#pragma unroll
+  for (int i = 0; i < kSortSmallRounds; ++i) ex[i] = i < rounds ? load_expert(indices, first + i * 32 + lane, a.S, a.E, lane) : -1 - lane;
+  __syncthreads();
+  int32_t* mine = base + w * a.E;
+#pragma unroll
+  for (int i = 0; i < kSortSmallRounds; ++i)
+    if (i < rounds) take_places(ex[i], mine, lane);
+  __syncthreads();
+  int total = 0;
+  if (tid < a.E) {
+#pragma unroll 8
+    for (int v = 0; v < kSortSmallWarps; ++v) {
+      const int c = base[v * a.E + tid];
+      base[v * a.E + tid] = total;
+      total += c;
+    }
+  }
+  const int kept = sort_kept(total, a.capacity);
+  const int end = block_scan<kSortSmallWarps>(kept, s_part);
+  if (tid == 0) offsets[0] = 0;
+  if (tid < a.E) offsets[tid + 1] = end;
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int e = tid; e <= a.E; e += kSortSmallThreads) a.offsets[e] = offsets[e];
+#pragma unroll
+  for (int i = 0; i < kSortSmallRounds; ++i)
+    if (i < rounds) {
+      const int e = ex[i], j = first + i * 32 + lane;
+      const int place = take_places(e, mine, lane);
+      int r = -1;
+      if (e >= 0 && (a.capacity < 0 || place < a.capacity)) r = (a.capacity < 0 ? offsets[e] : e * a.capacity) + place;
+      if (j < a.S) {
+        row_of[j] = r;
+        if (blockIdx.x == 0) a.row_of[j] = r;
+      }
+    }
+  __syncthreads();
+  const int n = (int)(a.row_bytes / sizeof(P)), chunks = (n + 31) / 32;
+  const int64_t warps = (int64_t)gridDim.x * kSortSmallWarps, at = (int64_t)blockIdx.x * kSortSmallWarps + w;
+  for (int64_t u = at; u < a.T * chunks; u += warps) {
+    const int64_t t = u / chunks;
+    copy_piece<P>(a, t, (int)(u - t * chunks) * 32 + lane, n, row_of + t * a.K);
+  }
+  for (int64_t r = at * 32; r < a.R; r += warps * 32) zero_unused<P>(a, r, n, lane, offsets);
+}
+
+// ---- large: count, rank, copy -------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(kSortThreads)
+sort_count_kernel(SortArgs a) {
+  extern __shared__ int32_t smem_i[];                  // [E]
+  for (int e = threadIdx.x; e < a.E; e += kSortThreads) smem_i[e] = 0;
+  pdl_trigger();
+  pdl_wait();
+  const int64_t* indices = after_wait(a.indices);
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * a.parts * kSortPart;
+  const int64_t end = min((int64_t)a.S, first + (int64_t)a.parts * kSortPart);
+  for (int64_t j = first + threadIdx.x; j < end; j += kSortThreads) {
+    const int64_t v = indices[j];
+    if (v >= 0 && v < a.E) atomicAdd(&smem_i[v], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += kSortThreads) a.counts[(size_t)blockIdx.x * a.E + e] = smem_i[e];
+}
+
+inline size_t sort_rank_smem(int E) { return ((size_t)kSortWarps * E + 3 * E + 1) * sizeof(int32_t); }
+
+__global__ void __launch_bounds__(kSortThreads)
+sort_rank_kernel(SortArgs a) {
+  extern __shared__ int32_t smem_i[];
+  int32_t* base = smem_i;                        // [warps][E]
+  int32_t* next = smem_i + kSortWarps * a.E;     // [E] place of this block's next assignment of an expert
+  int32_t* kept = next + a.E;                    // [E]
+  int32_t* offsets = kept + a.E;                 // [E + 1]
+  __shared__ int s_part[kSortWarps];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  pdl_trigger();
+  pdl_wait();
+  const int64_t* indices = after_wait(a.indices);
+  const int32_t* counts = after_wait(a.counts);
+  for (int e = tid; e < a.E; e += kSortThreads) {
+    int lower = 0, total = 0;
+#pragma unroll 8
+    for (int b = 0; b < (int)gridDim.x; ++b) {
+      const int c = counts[(size_t)b * a.E + e];
+      total += c;
+      lower += b < (int)blockIdx.x ? c : 0;
+    }
+    next[e] = lower;
+    kept[e] = sort_kept(total, a.capacity);
+  }
+  __syncthreads();
+  // four neighbouring experts to a thread
+  int v[kSortMaxExperts / kSortThreads], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kSortMaxExperts / kSortThreads; ++i) {
+    const int e = tid * (kSortMaxExperts / kSortThreads) + i;
+    v[i] = e < a.E ? kept[e] : 0;
+    sum += v[i];
+  }
+  int end = block_scan<kSortWarps>(sum, s_part) - sum;
+  if (tid == 0) offsets[0] = 0;
+#pragma unroll
+  for (int i = 0; i < kSortMaxExperts / kSortThreads; ++i) {
+    const int e = tid * (kSortMaxExperts / kSortThreads) + i;
+    end += v[i];
+    if (e < a.E) offsets[e + 1] = end;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int e = tid; e <= a.E; e += kSortThreads) a.offsets[e] = offsets[e];
+  for (int part = 0; part < a.parts; ++part) {
+    const int64_t part0 = ((int64_t)blockIdx.x * a.parts + part) * kSortPart;
+    if (part0 >= a.S) break;
+    const int first = (int)part0 + w * 32 * kSortRounds;
+    for (int i = tid; i < kSortWarps * a.E; i += kSortThreads) base[i] = 0;
+    int ex[kSortRounds];
+#pragma unroll
+    for (int i = 0; i < kSortRounds; ++i) ex[i] = load_expert(indices, first + i * 32 + lane, a.S, a.E, lane);
+    __syncthreads();
+    int32_t* mine = base + w * a.E;
+#pragma unroll
+    for (int i = 0; i < kSortRounds; ++i) take_places(ex[i], mine, lane);
+    __syncthreads();
+    for (int e = tid; e < a.E; e += kSortThreads) {
+      int run = next[e];
+#pragma unroll
+      for (int u = 0; u < kSortWarps; ++u) {
+        const int c = base[u * a.E + e];
+        base[u * a.E + e] = run;
+        run += c;
+      }
+      next[e] = run;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSortRounds; ++i) {
+      const int e = ex[i], j = first + i * 32 + lane;
+      const int place = take_places(e, mine, lane);
+      int r = -1;
+      if (e >= 0 && (a.capacity < 0 || place < a.capacity)) r = (a.capacity < 0 ? offsets[e] : e * a.capacity) + place;
+      if (j < a.S) a.row_of[j] = r;
+    }
+    __syncthreads();
+  }
+}
+
+constexpr int kCopyWarps = 8;
+
+// CTAs below `copy_ctas` copy, the others zero rows without an assignment.
+template <typename P>
+__global__ void __launch_bounds__(kCopyWarps * 32)
+sort_copy_kernel(SortArgs a, unsigned copy_ctas) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int n = (int)(a.row_bytes / sizeof(P)), chunks = (n + 31) / 32;
+  pdl_trigger();
+  pdl_wait();
+  a.hidden = after_wait(a.hidden);
+  const int32_t* row_of = after_wait(a.row_of);
+  if (blockIdx.x < copy_ctas) {
+    const int64_t u = (int64_t)blockIdx.x * kCopyWarps + w, t = u / chunks;
+    if (t < a.T) copy_piece<P>(a, t, (int)(u - t * chunks) * 32 + lane, n, row_of + t * a.K);
+  } else {
+    const int64_t first = ((int64_t)(blockIdx.x - copy_ctas) * kCopyWarps + w) * 32;
+    if (first < a.R) zero_unused<P>(a, first, n, lane, after_wait(a.offsets));
+  }
+}
+
+// Blocks of a large sort and the parts that each takes.
+struct SortBlocks { int blocks, parts; };
+inline SortBlocks sort_blocks(int64_t S) {
+  const int64_t all = ceil_div(S, kSortPart), parts = std::max<int64_t>(1, ceil_div(all, kSortMaxBlocks));
+  return SortBlocks{(int)ceil_div(all, parts), (int)parts};
+}
+inline size_t sort_counts_bytes(int64_t S, int E) {
+  return S <= kSortSmallMax ? 0 : (size_t)sort_blocks(S).blocks * E * sizeof(int32_t);
+}
+
+template <typename Kern>
+inline int allow_smem(Kern kern, size_t smem, PerDevice<size_t>& configured) {
+  const int dev = current_device_index();
+  if (smem > 48 * 1024 && smem > configured.get(dev)) {
+    YB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    configured.set(dev, smem);
+  }
+  return YAMOE_OK;
+}
+
+template <typename P>
+inline int launch_sort(SortArgs a, cudaStream_t st) {
+  const int64_t n = a.row_bytes / (int64_t)sizeof(P), chunks = ceil_div(n, 32);
+  if (a.S <= kSortSmallMax) {
+    static PerDevice<size_t> configured;
+    const size_t smem = sort_small_smem(a.S, a.E);
+    if (const int rc = allow_smem(sort_small_kernel<P>, smem, configured)) return rc;
+    const int rounds = std::max(1, (int)ceil_div(a.S, kSortSmallThreads));
+    const int64_t work = std::max(ceil_div(a.T * chunks, kSortSmallWarps), ceil_div(a.R, kSortSmallWarps * 32));
+    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(work, kSMs));
+    return launch_behind(sort_small_kernel<P>, dim3((unsigned)grid), dim3(kSortSmallThreads), smem, st, a, rounds);
+  }
+  const SortBlocks b = sort_blocks(a.S);
+  a.parts = b.parts;
+  int rc = launch_behind(sort_count_kernel, dim3(b.blocks), dim3(kSortThreads), a.E * sizeof(int32_t), st, a);
+  if (rc) return rc;
+  static PerDevice<size_t> configured;
+  if ((rc = allow_smem(sort_rank_kernel, sort_rank_smem(a.E), configured))) return rc;
+  if ((rc = launch_behind(sort_rank_kernel, dim3(b.blocks), dim3(kSortThreads), sort_rank_smem(a.E), st, a))) return rc;
+  const int64_t copy = ceil_div(a.T * chunks, kCopyWarps), zero = ceil_div(a.R, kCopyWarps * 32);
+  if (copy + zero > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
+  if (copy + zero == 0) return YAMOE_OK;
+  return launch_behind(sort_copy_kernel<P>, dim3((unsigned)(copy + zero)), dim3(kCopyWarps * 32), 0, st, a, (unsigned)copy);
+}
+
+// ---- combine --------------------------------------------------------------------------------------------------------------
+template <typename T, typename TW>
+struct CombineArgs {
+  const T* rows;                // [n_rows, H]
+  const int32_t* row_of;        // [T, K]; outside [0, n_rows): nothing
+  const TW* weights;            // [T, K], or [T, E] with indices; null: 1
+  const int64_t* indices;       // [T, K] columns of the weights; null: the slots
+  int64_t Tn, n_rows, H;
+  int K, E;
+  __device__ __forceinline__ void behind_wait() {
+    rows = after_wait(rows);
+    row_of = after_wait(row_of);
+    weights = after_wait(weights);
+    indices = after_wait(indices);
+  }
+  // row of assignment p, -1 for none
+  __device__ __forceinline__ int row(int64_t p) const {
+    const int r = row_of[p];
+    return r >= 0 && r < n_rows ? r : -1;
+  }
+  __device__ __forceinline__ int64_t column(int64_t t, int k) const {
+    return indices == nullptr ? k : indices[t * K + k];
+  }
+  // weight of slot k of token t; 0 for a column that does not exist
+  __device__ __forceinline__ float weight(int64_t t, int k) const {
+    if (weights == nullptr) return 1.f;
+    if (indices == nullptr) return DT<TW>::ld(weights + t * K + k);
+    const int64_t c = indices[t * K + k];
+    return c >= 0 && c < E ? DT<TW>::ld(weights + t * E + c) : 0.f;
+  }
+};
+
+// VE neighbouring values: a 16-byte piece, or one value.
+template <typename T, int VE> struct Piece {
+  uint4 q;
+  __device__ __forceinline__ void load(const T* p) { q = ld_written(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void get(float (&v)[VE]) const {
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        v[j] = __uint_as_float(u[j]);
+      } else {
+        v[2 * j] = __uint_as_float(u[j] << 16);
+        v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+      }
+    }
+  }
+  static __device__ __forceinline__ void put(T* p, const float (&v)[VE]) {
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        u[j] = __float_as_uint(v[j]);
+      } else {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        u[j] = *reinterpret_cast<const uint32_t*>(&two);
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+template <typename T> struct Piece<T, 1> {
+  T q;
+  __device__ __forceinline__ void load(const T* p) { q = *p; }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = DT<T>::ld(&q); }
+  static __device__ __forceinline__ void put(T* p, const float (&v)[1]) { DT<T>::st(p, v[0]); }
+};
+
+// One warp per 32 pieces of a token; the rows of KB slots are on their way together.  Sums in fp32 in the order of the slots.
+template <typename T, typename TW, int VE, int KB>
+__global__ void __launch_bounds__(kCopyWarps * 32)
+combine_tokens_kernel(CombineArgs<T, TW> a, T* out) {
+  pdl_trigger();
+  pdl_wait();
+  a.behind_wait();
+  const int64_t pieces = a.H / VE, chunks = (pieces + 31) / 32;
+  const int64_t u = (int64_t)blockIdx.x * kCopyWarps + (threadIdx.x >> 5), t = u / chunks;
+  const int64_t i = (u - t * chunks) * 32 + (threadIdx.x & 31);
+  if (t >= a.Tn || i >= pieces) return;
+  float acc[VE];
+#pragma unroll
+  for (int j = 0; j < VE; ++j) acc[j] = 0.f;
+  for (int k0 = 0; k0 < a.K; k0 += KB) {
+    int r[KB];
+    float w[KB];
+    Piece<T, VE> q[KB];
+#pragma unroll
+    for (int k = 0; k < KB; ++k) r[k] = k0 + k < a.K ? a.row(t * a.K + k0 + k) : -1;
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+      if (r[k] >= 0) q[k].load(a.rows + r[k] * a.H + i * VE);
+#pragma unroll
+    for (int k = 0; k < KB; ++k) w[k] = r[k] >= 0 ? a.weight(t, k0 + k) : 0.f;
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+      if (r[k] >= 0) {
+        float v[VE];
+        q[k].get(v);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) acc[j] = fmaf(w[k], v[j], acc[j]);
+      }
+  }
+  Piece<T, VE>::put(out + t * a.H + i * VE, acc);
+}
+
+// ---- gradients of the combine -----------------------------------------------------------------------------------------------
+// Whose row a row is: head[r] is one of its assignments (-1: none), next[p] the one behind p (-1: none).  The rows of sort_tokens
+// have one assignment or none, but row_of may name a row as often as it likes.
+__global__ void __launch_bounds__(256)
+link_rows_kernel(const int32_t* row_of, int64_t S, int64_t n_rows, int32_t* head, int32_t* next) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (p >= S) return;
+  const int r = after_wait(row_of)[p];
+  if (r >= 0 && r < n_rows) next[p] = atomicExch(head + r, (int32_t)p);
+}
+
+// From the tokens' side, so that d_out is read once: `wpt` warps (1, 2, 4 or 8) share a token, write the rows that only it has and add up
+// the products with all its rows, each warp its pieces, the warps in order.  The CTAs behind `token_ctas` look for the other rows: those
+// of no assignment become zero, those of several the sum over them (in the order of their list, which is not fixed beyond two).
+template <typename T, typename TW, int VE, int KB>
+__global__ void __launch_bounds__(kCopyWarps * 32)
+combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_weights, const int32_t* head, const int32_t* next,
+                        int wpt, unsigned token_ctas) {
+  extern __shared__ float s_dot[];              // [warps][K]
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t pieces = a.H / VE;
+  pdl_trigger();
+  pdl_wait();
+  a.behind_wait();
+  d_out = after_wait(d_out);
+  head = after_wait(head);
+  next = after_wait(next);
+  if (blockIdx.x >= token_ctas) {
+    const int64_t first = ((int64_t)(blockIdx.x - token_ctas) * kCopyWarps + w) * 32;
+    int h = -1;
+    bool mine = false;
+    if (first + lane < a.n_rows) {
+      h = head[first + lane];
+      mine = h < 0 || next[h] >= 0;
+    }
+    for (unsigned todo = __ballot_sync(0xffffffffu, mine); todo != 0; todo &= todo - 1) {
+      const int l = __ffs(todo) - 1, p0 = __shfl_sync(0xffffffffu, h, l);
+      for (int64_t i = lane; i < pieces; i += 32) {
+        float acc[VE];
+#pragma unroll
+        for (int j = 0; j < VE; ++j) acc[j] = 0.f;
+        for (int p = p0; p >= 0; p = next[p]) {
+          const int64_t t = p / a.K;
+          const float wgt = a.weight(t, (int)(p - t * a.K));
+          Piece<T, VE> q;
+          q.load(d_out + t * a.H + i * VE);
+          float v[VE];
+          q.get(v);
+#pragma unroll
+          for (int j = 0; j < VE; ++j) acc[j] = fmaf(wgt, v[j], acc[j]);
+        }
+        Piece<T, VE>::put(d_rows + (first + l) * a.H + i * VE, acc);
+      }
+    }
+    return;
+  }
+  const int64_t t = (int64_t)blockIdx.x * (kCopyWarps / wpt) + w / wpt;
+  const int part = w % wpt;
+  for (int k0 = 0; k0 < a.K && t < a.Tn; k0 += KB) {
+    int r[KB];
+    float wgt[KB], dot[KB];
+    bool own[KB];
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+      r[k] = k0 + k < a.K ? a.row(t * a.K + k0 + k) : -1;
+      wgt[k] = r[k] >= 0 ? a.weight(t, k0 + k) : 0.f;
+      dot[k] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+      own[k] = d_rows != nullptr && r[k] >= 0 && head[r[k]] == (int)(t * a.K + k0 + k) && next[t * a.K + k0 + k] < 0;
+    for (int64_t i = lane + 32 * part; i < pieces; i += 32 * wpt) {
+      Piece<T, VE> g, q[KB];
+      g.load(d_out + t * a.H + i * VE);
+      if (d_weights != nullptr) {
+#pragma unroll
+        for (int k = 0; k < KB; ++k)
+          if (r[k] >= 0) q[k].load(a.rows + r[k] * a.H + i * VE);
+      }
+      float d[VE];
+      g.get(d);
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        if (r[k] < 0) continue;
+        float v[VE];
+        if (d_weights != nullptr) {
+          q[k].get(v);
+#pragma unroll
+          for (int j = 0; j < VE; ++j) dot[k] = fmaf(d[j], v[j], dot[k]);
+        }
+#pragma unroll
+        for (int j = 0; j < VE; ++j) v[j] = wgt[k] * d[j];
+        if (own[k]) Piece<T, VE>::put(d_rows + r[k] * a.H + i * VE, v);
+      }
+    }
+    if (d_weights != nullptr) {
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot[k] += __shfl_xor_sync(0xffffffffu, dot[k], o);
+        if (lane == 0 && k0 + k < a.K) s_dot[w * a.K + k0 + k] = dot[k];
+      }
+    }
+  }
+  if (d_weights == nullptr) return;
+  __syncthreads();
+  if (part != 0 || t >= a.Tn) return;
+  // of each slot the sum over the token's warps, by its first one
+  for (int k = lane; k < a.K; k += 32) {
+    float sum = 0.f;
+    for (int o = 0; o < wpt; ++o) sum += s_dot[(w + o) * a.K + k];
+    s_dot[w * a.K + k] = sum;
+    if (a.indices == nullptr) DT<TW>::st(d_weights + t * a.K + k, sum);
+  }
+  if (a.indices == nullptr) return;
+  __syncwarp();
+  for (int c = lane; c < a.E; c += 32) {        // every column of the dense weights, also where two slots have the same
+    float sum = 0.f;
+    for (int k = 0; k < a.K; ++k)
+      if (a.indices[t * a.K + k] == c) sum += s_dot[w * a.K + k];
+    DT<TW>::st(d_weights + t * a.E + c, sum);
+  }
+}
+
+template <typename T, typename TW, int VE>
+inline int launch_combine_tokens_ve(const CombineArgs<T, TW>& a, T* out, cudaStream_t st) {
+  const int64_t ctas = ceil_div(a.Tn * ceil_div(a.H / VE, 32), kCopyWarps);
+  if (ctas > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
+  auto kern = a.K <= 4 ? combine_tokens_kernel<T, TW, VE, 4> : combine_tokens_kernel<T, TW, VE, 8>;
+  return launch_behind(kern, dim3((unsigned)ctas), dim3(kCopyWarps * 32), 0, st, a, out);
+}
+
+template <typename T, typename TW, int VE>
+inline int launch_combine_backward_ve(const CombineArgs<T, TW>& a, const T* d_out, T* d_rows, TW* d_weights, int32_t* head, int32_t* next,
+                                      cudaStream_t st) {
+  // at least 32 warps per SM, while each has pieces of the token
+  int wpt = 1;
+  while (wpt < kCopyWarps && a.Tn * wpt < kSMs * 32 && a.H / VE > 32 * wpt) wpt *= 2;
+  const int64_t S = a.Tn * a.K, token = ceil_div(a.Tn * wpt, kCopyWarps), row = d_rows != nullptr ? ceil_div(a.n_rows, kCopyWarps * 32) : 0;
+  if (token + row > 0x7fffffff || ceil_div(S, 256) > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
+  if (d_rows != nullptr && a.n_rows > 0) {
+    YB_CUDA_OK(cudaMemsetAsync(head, 0xFF, (size_t)a.n_rows * sizeof(int32_t), st));
+    const int rc = S == 0 ? YAMOE_OK
+                          : launch_behind(link_rows_kernel, dim3((unsigned)ceil_div(S, 256)), dim3(256), 0, st, a.row_of, S, a.n_rows, head, next);
+    if (rc) return rc;
+  }
+  if (token + row == 0) return YAMOE_OK;
+  auto kern = a.K <= 4 ? combine_backward_kernel<T, TW, VE, 4> : combine_backward_kernel<T, TW, VE, 8>;
+  return launch_behind(kern, dim3((unsigned)(token + row)), dim3(kCopyWarps * 32), kCopyWarps * a.K * sizeof(float), st, a, d_out, d_rows,
+                       d_weights, (const int32_t*)head, (const int32_t*)next, wpt, (unsigned)token);
+}
+
+inline bool pieces_of_16_bytes(int64_t row_bytes, std::initializer_list<const void*> at) {
+  uintptr_t bits = (uintptr_t)row_bytes;
+  for (const void* p : at) bits |= reinterpret_cast<uintptr_t>(p);
+  return (bits & 15) == 0;
+}
+
+}  // namespace yb

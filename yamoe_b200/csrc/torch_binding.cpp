@@ -5,22 +5,16 @@
 // current stream.  Takes the place of torch-ext/torch_binding.cpp + csrc/moe.cpp:45-136 of the
 // reference; the preconditions and their messages follow csrc/moe.cpp:58-96.
 //
+// The steps of the expert layer are in torch_steps.cpp.
+//
 // Built separately from the CUDA library (host compiler only) and loaded with
 // torch.ops.load_library; when it is absent the same operators are registered from Python
 // (yamoe_b200/ops.py), which costs some tens of microseconds more per call.
-#include <ATen/ATen.h>
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/library.h>
-
-#include <cstdlib>
 #include <optional>
 #include <tuple>
 #include <vector>
 
-#include "../../include/yamoe_b200.h"
+#include "torch_common.h"
 
 namespace {
 
@@ -62,28 +56,6 @@ Shape validate(const at::Tensor& hidden_states, const at::Tensor& router_indices
   TORCH_CHECK(router_indices.scalar_type() == at::kLong || router_indices.scalar_type() == at::kInt,
               "router_indices must be int64");
   return Shape{T, (int)H, (int)E, (int)K, dt == at::kBFloat16 ? YAMOE_BF16 : YAMOE_F32};
-}
-
-void check(int status, const char* what) {
-  TORCH_CHECK(status == YAMOE_OK, "yamoe_b200: ", what, " failed: ", yamoe_b200_status_string(status), " (status ",
-              status, ")");
-}
-
-// YAMOE_B200_CHECK_STATUS=1: read the device status word after the call (one stream synchronisation)
-void check_device_status(const at::Tensor& ws, cudaStream_t st, const char* what) {
-  static const bool on = []() {
-    const char* env = std::getenv("YAMOE_B200_CHECK_STATUS");
-    return env != nullptr && env[0] != '\0' && !(env[0] == '0' && env[1] == '\0');
-  }();
-  if (!on) return;
-  int32_t status = 0;
-  check(yamoe_b200_device_status(ws.data_ptr(), st, &status), what);
-  TORCH_CHECK(status == 0, "yamoe_b200: ", what, " failed: ", yamoe_b200_status_string(YAMOE_ERR_DEVICE_TIMEOUT),
-              " (device status ", status, ")");
-}
-
-at::Tensor workspace(size_t nbytes, const at::Tensor& like) {
-  return at::empty({(int64_t)(nbytes > 256 ? nbytes : 256)}, like.options().dtype(at::kByte));
 }
 
 at::Tensor experts_cuda(const at::Tensor& hidden_states, const at::Tensor& router_indices,
@@ -146,10 +118,6 @@ std::vector<at::Tensor> experts_backward_cuda(const at::Tensor& grad_out, const 
 // ---- 8-bit operands --------------------------------------------------------------------------------------------------
 
 constexpr int64_t kGroup = 128;
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-int dtype_of(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? YAMOE_BF16 : YAMOE_F32; }
-cudaStream_t current_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
-
 // A quantised operand: codes [B, rows, cols] or [rows, cols] with scales [.., rows or row blocks, groups].
 struct Quantised {
   at::Tensor q, scale;
@@ -308,16 +276,6 @@ at::Tensor fp8_linear_cuda(const at::Tensor& x, const at::Tensor& weight) {
   return mm(xq, wq, x.scalar_type()).view(linear_shape(x, weight));
 }
 
-// Backward computes on codes, below the autograd layer: what it returns has no derivative.  Where a graph of it is asked for
-// (create_graph), it leads through a node that raises when it is differentiated, on to all that it depends on.
-void differentiate_no_further(const at::Tensor& dy, at::Tensor& dx, at::Tensor& dw) {
-  torch::autograd::edge_list on = torch::autograd::get_current_node()->next_edges();
-  for (const torch::autograd::Edge& e : torch::autograd::collect_next_edges(dy)) on.push_back(e);
-  const auto node = std::make_shared<torch::autograd::Error>("fp8_linear can be differentiated once only", std::move(on));
-  for (at::Tensor* t : {&dx, &dw})
-    if (t->defined()) torch::autograd::create_gradient_edge(*t, node);
-}
-
 // y = Q(x) Q(w)^T with dx = Q(dy) Q(w) and dw = Q(dy^T) Q(x^T)^T; what backward needs of x and w is kept as codes.
 struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight) {
@@ -352,30 +310,17 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
       if (want_x) dx = mm(g, wt, d.scalar_type()).view(ctx->saved_data["x_shape"].toIntVector());
       if (want_w) dw = mm(gt, xt, d.scalar_type());
     }
-    if (at::GradMode::is_enabled()) differentiate_no_further(dy, dx, dw);
+    if (at::GradMode::is_enabled()) differentiate_no_further("fp8_linear", {dy}, {&dx, &dw});
     return {dx, dw};
   }
 };
 
-// Forward mode: a tangent that nobody takes up would count as zero.
-void check_no_tangent(const at::Tensor& t) {
-  TORCH_CHECK(!t._fw_grad(0).defined(), "fp8_linear: forward-mode differentiation is not supported");
-}
-
 at::Tensor fp8_linear_autograd(const at::Tensor& x, const at::Tensor& weight) {
-  if (c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
-    check_no_tangent(x);
-    check_no_tangent(weight);
-  }
+  check_no_tangent("fp8_linear", x);
+  check_no_tangent("fp8_linear", weight);
   if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad())) return Fp8Linear::apply(x, weight);
   at::AutoDispatchBelowAutograd below;
   return fp8_linear_cuda(x, weight);
-}
-
-// contiguous, on the 16-byte boundary that the kernels' wide loads and copies want
-at::Tensor aligned(const at::Tensor& t) {
-  const at::Tensor c = t.contiguous();
-  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
 at::Tensor experts_fp8_cuda(const at::Tensor& hidden_states, const at::Tensor& router_indices, const at::Tensor& routing_weights,

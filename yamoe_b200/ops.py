@@ -464,6 +464,11 @@ fp8_mm = _cpp_operator("fp8_mm")
 fp8_linear = _cpp_operator("fp8_linear")
 experts_fp8 = _cpp_operator("experts_fp8")
 moe_layer = _cpp_operator("moe_layer")
+sort_tokens = _cpp_operator("sort_tokens")
+combine_tokens = _cpp_operator("combine_tokens")
+quantize_int8 = _cpp_operator("quantize_int8")
+int8_mm = _cpp_operator("int8_mm")
+glu_fp8 = _cpp_operator("glu_fp8")
 
 
 def quantize_experts(gate_up_proj, down_proj):
