@@ -6,9 +6,11 @@
 // codes 0 and the scale NaN, so that whatever is computed from it is NaN.
 //
 // Bound by HBM: a value is read once and its code written once, 3 bytes for bf16.  Rows: 1 to 8 warps hold one in registers; a longer one is read
-// twice.  Transposed (the codes of x^T, a scale per column of x): a CTA has a strip of 64 columns, reads it for the largest
-// magnitudes and once more, from L2, for the codes, which it turns around in shared memory.
+// twice.  Transposed (the codes of x^T, a scale per column of x): a cluster has a strip of 64 columns, reads it for the largest
+// magnitudes and, but for its last rows, once more for the codes, which it turns around in shared memory.
 #pragma once
+#include <algorithm>
+
 #include "fp8_quant.cuh"
 
 namespace yb {
@@ -35,31 +37,31 @@ struct Int8Out {
 constexpr int kInt8Pieces = 4;         // of 8 values that a lane holds
 constexpr int kInt8RowWarps = 8;
 
-// `wpr` warps (1, 2, 4, 8) per row of x [batch, M, K]
+// 2^log_wpr warps (1, 2, 4, 8) per row of x [batch, M, K]
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kInt8RowWarps * 32)
-int8_rows_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, int wpr) {
+int8_rows_quantize_kernel(const T* x, const Int8Out d, int64_t M, int K, int log_wpr) {
   __shared__ uint32_t s_most[kInt8RowWarps];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, sub = w % wpr;
-  const int64_t row = (int64_t)blockIdx.x * (kInt8RowWarps / wpr) + w / wpr;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, wpr = 1 << log_wpr, sub = w & (wpr - 1);
+  const int64_t row = (int64_t)blockIdx.x * (kInt8RowWarps >> log_wpr) + (w >> log_wpr);
   const bool there = row < M;
   pdl_trigger();
   pdl_wait();
   const T* src = after_wait(x) + ((int64_t)blockIdx.y * M + (there ? row : 0)) * K;
-  const int64_t step = (int64_t)wpr * 256, first = (sub * 32 + lane) * 8;
-  const int64_t end = there ? K : 0;
+  // (unsigned, as the step behind the last value may pass 31 bits)
+  const unsigned step = wpr * 256, first = (sub * 32 + lane) * 8, end = there ? K : 0;
   Eight<T> v[kInt8Pieces];
   uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < kInt8Pieces; ++i) {
-    const int64_t k = first + i * step;
-    v[i].template load<VEC>(src + k, (int)max((int64_t)0, min((int64_t)8, end - k)));
+    const unsigned k = first + i * step;
+    v[i].template load<VEC>(src + k, k < end ? (int)min(8u, end - k) : 0);
   }
 #pragma unroll
   for (int i = 0; i < kInt8Pieces; ++i) most = max(most, v[i].most());
-  for (int64_t k = first + kInt8Pieces * step; k < end; k += step) {
+  for (unsigned k = first + kInt8Pieces * step; k < end; k += step) {
     Eight<T> more;
-    more.template load<VEC>(src + k, (int)min((int64_t)8, end - k));
+    more.template load<VEC>(src + k, (int)min(8u, end - k));
     most = max(most, more.most());
   }
   most = __reduce_max_sync(0xffffffffu, most);
@@ -73,7 +75,7 @@ int8_rows_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, int
   const bool bad = int8_bad(most);
   if (sub == 0 && lane == 0) d.scale[blockIdx.y * d.scale_batch + row * d.scale_row] = int8_scale(most);
   uint8_t* dst = d.q + blockIdx.y * d.q_batch + row * d.ld;
-  auto put = [&](const Eight<T>& e, int64_t k) {
+  auto put = [&](const Eight<T>& e, unsigned k) {
     uint32_t c[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) c[j] = int8_code(e.value(j), inv);
@@ -83,39 +85,49 @@ int8_rows_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, int
 #pragma unroll
   for (int i = 0; i < kInt8Pieces; ++i)
     if (first + i * step < end) put(v[i], first + i * step);
-  for (int64_t k = first + kInt8Pieces * step; k < end; k += step) {
+  for (unsigned k = first + kInt8Pieces * step; k < end; k += step) {
     Eight<T> more;
-    more.template load<VEC>(src + k, (int)min((int64_t)8, end - k));
+    more.template load<VEC>(src + k, (int)min(8u, end - k));
     put(more, k);
   }
 }
 
-// Codes of x^T [K, M] of x [M, K].  A CTA: 64 columns; thread (rg, cg) has rows 8 rg .. 8 rg + 7 of 256 and columns 8 cg .. 8 cg + 7.
+// Codes of x^T [K, M] of x [M, K].  A cluster of `parts` CTAs has 64 columns and shares out the rows; each keeps the last 256 of its own in
+// registers, thread (rg, cg) rows 8 rg .. 8 rg + 7 of each 256 and columns 8 cg .. 8 cg + 7, and reads what is before them twice, from L2 the
+// second time: four CTAs to a strip, since of one to a strip what all have under way is more than L2 holds (2880 x 5760 of 32 experts: 410 us,
+// two 379, four 344, eight 539; 512 rows each in registers, clusters of six: 373).
 // Codes are parked as [64 columns][256 rows] with the 8-byte units of a column permuted (unit rg lies at rg ^ 4 cg), so that the eight
 // columns that a warp writes at a time fall on different banks.
+constexpr int kInt8MaxParts = 4;
+
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
-int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K) {
-  constexpr int kWords = sizeof(T) == 2 ? 4 : 8;           // largest magnitudes of eight columns: bf16 two to a word
+__global__ void __launch_bounds__(256, VEC && sizeof(T) == 2 ? 4 : 2)
+int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, int parts) {
+  constexpr int kWords = sizeof(T) == 2 ? 4 : 8;      // largest magnitudes of eight columns: bf16 two to a word
   __shared__ __align__(16) uint8_t s_codes[64 * 256];
   __shared__ uint32_t s_max[8][8 * kWords];
+  __shared__ uint32_t s_top[64];
   __shared__ float s_inv[64];
-  __shared__ uint32_t s_bad[64];
+  __shared__ uint32_t s_keep[64];
   const int cg = threadIdx.x & 7, rg = threadIdx.x >> 3, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c0 = (int64_t)blockIdx.x * 64, k = c0 + 8 * cg;
+  const unsigned part = cluster_ctarank();
+  const int64_t rows = ((M + parts - 1) / parts + 15) & ~(int64_t)15, first = part * rows, end = min(M, first + rows);
+  const int64_t held = first + (rows - 1) / 256 * 256;         // rows from here on stay in registers
+  const int64_t c0 = (int64_t)(blockIdx.x / parts) * 64, k = c0 + 8 * cg;
   const int columns = (int)max((int64_t)0, min((int64_t)8, K - k));
   pdl_trigger();
   pdl_wait();
   const T* src = after_wait(x) + (int64_t)blockIdx.y * M * K + k;
   Eight<T> v[8];
   auto load = [&](int64_t m) {
+    const T* p = src + m * K;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i].template load<VEC>(src + (m + i) * K, m + i < M ? columns : 0);
+    for (int i = 0; i < 8; ++i, p += K) v[i].template load<VEC>(p, m + i < end ? columns : 0);
   };
   uint32_t most[kWords];
 #pragma unroll
   for (int j = 0; j < kWords; ++j) most[j] = 0;
-  for (int64_t m0 = 0; m0 < M; m0 += 256) {
+  for (int64_t m0 = first; m0 <= held; m0 += 256) {
     load(m0 + 8 * rg);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i].most_by_column(most);
@@ -130,8 +142,8 @@ int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K) 
     if (lane < 8) s_max[warp][kWords * cg + j] = most[j];
   }
   __syncthreads();
-  if (threadIdx.x < 64) {
-    const int c = threadIdx.x;
+  const int c = threadIdx.x;               // (below 64: a column)
+  if (c < 64) {
     uint32_t top = 0;
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
@@ -142,33 +154,43 @@ int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K) 
         top = max(top, s_max[w][c]);
       }
     }
-    s_inv[c] = int8_inverse(top);
-    s_bad[c] = int8_bad(top) ? 0u : 0xffffffffu;
-    if (c0 + c < K) d.scale[blockIdx.y * d.scale_batch + (c0 + c) * d.scale_row] = int8_scale(top);
+    s_top[c] = top;
   }
-  __syncthreads();
+  cluster_sync_all();
+  if (c < 64) {
+    const uint32_t at = smem_addr_u32(s_top + c);
+    uint32_t top = 0;
+    for (int o = 0; o < parts; ++o) top = max(top, __float_as_uint(ld_shared_cluster_f32(mapa_u32(at, (uint32_t)o))));
+    s_inv[c] = int8_inverse(top);
+    s_keep[c] = int8_bad(top) ? 0u : 0xffffffffu;
+    if (part == 0 && c0 + c < K) d.scale[blockIdx.y * d.scale_batch + (c0 + c) * d.scale_row] = int8_scale(top);
+  }
+  cluster_sync_all();                      // (also: no CTA ends before the others have read its maxima)
   uint8_t* dst = d.q + blockIdx.y * d.q_batch;
-  // the part that is still in registers first, the others backwards: L2 holds the last ones best
-  for (int64_t m0 = (M - 1) / 256 * 256; m0 >= 0; m0 -= 256) {
-    if (m0 + 256 < M) load(m0 + 8 * rg);
+  auto put = [&](int64_t m0) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float f = s_inv[8 * cg + j];
-      const uint32_t keep = s_bad[8 * cg + j];
-      uint32_t c[8];
+      const uint32_t keep = s_keep[8 * cg + j];
+      uint32_t q[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = int8_code(v[i].value(j), f);
+      for (int i = 0; i < 8; ++i) q[i] = int8_code(v[i].value(j), f);
       *reinterpret_cast<uint2*>(s_codes + (8 * cg + j) * 256 + ((rg ^ (cg << 2)) << 3)) =
-          make_uint2(int8x4(c[0], c[1], c[2], c[3]) & keep, int8x4(c[4], c[5], c[6], c[7]) & keep);
+          make_uint2(int8x4(q[0], q[1], q[2], q[3]) & keep, int8x4(q[4], q[5], q[6], q[7]) & keep);
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int c = 16 * i + (threadIdx.x >> 4), u = threadIdx.x & 15;      // 16 bytes: rows m0 + 16 u ...
-      const uint4 q = *reinterpret_cast<const uint4*>(s_codes + c * 256 + (((2 * u) ^ ((c >> 3) << 2)) << 3));
-      if (c0 + c < K && m0 + 16 * u < M) *reinterpret_cast<uint4*>(dst + (c0 + c) * d.ld + m0 + 16 * u) = q;
+      const int col = 16 * i + (threadIdx.x >> 4), u = threadIdx.x & 15;      // 16 bytes: rows m0 + 16 u ...
+      const uint4 q = *reinterpret_cast<const uint4*>(s_codes + col * 256 + (((2 * u) ^ ((col >> 3) << 2)) << 3));
+      if (c0 + col < K && m0 + 16 * u < end) *reinterpret_cast<uint4*>(dst + (c0 + col) * d.ld + m0 + 16 * u) = q;
     }
     __syncthreads();
+  };
+  put(held);
+  for (int64_t m0 = held - 256; m0 >= first; m0 -= 256) {      // backwards: L2 holds the last ones best
+    load(m0 + 8 * rg);
+    put(m0);
   }
 }
 
@@ -178,16 +200,17 @@ inline int launch_int8_quantize(const T* x, const Int8Out& d, int64_t B, int64_t
   const bool vec = rows_of_16_bytes<T>(x, K);
   if (transpose) {
     const int64_t strips = ceil_div(K, 64);
-    if (strips > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
+    if (strips * kInt8MaxParts > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
     auto kern = vec ? int8_columns_quantize_kernel<T, true> : int8_columns_quantize_kernel<T, false>;
-    return launch_behind(kern, dim3((unsigned)strips, (unsigned)B), dim3(256), 0, st, x, d, M, K);
+    const int parts = (int)std::min<int64_t>(kInt8MaxParts, ceil_div(M, 256));
+    return launch_clusters(kern, parts, true, dim3((unsigned)(strips * parts), (unsigned)B), dim3(256), 0, st, x, d, M, K, parts);
   }
-  int wpr = 1;
-  while (wpr < kInt8RowWarps && K > (int64_t)wpr * kInt8Pieces * 256) wpr *= 2;
-  const int64_t ctas = ceil_div(M, kInt8RowWarps / wpr);
+  int log_wpr = 0;
+  while ((1 << log_wpr) < kInt8RowWarps && K > (kInt8Pieces * 256) << log_wpr) ++log_wpr;
+  const int64_t ctas = ceil_div(M, kInt8RowWarps >> log_wpr);
   if (ctas > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
   auto kern = vec ? int8_rows_quantize_kernel<T, true> : int8_rows_quantize_kernel<T, false>;
-  return launch_behind(kern, dim3((unsigned)ctas, (unsigned)B), dim3(kInt8RowWarps * 32), 0, st, x, d, M, K, wpr);
+  return launch_behind(kern, dim3((unsigned)ctas, (unsigned)B), dim3(kInt8RowWarps * 32), 0, st, x, d, M, (int)K, log_wpr);
 }
 
 }  // namespace yb

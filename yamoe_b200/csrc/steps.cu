@@ -36,7 +36,7 @@ struct CombineCall {
   int E, K;
   template <typename TT, typename TW>
   CombineArgs<TT, TW> args() const {
-    return CombineArgs<TT, TW>{reinterpret_cast<const TT*>(rows), row_of, reinterpret_cast<const TW*>(weights), indices, T, n_rows, H, K, E};
+    return CombineArgs<TT, TW>{reinterpret_cast<const TT*>(rows), row_of, reinterpret_cast<const TW*>(weights), indices, T, n_rows, (int)H, K, E};
   }
 };
 
@@ -63,7 +63,7 @@ static int combine_backward_impl(const CombineCall& c, const void* d_out, void* 
 static int check_combine(const CombineCall& c, int weight_dtype, int dtype) {
   if (!known_dtype(dtype) || (c.weights != nullptr && weight_dtype != dtype && weight_dtype != YAMOE_F32)) return YAMOE_ERR_DTYPE;
   if (c.T < 0 || c.n_rows < 0 || c.H < 0 || c.K < 0 || c.E < 0) return YAMOE_ERR_BAD_ARG;
-  if (!countable(c.T, c.K) || c.H >= kMaxExtent || c.n_rows > kMaxRows) return YAMOE_ERR_UNSUPPORTED;
+  if (!countable(c.T, c.K) || c.H > kMaxRows || c.n_rows > kMaxRows) return YAMOE_ERR_UNSUPPORTED;
   const int64_t S = c.T * c.K;
   if (S > 0 && (c.row_of == nullptr || !at_boundary(c.row_of, 4))) return YAMOE_ERR_BAD_ARG;
   if (S > 0 && c.n_rows > 0 && c.H > 0 && (c.rows == nullptr || !at_boundary(c.rows, size_of(dtype)))) return YAMOE_ERR_BAD_ARG;
@@ -174,7 +174,7 @@ int yamoe_b200_int8_quantize(const void* x, const yamoe_int8_matrix_t* out, int6
   if (batch == 0 || rows == 0) return YAMOE_OK;
   if (cols > 0 && (x == nullptr || !at_boundary(x, size_of(dtype)))) return YAMOE_ERR_BAD_ARG;
   if (!int8_matrix_ok(out, batch, cols)) return YAMOE_ERR_BAD_ARG;
-  if (M >= kMaxExtent || K >= kMaxExtent) return YAMOE_ERR_UNSUPPORTED;
+  if (M > kMaxRows || K > kMaxRows) return YAMOE_ERR_UNSUPPORTED;
   const Int8Out d{reinterpret_cast<uint8_t*>(out->q), out->scale, out->ld, out->q_batch, out->scale_row, out->scale_batch};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == YAMOE_BF16 ? launch_int8_quantize(reinterpret_cast<const __nv_bfloat16*>(x), d, batch, M, K, transpose != 0, st)

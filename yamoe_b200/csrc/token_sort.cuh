@@ -78,14 +78,18 @@ __device__ __forceinline__ int load_expert(const int64_t* indices, int j, int en
   return -1 - lane;            // a key that no other lane has
 }
 
-// One 32-lane piece of a token's row to the rows of its K assignments.
+// One 32-lane piece of a token's row to the rows of its K assignments, the first four of which are looked up while it is on its way.
 template <typename P>
 __device__ __forceinline__ void copy_piece(const SortArgs& a, int64_t t, int i, int n, const int32_t* row_of) {
   if (i >= n) return;
   const P v = reinterpret_cast<const P*>(a.hidden + t * a.row_bytes)[i];
-  for (int k = 0; k < a.K; ++k) {
-    const int r = row_of[k];
-    if (r >= 0) reinterpret_cast<P*>(a.rows + r * a.row_bytes)[i] = v;
+  for (int k0 = 0; k0 < a.K; k0 += 4) {
+    int r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = k0 + k < a.K ? row_of[k0 + k] : -1;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (r[k] >= 0) reinterpret_cast<P*>(a.rows + r[k] * a.row_bytes)[i] = v;
   }
 }
 template <typename P>
@@ -93,12 +97,13 @@ __device__ __forceinline__ void zero_row(const SortArgs& a, int64_t r, int n, in
   P* d = reinterpret_cast<P*>(a.rows + r * a.row_bytes);
   for (int i = lane; i < n; i += 32) d[i] = P{};
 }
-// Rows without an assignment, 32 to a warp: lanes look, the warp writes.
+// Rows without an assignment, eight to a warp: lanes look, the warp writes.
+constexpr int kZeroRows = 8;
 template <typename P>
 __device__ __forceinline__ void zero_unused(const SortArgs& a, int64_t first, int n, int lane, const int32_t* offsets) {
   const int64_t r = first + lane;
   bool unused = false;
-  if (r < a.R) {
+  if (lane < kZeroRows && r < a.R) {
     if (a.capacity < 0) {
       unused = r >= offsets[a.E];
     } else {
@@ -167,13 +172,14 @@ sort_small_kernel(SortArgs a, int rounds) {
       }
     }
   __syncthreads();
-  const int n = (int)(a.row_bytes / sizeof(P)), chunks = (n + 31) / 32;
-  const int64_t warps = (int64_t)gridDim.x * kSortSmallWarps, at = (int64_t)blockIdx.x * kSortSmallWarps + w;
-  for (int64_t u = at; u < a.T * chunks; u += warps) {
-    const int64_t t = u / chunks;
+  const int n = (int)(a.row_bytes / sizeof(P));
+  const unsigned chunks = (unsigned)(n + 31) / 32;
+  const unsigned warps = gridDim.x * kSortSmallWarps, at = blockIdx.x * kSortSmallWarps + w;
+  for (unsigned u = at; u < (unsigned)a.T * chunks; u += warps) {
+    const unsigned t = u / chunks;
     copy_piece<P>(a, t, (int)(u - t * chunks) * 32 + lane, n, row_of + t * a.K);
   }
-  for (int64_t r = at * 32; r < a.R; r += warps * 32) zero_unused<P>(a, r, n, lane, offsets);
+  for (int64_t r = at * kZeroRows; r < a.R; r += warps * kZeroRows) zero_unused<P>(a, r, n, lane, offsets);
 }
 
 // ---- large: count, rank, copy -------------------------------------------------------------------------------------------
@@ -279,22 +285,23 @@ sort_rank_kernel(SortArgs a) {
 
 constexpr int kCopyWarps = 8;
 
-// CTAs below `copy_ctas` copy, the others zero rows without an assignment.
+// CTAs below `zero_ctas` zero rows without an assignment, the others copy.
 template <typename P>
 __global__ void __launch_bounds__(kCopyWarps * 32)
-sort_copy_kernel(SortArgs a, unsigned copy_ctas) {
+sort_copy_kernel(SortArgs a, unsigned zero_ctas) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int n = (int)(a.row_bytes / sizeof(P)), chunks = (n + 31) / 32;
+  const int n = (int)(a.row_bytes / sizeof(P));
+  const unsigned chunks = (unsigned)(n + 31) / 32;
   pdl_trigger();
   pdl_wait();
   a.hidden = after_wait(a.hidden);
   const int32_t* row_of = after_wait(a.row_of);
-  if (blockIdx.x < copy_ctas) {
-    const int64_t u = (int64_t)blockIdx.x * kCopyWarps + w, t = u / chunks;
-    if (t < a.T) copy_piece<P>(a, t, (int)(u - t * chunks) * 32 + lane, n, row_of + t * a.K);
-  } else {
-    const int64_t first = ((int64_t)(blockIdx.x - copy_ctas) * kCopyWarps + w) * 32;
+  if (blockIdx.x < zero_ctas) {
+    const int64_t first = ((int64_t)blockIdx.x * kCopyWarps + w) * kZeroRows;
     if (first < a.R) zero_unused<P>(a, first, n, lane, after_wait(a.offsets));
+  } else {
+    const unsigned u = (blockIdx.x - zero_ctas) * kCopyWarps + w, t = u / chunks;
+    if (t < a.T) copy_piece<P>(a, t, (int)(u - t * chunks) * 32 + lane, n, row_of + t * a.K);
   }
 }
 
@@ -321,12 +328,13 @@ inline int allow_smem(Kern kern, size_t smem, PerDevice<size_t>& configured) {
 template <typename P>
 inline int launch_sort(SortArgs a, cudaStream_t st) {
   const int64_t n = a.row_bytes / (int64_t)sizeof(P), chunks = ceil_div(n, 32);
+  if (n > 0x7fffffff || a.T * chunks > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;      // 2^31 pieces of 512 bytes are 1 TB
   if (a.S <= kSortSmallMax) {
     static PerDevice<size_t> configured;
     const size_t smem = sort_small_smem(a.S, a.E);
     if (const int rc = allow_smem(sort_small_kernel<P>, smem, configured)) return rc;
     const int rounds = std::max(1, (int)ceil_div(a.S, kSortSmallThreads));
-    const int64_t work = std::max(ceil_div(a.T * chunks, kSortSmallWarps), ceil_div(a.R, kSortSmallWarps * 32));
+    const int64_t work = std::max(ceil_div(a.T * chunks, kSortSmallWarps), ceil_div(a.R, kSortSmallWarps * kZeroRows));
     const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(work, kSMs));
     return launch_behind(sort_small_kernel<P>, dim3((unsigned)grid), dim3(kSortSmallThreads), smem, st, a, rounds);
   }
@@ -337,10 +345,9 @@ inline int launch_sort(SortArgs a, cudaStream_t st) {
   static PerDevice<size_t> configured;
   if ((rc = allow_smem(sort_rank_kernel, sort_rank_smem(a.E), configured))) return rc;
   if ((rc = launch_behind(sort_rank_kernel, dim3(b.blocks), dim3(kSortThreads), sort_rank_smem(a.E), st, a))) return rc;
-  const int64_t copy = ceil_div(a.T * chunks, kCopyWarps), zero = ceil_div(a.R, kCopyWarps * 32);
-  if (copy + zero > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
+  const int64_t copy = ceil_div(a.T * chunks, kCopyWarps), zero = ceil_div(a.R, kCopyWarps * kZeroRows);
   if (copy + zero == 0) return YAMOE_OK;
-  return launch_behind(sort_copy_kernel<P>, dim3((unsigned)(copy + zero)), dim3(kCopyWarps * 32), 0, st, a, (unsigned)copy);
+  return launch_behind(sort_copy_kernel<P>, dim3((unsigned)(copy + zero)), dim3(kCopyWarps * 32), 0, st, a, (unsigned)zero);
 }
 
 // ---- combine --------------------------------------------------------------------------------------------------------------
@@ -350,8 +357,8 @@ struct CombineArgs {
   const int32_t* row_of;        // [T, K]; outside [0, n_rows): nothing
   const TW* weights;            // [T, K], or [T, E] with indices; null: 1
   const int64_t* indices;       // [T, K] columns of the weights; null: the slots
-  int64_t Tn, n_rows, H;
-  int K, E;
+  int64_t Tn, n_rows;
+  int H, K, E;
   __device__ __forceinline__ void behind_wait() {
     rows = after_wait(rows);
     row_of = after_wait(row_of);
@@ -378,6 +385,7 @@ struct CombineArgs {
 // VE neighbouring values: a 16-byte piece, or one value.
 template <typename T, int VE> struct Piece {
   uint4 q;
+  __device__ __forceinline__ void clear() { q = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void load(const T* p) { q = ld_written(reinterpret_cast<const uint4*>(p)); }
   __device__ __forceinline__ void get(float (&v)[VE]) const {
     const uint32_t u[4] = {q.x, q.y, q.z, q.w};
@@ -407,6 +415,7 @@ template <typename T, int VE> struct Piece {
 };
 template <typename T> struct Piece<T, 1> {
   T q;
+  __device__ __forceinline__ void clear() { DT<T>::st(&q, 0.f); }
   __device__ __forceinline__ void load(const T* p) { q = *p; }
   __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = DT<T>::ld(&q); }
   static __device__ __forceinline__ void put(T* p, const float (&v)[1]) { DT<T>::st(p, v[0]); }
@@ -414,39 +423,43 @@ template <typename T> struct Piece<T, 1> {
 
 // One warp per 32 pieces of a token; the rows of KB slots are on their way together.  Sums in fp32 in the order of the slots.
 template <typename T, typename TW, int VE, int KB>
-__global__ void __launch_bounds__(kCopyWarps * 32)
+__global__ void __launch_bounds__(kCopyWarps * 32, KB > 4 ? 4 : 5)
 combine_tokens_kernel(CombineArgs<T, TW> a, T* out) {
   pdl_trigger();
   pdl_wait();
   a.behind_wait();
-  const int64_t pieces = a.H / VE, chunks = (pieces + 31) / 32;
-  const int64_t u = (int64_t)blockIdx.x * kCopyWarps + (threadIdx.x >> 5), t = u / chunks;
-  const int64_t i = (u - t * chunks) * 32 + (threadIdx.x & 31);
-  if (t >= a.Tn || i >= pieces) return;
+  const unsigned pieces = (unsigned)a.H / VE, chunks = (pieces + 31) / 32;
+  const unsigned u = blockIdx.x * kCopyWarps + (threadIdx.x >> 5);
+  const int64_t t = u / chunks;
+  const int lane = threadIdx.x & 31;
+  const unsigned i = (u - (unsigned)t * chunks) * 32 + lane;
+  if (t >= a.Tn) return;
+  const bool there = i < pieces;
   float acc[VE];
 #pragma unroll
   for (int j = 0; j < VE; ++j) acc[j] = 0.f;
   for (int k0 = 0; k0 < a.K; k0 += KB) {
-    int r[KB];
-    float w[KB];
+    // lane k looks up slot k0 + k for all
+    const int slot = k0 + lane;
+    const int mine = lane < KB && slot < a.K ? a.row(t * a.K + slot) : -1;
     Piece<T, VE> q[KB];
 #pragma unroll
-    for (int k = 0; k < KB; ++k) r[k] = k0 + k < a.K ? a.row(t * a.K + k0 + k) : -1;
+    for (int k = 0; k < KB; ++k) {
+      const int r = __shfl_sync(0xffffffffu, mine, k);
+      q[k].clear();                        // what is left out adds 0 * 0
+      if (r >= 0 && there) q[k].load(a.rows + (int64_t)r * a.H + i * VE);
+    }
+    const float weight = mine >= 0 ? a.weight(t, slot) : 0.f;
 #pragma unroll
-    for (int k = 0; k < KB; ++k)
-      if (r[k] >= 0) q[k].load(a.rows + r[k] * a.H + i * VE);
+    for (int k = 0; k < KB; ++k) {
+      const float w = __shfl_sync(0xffffffffu, weight, k);
+      float v[VE];
+      q[k].get(v);
 #pragma unroll
-    for (int k = 0; k < KB; ++k) w[k] = r[k] >= 0 ? a.weight(t, k0 + k) : 0.f;
-#pragma unroll
-    for (int k = 0; k < KB; ++k)
-      if (r[k] >= 0) {
-        float v[VE];
-        q[k].get(v);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) acc[j] = fmaf(w[k], v[j], acc[j]);
-      }
+      for (int j = 0; j < VE; ++j) acc[j] = fmaf(w, v[j], acc[j]);
+    }
   }
-  Piece<T, VE>::put(out + t * a.H + i * VE, acc);
+  if (there) Piece<T, VE>::put(out + t * a.H + i * VE, acc);
 }
 
 // ---- gradients of the combine -----------------------------------------------------------------------------------------------
@@ -471,7 +484,7 @@ combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_w
                         int wpt, unsigned token_ctas) {
   extern __shared__ float s_dot[];              // [warps][K]
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t pieces = a.H / VE;
+  const unsigned pieces = (unsigned)a.H / VE;
   pdl_trigger();
   pdl_wait();
   a.behind_wait();
@@ -488,7 +501,7 @@ combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_w
     }
     for (unsigned todo = __ballot_sync(0xffffffffu, mine); todo != 0; todo &= todo - 1) {
       const int l = __ffs(todo) - 1, p0 = __shfl_sync(0xffffffffu, h, l);
-      for (int64_t i = lane; i < pieces; i += 32) {
+      for (unsigned i = lane; i < pieces; i += 32) {
         float acc[VE];
 #pragma unroll
         for (int j = 0; j < VE; ++j) acc[j] = 0.f;
@@ -522,13 +535,13 @@ combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_w
 #pragma unroll
     for (int k = 0; k < KB; ++k)
       own[k] = d_rows != nullptr && r[k] >= 0 && head[r[k]] == (int)(t * a.K + k0 + k) && next[t * a.K + k0 + k] < 0;
-    for (int64_t i = lane + 32 * part; i < pieces; i += 32 * wpt) {
+    for (unsigned i = lane + 32 * part; i < pieces; i += 32 * wpt) {
       Piece<T, VE> g, q[KB];
       g.load(d_out + t * a.H + i * VE);
       if (d_weights != nullptr) {
 #pragma unroll
         for (int k = 0; k < KB; ++k)
-          if (r[k] >= 0) q[k].load(a.rows + r[k] * a.H + i * VE);
+          if (r[k] >= 0) q[k].load(a.rows + (int64_t)r[k] * a.H + i * VE);
       }
       float d[VE];
       g.get(d);
@@ -543,7 +556,7 @@ combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_w
         }
 #pragma unroll
         for (int j = 0; j < VE; ++j) v[j] = wgt[k] * d[j];
-        if (own[k]) Piece<T, VE>::put(d_rows + r[k] * a.H + i * VE, v);
+        if (own[k]) Piece<T, VE>::put(d_rows + (int64_t)r[k] * a.H + i * VE, v);
       }
     }
     if (d_weights != nullptr) {
@@ -577,8 +590,8 @@ combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_w
 
 template <typename T, typename TW, int VE>
 inline int launch_combine_tokens_ve(const CombineArgs<T, TW>& a, T* out, cudaStream_t st) {
-  const int64_t ctas = ceil_div(a.Tn * ceil_div(a.H / VE, 32), kCopyWarps);
-  if (ctas > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
+  const int64_t chunks = a.Tn * ceil_div(a.H / VE, 32), ctas = ceil_div(chunks, kCopyWarps);
+  if (chunks > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
   auto kern = a.K <= 4 ? combine_tokens_kernel<T, TW, VE, 4> : combine_tokens_kernel<T, TW, VE, 8>;
   return launch_behind(kern, dim3((unsigned)ctas), dim3(kCopyWarps * 32), 0, st, a, out);
 }
