@@ -126,6 +126,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
   int32_t* s_tile = s_row + p.B + 1;                                           // grouped: [B + 1] row tiles before each expert's
 
   if (threadIdx.x == 0) {
+    for (const CUtensorMap* map : {&tmW, &tmX, &tmXsmall}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     for (int s = 0; s < kInt8Stages; ++s) mbar_init(smem_u32(&bar_full[s]), 2);   // arrive.expect_tx of both CTAs
     for (int s = 0; s < kInt8Groups; ++s) mbar_init(smem_u32(&bar_empty[s]), 1);
     for (int a = 0; a < 2; ++a) {
@@ -435,7 +436,7 @@ struct Int8Rows {
 // A sum does not depend on the order of its terms: lane (g, t) takes 16 neighbouring bytes of rows g and g + 8, words 0 and 1 of which are one
 // instruction's k, 2 and 3 the next one's, of weights and tokens alike.
 template <typename T, int NT, int U, bool GROUPED>
-__global__ void __launch_bounds__(kInt8RowsThreads)
+__global__ void __launch_bounds__(kInt8RowsThreads, NT == 1 ? 4 : 3)
 int8_rows_kernel(const Int8Rows d, const Int8Params<T> p) {
   constexpr int kRows = 8 * NT;
   __shared__ int s_sum[8][kRows][17];
@@ -638,20 +639,28 @@ inline int launch_int8_pair(const Int8Operand& X, const Int8Operand& W, Int8Para
     p.MT = (int)ceil_div(p.M, c.width);
     const int64_t tiles = (int64_t)p.B * p.MT * p.NT;
     const int64_t grid = c.splits > 1 ? 2 * c.splits * tiles : 2 * std::min<int64_t>(tiles, pairs);
-    // (clusters of four and more start behind the kernel before them: while that one holds SMs they would be placed badly)
-    return launch_clusters(kern, 2 * c.splits, c.splits == 1, dim3((unsigned)grid), dim3(kInt8Threads), smem, st, tmW, tmX, tmXs, p);
+    return launch_clusters(kern, 2 * c.splits, true, dim3((unsigned)grid), dim3(kInt8Threads), smem, st, tmW, tmX, tmXs, p);
   }
 }
 
+// U: with it four CTAs of eight rows fit an SM (1 x 5760 x 2880: 5.1 us; six blocks on their way, two CTAs, 6.7), three of up to 32 (16 rows 6.0,
+// 32 rows 9.1).  Blocks that a warp has come out even with U = 2 or 3.
 template <typename T, bool GROUPED>
 inline int launch_int8_rows(const Int8Rows& d, const Int8Params<T>& p, cudaStream_t st) {
   const dim3 grid((unsigned)ceil_div(p.N, 16), (unsigned)(GROUPED ? std::min<int64_t>(p.B, p.M) : p.B));
-  auto kern = p.M <= 8 ? int8_rows_kernel<T, 1, 6, GROUPED> : p.M <= 16 ? int8_rows_kernel<T, 2, 4, GROUPED> : int8_rows_kernel<T, 4, 2, GROUPED>;
+  const int64_t blocks = ceil_div(ceil_div(p.K, 64), 8);
+  auto kern = round_up(blocks, 2) < round_up(blocks, 3) ? int8_rows_kernel<T, 1, 2, GROUPED> : int8_rows_kernel<T, 1, 3, GROUPED>;
+  if constexpr (!GROUPED) {
+    if (p.M > 16) kern = int8_rows_kernel<T, 4, 1, GROUPED>;
+    else if (p.M > 8) kern = int8_rows_kernel<T, 2, 2, GROUPED>;
+  }
   return launch_behind(kern, grid, dim3(kInt8RowsThreads), 0, st, d, p);
 }
 
-// Few rows go by int8_rows_kernel.
-inline bool int8_few_rows(int64_t M, int64_t B, bool grouped) { return B <= 65535 && M <= (grouped ? 32 : 16); }
+// Few rows go by int8_rows_kernel: up to 32 (rows kernel / pairs, us: 32 x 5760 x 2880 9.1 / 9.2, 32 x 2048 x 1024 4.0 / 7.5; 64 x 5760 x 2880
+// 20 / 9.4), and up to eight of experts, which share weights no more than their number (one token of four experts, 5760 x 2880 each:
+// 12.9 / 16.4; sixteen rows of sixteen experts 89 / 44).
+inline bool int8_few_rows(int64_t M, int64_t B, bool grouped) { return B <= 65535 && M <= (grouped ? 8 : 32); }
 
 template <typename T>
 inline int launch_int8_mm(const Int8Operand& X, const Int8Operand& W, const Int8Params<T>& p, cudaStream_t st) {
