@@ -80,7 +80,7 @@ static int int8_mm_impl(const yamoe_int8_matrix_t& a, const yamoe_int8_matrix_t&
   p.sb = b.scale; p.sb_b = b.scale_batch; p.sb_n = b.scale_row;
   p.offsets = offsets;
   p.out = reinterpret_cast<T*>(out);
-  p.vec = N % 2 == 0 && at_boundary(out, 4);
+  p.wide = sizeof(T) == 2 && N % 8 == 0 && at_boundary(out, 16);
   p.status = status;
   p.splits = 1;
   return launch_int8_mm(Int8Operand{a.q, M, a.ld, a.q_batch}, Int8Operand{b.q, N, b.ld, b.q_batch}, p, st);
