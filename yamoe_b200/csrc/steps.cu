@@ -119,6 +119,7 @@ int yamoe_b200_sort_tokens(const void* hidden_states, const int64_t* router_indi
   a.offsets = offsets;
   a.T = K > 0 ? T : 0; a.R = R; a.row_bytes = H * (int64_t)size;
   a.S = (int)S; a.E = E; a.K = K;
+  while ((1 << a.bits) < E) ++a.bits;
   a.capacity = capacity < 0 ? -1 : (int)capacity;
   a.counts = reinterpret_cast<int32_t*>(workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
