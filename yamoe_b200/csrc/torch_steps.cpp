@@ -1,5 +1,7 @@
 // Torch binding of the expert layer's steps: `sort_tokens`, `combine_tokens`, `quantize_int8`, `int8_mm` and `glu_fp8` over the C ABI, with
 // the gradients of the three that have one.
+#include <ATen/cuda/EmptyTensor.h>
+
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -18,6 +20,12 @@ bool wants_grad(std::initializer_list<at::Tensor> tensors) {
   return false;
 }
 
+// A new tensor on the device of `like`, without the dispatcher (which takes as long as the smallest kernels do)
+at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) {
+  return at::detail::empty_cuda(shape, dtype, like.device(), std::nullopt);
+}
+at::Tensor scratch(size_t bytes, const at::Tensor& like) { return empty_on(like, {(int64_t)bytes}, at::kByte); }
+
 void check_float(const char* op, const char* name, const at::Tensor& t) {
   TORCH_CHECK(t.is_cuda(), op, ": ", name, " must be on CUDA");
   TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, op, ": ", name, " must be float32 or bfloat16, got ",
@@ -30,7 +38,7 @@ at::Tensor combine(const at::Tensor& rows, const at::Tensor& row_of, const at::T
   const at::Tensor r = rows.contiguous(), of = row_of.contiguous(), w = weights.defined() ? weights.contiguous() : weights,
                    idx = indices.defined() ? indices.contiguous() : indices;
   const int64_t T = of.size(0), K = of.size(1), H = r.size(-1);
-  at::Tensor out = at::empty({T, H}, r.options().requires_grad(false));
+  at::Tensor out = empty_on(r, {T, H}, r.scalar_type());
   int64_t n_rows = 1;                                  // (H may be 0)
   for (int64_t i = 0; i + 1 < r.dim(); ++i) n_rows *= r.size(i);
   check(yamoe_b200_combine_tokens(r.data_ptr(), n_rows, of.data_ptr<int32_t>(), w.defined() ? w.data_ptr() : nullptr,
@@ -60,12 +68,10 @@ Sorted sort_tokens(const at::Tensor& hidden_states, const at::Tensor& router_ind
   const c10::cuda::CUDAGuard guard(hidden_states.device());
   const at::Tensor hs = hidden_states.contiguous(), ri = router_indices.to(at::kLong).contiguous();
   Sorted s;
-  const auto ints = hs.options().dtype(at::kInt).requires_grad(false);
-  const auto floats = hs.options().requires_grad(false);
-  s.rows = C < 0 ? at::empty({T * K, H}, floats) : at::empty({E, C, H}, floats);
-  s.row_of = at::empty({T, K}, ints);
-  s.offsets = at::empty({E + 1}, ints);
-  const at::Tensor ws = workspace(yamoe_b200_sort_tokens_workspace_bytes(T, (int)E, (int)K), hs);
+  s.rows = C < 0 ? empty_on(hs, {T * K, H}, hs.scalar_type()) : empty_on(hs, {E, C, H}, hs.scalar_type());
+  s.row_of = empty_on(hs, {T, K}, at::kInt);
+  s.offsets = empty_on(hs, {E + 1}, at::kInt);
+  const at::Tensor ws = scratch(yamoe_b200_sort_tokens_workspace_bytes(T, (int)E, (int)K), hs);
   check(yamoe_b200_sort_tokens(hs.data_ptr(), ri.data_ptr<int64_t>(), s.rows.data_ptr(), s.row_of.data_ptr<int32_t>(),
                                s.offsets.data_ptr<int32_t>(), T, H, (int)E, (int)K, C, dtype_of(hs), ws.data_ptr(), (size_t)ws.numel(),
                                current_stream()),
@@ -167,10 +173,10 @@ struct CombineTokens : torch::autograd::Function<CombineTokens> {
       int64_t n_rows = 1;
       for (size_t i = 0; i + 1 < shape.size(); ++i) n_rows *= shape[i];
       const int64_t T = of.size(0), K = of.size(1), H = shape.back();
-      if (want_rows) out[0] = at::empty(shape, g.options());
+      if (want_rows) out[0] = empty_on(g, shape, g.scalar_type());
       // (indices without elements have no address: dense weights of tokens without slots)
       if (want_weights) out[2] = K > 0 ? at::empty_like(w) : at::zeros_like(w);
-      const at::Tensor ws = workspace(yamoe_b200_combine_tokens_backward_workspace_bytes(n_rows, T, (int)K), g);
+      const at::Tensor ws = scratch(yamoe_b200_combine_tokens_backward_workspace_bytes(n_rows, T, (int)K), g);
       check(yamoe_b200_combine_tokens_backward(g.data_ptr(), r.defined() ? r.data_ptr() : nullptr, n_rows, of.data_ptr<int32_t>(),
                                                w.defined() ? w.data_ptr() : nullptr, w.defined() ? dtype_of(w) : YAMOE_F32,
                                                idx.defined() ? idx.data_ptr<int64_t>() : nullptr, want_rows ? out[0].data_ptr() : nullptr,
@@ -227,7 +233,7 @@ yamoe_int8_matrix_t matrix_of(const Integers& m) {
 at::Tensor empty_codes(at::IntArrayRef shape, const at::Tensor& like) {
   std::vector<int64_t> held = shape.vec();
   held.back() = ceil_div(held.back(), 16) * 16;
-  const at::Tensor q = at::empty(held, like.options().dtype(at::kChar).requires_grad(false));
+  const at::Tensor q = empty_on(like, held, at::kChar);
   return held.back() == shape.back() ? q : q.narrow(-1, 0, shape.back());
 }
 
@@ -242,7 +248,7 @@ std::tuple<at::Tensor, at::Tensor> quantize_int8_cuda(const at::Tensor& x, bool 
   if (transpose) std::swap(shape[shape.size() - 1], shape[shape.size() - 2]);
   Integers m{empty_codes(shape, x), at::Tensor()};
   shape.pop_back();
-  m.scale = at::empty(shape, x.options().dtype(at::kFloat).requires_grad(false));
+  m.scale = empty_on(x, shape, at::kFloat);
   if (x.numel() == 0) {                                 // rows without values
     m.scale.fill_(0x1p-100f / 127.f);
     return {m.q, m.scale};
@@ -294,12 +300,11 @@ at::Tensor int8_mm_cuda(const at::Tensor& a, const at::Tensor& a_scale, const at
   } else {
     TORCH_CHECK(a.dim() == 2 || a.size(0) == B, "int8_mm: a and b must hold the same number of matrices");
   }
-  const auto options = a.options().dtype(out_dtype);
-  const at::Tensor out = a.dim() == 3 ? at::empty({B, M, N}, options) : at::empty({M, N}, options);
+  const at::Tensor out = a.dim() == 3 ? empty_on(a, {B, M, N}, out_dtype) : empty_on(a, {M, N}, out_dtype);
   if (out.numel() == 0) return out;
   if (K == 0 || B == 0) return out.zero_();
   const yamoe_int8_matrix_t x = matrix_of(ma), w = matrix_of(mb);
-  const at::Tensor ws = workspace(yamoe_b200_int8_mm_workspace_bytes(B, M, N, K), a);
+  const at::Tensor ws = scratch(yamoe_b200_int8_mm_workspace_bytes(B, M, N, K), a);
   check(yamoe_b200_int8_mm(&x, &w, grouped ? first.data_ptr<int32_t>() : nullptr, out.data_ptr(), B, M, N, K,
                            out_dtype == at::kFloat ? YAMOE_F32 : YAMOE_BF16, ws.data_ptr(), (size_t)ws.numel(), current_stream()),
         "int8_mm");
@@ -320,11 +325,11 @@ at::Tensor glu(const at::Tensor& pre, Checkpoint* keep) {
   int64_t M = 1;
   for (size_t i = 0; i + 1 < shape.size(); ++i) M *= shape[i];
   shape.back() = W / 2;
-  const at::Tensor out = at::empty(shape, x.options().requires_grad(false));
+  const at::Tensor out = empty_on(x, shape, x.scalar_type());
   const int64_t ld = ceil_div(W, 16) * 16;
   if (keep) {
-    keep->q = at::empty({M, ld}, x.options().dtype(at::kFloat8_e4m3fn).requires_grad(false));
-    keep->scale = at::empty({M, ceil_div(W, 128)}, x.options().dtype(at::kFloat).requires_grad(false));
+    keep->q = empty_on(x, {M, ld}, at::kFloat8_e4m3fn);
+    keep->scale = empty_on(x, {M, ceil_div(W, 128)}, at::kFloat);
   }
   check(yamoe_b200_glu_forward(x.data_ptr(), out.data_ptr(), keep ? keep->q.data_ptr() : nullptr,
                                keep ? keep->scale.data_ptr<float>() : nullptr, ld, M, W / 2, dtype_of(x), current_stream()),
@@ -358,7 +363,7 @@ struct GluFp8 : torch::autograd::Function<GluFp8> {
       const at::AutoDispatchBelowADInplaceOrView below;
       // hooks on saved tensors may give the codes back at another address
       const at::Tensor g = dy.contiguous(), q = aligned(saved[0]), scale = saved[1].contiguous();
-      d_pre = at::empty(ctx->saved_data["shape"].toIntVector(), g.options());
+      d_pre = empty_on(g, ctx->saved_data["shape"].toIntVector(), g.scalar_type());
       check(yamoe_b200_glu_backward(g.data_ptr(), q.data_ptr(), scale.data_ptr<float>(), q.size(1), d_pre.data_ptr(), q.size(0),
                                     d_pre.size(-1) / 2, dtype_of(g), current_stream()),
             "glu_fp8 (backward)");
