@@ -11,7 +11,7 @@
 // their way together, as in the quantisation of rows.  fp32 calls exp and divides as IEEE has it; for bf16 results the approximate
 // forms (2^-21) are far below half a step.
 #pragma once
-#include "fp8_quant.cuh"
+#include "int8_quant.cuh"
 
 namespace yb {
 
@@ -22,13 +22,6 @@ __device__ __forceinline__ float glu_sigmoid(float g) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * (-kAlpha * 1.4426950408889634f)));      // exp(x) = 2^(x log2 e)
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
   return s;
-}
-
-// Eight neighbouring values; VEC: rows are multiples of eight, so that all of them exist or none.
-template <bool VEC, typename T>
-__device__ __forceinline__ void load_eight(Eight<T>& v, const T* p, int n) {
-  if (VEC && n <= 0) v.template load<false>(p, 0);
-  else v.template load<VEC>(p, VEC ? 8 : n);
 }
 
 struct GluSaved {

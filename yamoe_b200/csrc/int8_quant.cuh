@@ -22,8 +22,15 @@ __device__ __forceinline__ float int8_scale(uint32_t most) {
   return int8_bad(most) ? __uint_as_float(0x7fc00000u) : __fdiv_rn(fp8_group_max(most), kInt8Max);
 }
 __device__ __forceinline__ float int8_inverse(uint32_t most) { return __fdiv_rn(kInt8Max, fp8_group_max(most)); }
-// x * inverse lies in [-127, 127]: added to 1.5 * 2^23 its nearest integer is the low byte of the sum.
+// x * inverse lies in [-127, 127]: added to 1.5 * 2^23 its nearest integer is the low byte of the sum.  (One value at a time: two, by mul.rn.f32x2 and
+// add.rn.f32x2, came out as one fma, which does not round the product.)
 __device__ __forceinline__ uint32_t int8_code(float x, float inverse) { return __float_as_uint(__fadd_rn(__fmul_rn(x, inverse), 12582912.f)); }
+// Eight neighbouring values of a row; VEC: rows are multiples of eight, so that all of them exist or none.
+template <bool VEC, typename T>
+__device__ __forceinline__ void load_eight(Eight<T>& v, const T* p, int n) {
+  if (VEC && n <= 0) v.template load<false>(p, 0);
+  else v.template load<VEC>(p, VEC ? 8 : n);
+}
 __device__ __forceinline__ uint32_t int8x4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
@@ -55,13 +62,13 @@ int8_rows_quantize_kernel(const T* x, const Int8Out d, int64_t M, int K, int log
 #pragma unroll
   for (int i = 0; i < kInt8Pieces; ++i) {
     const unsigned k = first + i * step;
-    v[i].template load<VEC>(src + k, k < end ? (int)min(8u, end - k) : 0);
+    load_eight<VEC>(v[i], src + k, k < end ? (int)min(8u, end - k) : 0);
   }
 #pragma unroll
   for (int i = 0; i < kInt8Pieces; ++i) most = max(most, v[i].most());
   for (unsigned k = first + kInt8Pieces * step; k < end; k += step) {
     Eight<T> more;
-    more.template load<VEC>(src + k, (int)min(8u, end - k));
+    load_eight<VEC>(more, src + k, (int)min(8u, end - k));
     most = max(most, more.most());
   }
   most = __reduce_max_sync(0xffffffffu, most);
@@ -87,7 +94,7 @@ int8_rows_quantize_kernel(const T* x, const Int8Out d, int64_t M, int K, int log
     if (first + i * step < end) put(v[i], first + i * step);
   for (unsigned k = first + kInt8Pieces * step; k < end; k += step) {
     Eight<T> more;
-    more.template load<VEC>(src + k, (int)min(8u, end - k));
+    load_eight<VEC>(more, src + k, (int)min(8u, end - k));
     put(more, k);
   }
 }
@@ -104,7 +111,7 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(256, VEC && sizeof(T) == 2 ? 4 : 2)
 int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, int parts) {
   constexpr int kWords = sizeof(T) == 2 ? 4 : 8;      // largest magnitudes of eight columns: bf16 two to a word
-  __shared__ __align__(16) uint8_t s_codes[64 * 256];
+  __shared__ __align__(16) uint8_t s_parked[2][64 * 256];
   __shared__ uint32_t s_max[8][8 * kWords];
   __shared__ uint32_t s_top[64];
   __shared__ float s_inv[64];
@@ -122,7 +129,7 @@ int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, 
   auto load = [&](int64_t m) {
     const T* p = src + m * K;
 #pragma unroll
-    for (int i = 0; i < 8; ++i, p += K) v[i].template load<VEC>(p, m + i < end ? columns : 0);
+    for (int i = 0; i < 8; ++i, p += K) load_eight<VEC>(v[i], p, m + i < end ? columns : 0);
   };
   uint32_t most[kWords];
 #pragma unroll
@@ -167,7 +174,10 @@ int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, 
   }
   cluster_sync_all();                      // (also: no CTA ends before the others have read its maxima)
   uint8_t* dst = d.q + blockIdx.y * d.q_batch;
+  int turn = 0;
   auto put = [&](int64_t m0) {
+    uint8_t* s_codes = s_parked[turn];
+    turn ^= 1;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const float f = s_inv[8 * cg + j];
@@ -185,7 +195,6 @@ int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, 
       const uint4 q = *reinterpret_cast<const uint4*>(s_codes + col * 256 + (((2 * u) ^ ((col >> 3) << 2)) << 3));
       if (c0 + col < K && m0 + 16 * u < end) *reinterpret_cast<uint4*>(dst + (c0 + col) * d.ld + m0 + 16 * u) = q;
     }
-    __syncthreads();
   };
   put(held);
   for (int64_t m0 = held - 256; m0 >= first; m0 -= 256) {      // backwards: L2 holds the last ones best
@@ -197,7 +206,7 @@ int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, 
 template <typename T>
 inline int launch_int8_quantize(const T* x, const Int8Out& d, int64_t B, int64_t M, int64_t K, bool transpose, cudaStream_t st) {
   if (B > 65535) return YAMOE_ERR_UNSUPPORTED;
-  const bool vec = rows_of_16_bytes<T>(x, K);
+  const bool vec = K % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   if (transpose) {
     const int64_t strips = ceil_div(K, 64);
     if (strips * kInt8MaxParts > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
