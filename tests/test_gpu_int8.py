@@ -254,3 +254,18 @@ def test_refusals():
     for bad, args in [("2D", (sa,)), ("float32 or bfloat16", (a,)), ("float32 or bfloat16", (torch.zeros(2, 2).half().cuda(),))]:
         with pytest.raises(RuntimeError, match=bad):
             q(*args)
+
+
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("K", [64, 250])
+def test_values_between_two_codes(transpose, K):
+    """A product with 127 / a is rounded to 32 bits before it is rounded to an integer: bf16 values of half the largest and the like."""
+    import yamoe_b200
+    gen = torch.Generator().manual_seed(1)
+    top = (torch.randint(128, 256, (400, 1), generator=gen).float() * 2.0 ** -6)
+    x = top * (torch.randint(-254, 255, (400, K), generator=gen).float() / 254)
+    x = x.to(BF16)
+    x[:, 0], x[:, 1] = top[:, 0].to(BF16), (top[:, 0] / 2).to(BF16)
+    q, s = yamoe_b200.quantize_int8((x.t().contiguous() if transpose else x).cuda(), transpose)
+    want = quantised(x)
+    assert torch.equal(q.cpu(), want[0]) and torch.equal(s.cpu(), want[1])

@@ -193,7 +193,7 @@ int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, 
     for (int i = 0; i < 4; ++i) {
       const int col = 16 * i + (threadIdx.x >> 4), u = threadIdx.x & 15;      // 16 bytes: rows m0 + 16 u ...
       const uint4 q = *reinterpret_cast<const uint4*>(s_codes + col * 256 + (((2 * u) ^ ((col >> 3) << 2)) << 3));
-      if (c0 + col < K && m0 + 16 * u < end) *reinterpret_cast<uint4*>(dst + (c0 + col) * d.ld + m0 + 16 * u) = q;
+      if (c0 + col < K && m0 + 16 * u < end) __stcs(reinterpret_cast<uint4*>(dst + (c0 + col) * d.ld + m0 + 16 * u), q);
     }
   };
   put(held);

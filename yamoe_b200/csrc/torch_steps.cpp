@@ -26,6 +26,8 @@ at::Tensor empty_on(const at::Tensor& like, at::IntArrayRef shape, at::ScalarTyp
 }
 at::Tensor scratch(size_t bytes, const at::Tensor& like) { return empty_on(like, {(int64_t)bytes}, at::kByte); }
 
+at::Tensor as_int64(const at::Tensor& t) { return !t.defined() || t.scalar_type() == at::kLong ? t : t.to(at::kLong); }
+
 void check_float(const char* op, const char* name, const at::Tensor& t) {
   TORCH_CHECK(t.is_cuda(), op, ": ", name, " must be on CUDA");
   TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, op, ": ", name, " must be float32 or bfloat16, got ",
@@ -66,7 +68,7 @@ Sorted sort_tokens(const at::Tensor& hidden_states, const at::Tensor& router_ind
   TORCH_CHECK(C < (int64_t)1 << 31 && E * std::max<int64_t>(C, 0) < (int64_t)1 << 31, "sort_tokens: too many rows");
   TORCH_CHECK(T * K < (int64_t)1 << 30, "sort_tokens: fewer than 2^30 assignments expected, got ", T * K);
   const c10::cuda::CUDAGuard guard(hidden_states.device());
-  const at::Tensor hs = hidden_states.contiguous(), ri = router_indices.to(at::kLong).contiguous();
+  const at::Tensor hs = hidden_states.contiguous(), ri = as_int64(router_indices).contiguous();
   Sorted s;
   s.rows = C < 0 ? empty_on(hs, {T * K, H}, hs.scalar_type()) : empty_on(hs, {E, C, H}, hs.scalar_type());
   s.row_of = empty_on(hs, {T, K}, at::kInt);
@@ -143,7 +145,6 @@ void check_combine(const at::Tensor& rows, const at::Tensor& row_of, const at::T
 
 // arguments as the kernels take them
 at::Tensor or_none(const std::optional<at::Tensor>& t) { return t.has_value() ? *t : at::Tensor(); }
-at::Tensor as_int64(const at::Tensor& t) { return t.defined() ? t.to(at::kLong) : t; }
 
 struct CombineTokens : torch::autograd::Function<CombineTokens> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& rows, const at::Tensor& row_of,
