@@ -78,21 +78,21 @@ def numbers(text, name):
 
 
 def test_the_ring_fits_beside_the_tables():
-    """Stages by width, and shared memory with 1024 experts: 227 KB less the static arrays."""
-    def stage(width):
+    """Groups of k-blocks by width, and shared memory with 1024 experts: 227 KB less the static arrays."""
+    def block(width):
         return 128 * 128 + (width + 63) // 64 * 4096
-    ring = 10 * stage(64)
+    ring = 10 * block(64)
     for width in range(32, 257, 32):
-        stages = ring // stage(width) & ~1
-        assert 6 <= stages <= 10 and stages * stage(width) <= ring
+        groups = ring // (2 * block(width))
+        assert 3 <= groups <= 5 and 2 * groups * block(width) <= ring
         half = width // 2                       # rows of tokens that a CTA copies: boxes of 32, or one of 128
         boxes = 4 if half > 96 else -(-half // 32)
-        assert half <= 32 * boxes and 128 * 128 + boxes * 4096 <= stage(width)
+        assert half <= 32 * boxes and 128 * 128 + boxes * 4096 <= block(width)
         for splits in (2, 3, 4):                # sums that meet in the ring's place
             slots = {(c // splits * splits + part) for c in range(width // 32) for part in range(splits)}
             assert (max(slots) + 1) * 128 * 32 * 4 <= ring
     text = source("int8_gemm.cuh")
-    assert "return 128 * 128 + (width + 63) / 64 * 4096;" in text and "kInt8Ring = 10 * int8_stage_bytes(64)" in text
+    assert "return 128 * 128 + (width + 63) / 64 * 4096;" in text and "kInt8Ring = 10 * int8_block_bytes(64)" in text
     assert ring + 1024 + 8 * 32 * 64 + 2 * 1025 * 4 + 512 <= 227 * 1024
 
 

@@ -9,9 +9,10 @@
 //
 // int8_pair_kernel.  As in umma_pair.cuh, CTA pairs with the weights' rows (output columns) in the instruction's M dimension, 256 to a pair, and
 // the tokens' rows in its N dimension, any multiple of 32 up to 256: an expert's rows are cut into tiles of equal width wherever they
-// begin, so nothing is padded in memory, and few rows cost few clocks.  A k-block is 128 bytes wide, one swizzle row, 32 KB per CTA; six
-// stages, freed two at a time; two accumulators, so that a tile is scaled and stored while the next is multiplied.  Scales are met in the
-// epilogue alone, unlike the e4m3 products with a scale per 128 (fp8_gemm.cuh), whose sums leave TMEM after every block.
+// begin, so nothing is padded in memory, and few rows cost few clocks.  A k-block is 128 bytes wide, one swizzle row, up to 32 KB per CTA;
+// two accumulators, so that a tile is scaled and stored while the next is multiplied.  Scales are met in the epilogue alone, unlike the
+// e4m3 products with a scale per 128 (fp8_gemm.cuh), whose sums leave TMEM after every block.  8192 x 5760 x 2880: 88 us on a cool GPU, 3.1
+// PFLOP/s, 111 for seconds on end under the power cap; 2048 rows of 32 experts, 5760 x 2880 each: 98 us, 5.7 TB/s.
 // Few tiles: a cluster of up to four pairs shares a tile's k-blocks; the chunks of 32 rows are dealt out among the pairs, each of which gets
 // the others' sums of its chunks through distributed shared memory.
 //
@@ -26,12 +27,14 @@
 
 namespace yb {
 
-// A stage: this CTA's 128 rows of weights and half of the tile's rows of tokens in boxes of 32, 128 bytes each.  Narrow tiles have small stages
-// and more of them: what bounds them is how many copies are on their way (six of any width: 425 clocks per k-block up to 256 rows).
-constexpr int int8_stage_bytes(int width) { return 128 * 128 + (width + 63) / 64 * 4096; }
-constexpr int kInt8Ring = 10 * int8_stage_bytes(64), kInt8MaxStages = 10, kInt8MaxGroups = kInt8MaxStages / 2;
-constexpr int int8_stages(int width) { return kInt8Ring / int8_stage_bytes(width) & ~1; }
-static_assert(int8_stages(32) == 10 && int8_stages(128) == 8 && int8_stages(192) == 6 && int8_stages(256) == 6, "");
+// A k-block: this CTA's 128 rows of weights and half of the tile's rows of tokens in boxes of 32, 128 bytes each.  Blocks come, are multiplied and
+// are given back in groups: two at a time, which spares the warps every other wait (64 x 5760 x 2880: one at a time 9.3 us, two 8.3), but for
+// the widest tiles, whose instructions take longer than the waits and of which the ring holds three groups of two (8192 x 5760 x 2880: 88, 93).
+constexpr int int8_block_bytes(int width) { return 128 * 128 + (width + 63) / 64 * 4096; }
+constexpr int int8_depth(int width) { return width > 192 ? 1 : 2; }
+constexpr int kInt8Ring = 10 * int8_block_bytes(64), kInt8MaxGroups = 6;
+constexpr int int8_groups(int width) { return kInt8Ring / (int8_depth(width) * int8_block_bytes(width)); }
+static_assert(int8_groups(32) == 5 && int8_groups(128) == 4 && int8_groups(192) == 3 && int8_groups(256) == kInt8MaxGroups, "");
 constexpr int kInt8EpiWarps = 8, kInt8Threads = 32 * (3 + kInt8EpiWarps);
 constexpr int kInt8ParkBytes = 32 * 64;                  // 32 rows of an epilogue warp's 32 columns on their way out
 constexpr int kInt8RingBytes = kInt8Ring + 1024;         // + slack for 1024-byte alignment
@@ -50,7 +53,7 @@ struct Int8Params {
   int64_t M;                    // rows per matrix, or of all experts
   int N, K, B;                  // columns, reduction length, matrices (experts)
   int width;                    // rows of a tile at most, a multiple of 32
-  int stages, stage_bytes;      // of the ring, for tiles of that width
+  int groups, depth, block_bytes;       // of the ring: groups of `depth` k-blocks, for tiles of that width
   int MT, NT;                   // tiles of `width` rows per matrix (not grouped), of 256 columns
   const float* sa;              // scale of (matrix b, row m) at b * sa_b + m * sa_m
   const float* sb;
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(kInt8Threads, 1)
 int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                  const __grid_constant__ CUtensorMap tmXsmall, const Int8Params<T> p) {
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_full[kInt8MaxStages];       // used in the leader CTA of the pair
+  __shared__ __align__(8) uint64_t bar_full[kInt8MaxGroups];       // used in the leader CTA of the pair
   __shared__ __align__(8) uint64_t bar_empty[kInt8MaxGroups];      // per CTA
   __shared__ __align__(8) uint64_t bar_tmem_full[2];            // per CTA
   __shared__ __align__(8) uint64_t bar_tmem_empty[2];           // used in the leader CTA
@@ -150,15 +153,17 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
   const bool leader = rank == 0;
   const uint16_t pair_mask = (uint16_t)(3u << lead);
   const int splits = GROUPED ? 1 : p.splits, part = (int)(cta >> 1);
-  const int stages = p.stages, stage_bytes = p.stage_bytes;
+  const int groups = p.groups, depth = p.depth, block_bytes = p.block_bytes;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   int32_t* s_row = reinterpret_cast<int32_t*>(smem_raw + kInt8RingBytes + kInt8EpiWarps * kInt8ParkBytes);      // grouped: [B + 1] first row of each expert
   int32_t* s_tile = s_row + p.B + 1;                                           // grouped: [B + 1] row tiles before each expert's
 
   if (threadIdx.x == 0) {
     for (const CUtensorMap* map : {&tmW, &tmX, &tmXsmall}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-    for (int s = 0; s < stages; ++s) mbar_init(smem_u32(&bar_full[s]), 2);   // arrive.expect_tx of both CTAs
-    for (int s = 0; s < stages / 2; ++s) mbar_init(smem_u32(&bar_empty[s]), 1);
+    for (int s = 0; s < groups; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), 2);    // arrive.expect_tx of both CTAs
+      mbar_init(smem_u32(&bar_empty[s]), 1);
+    }
     for (int a = 0; a < 2; ++a) {
       mbar_init(smem_u32(&bar_tmem_full[a]), 1);
       mbar_init(smem_u32(&bar_tmem_empty[a]), 2 * kInt8EpiWarps);
@@ -184,33 +189,45 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     for (int i = threadIdx.x; i <= p.B; i += kInt8Threads) s_row[i] = int8_offset(offsets, i, p.M);
     __syncthreads();
     if (warp == 0) {
-      int before = 0;
+      // first rows, none below one before it (which keeps whatever the table holds within the rows), and the numbers of tiles
+      int before = 0, top = s_row[0];
       for (int e0 = 0; e0 < p.B; e0 += 32) {
         const int e = e0 + lane;
-        int tiles = e < p.B ? (max(0, s_row[e + 1] - s_row[e]) + p.width - 1) / p.width : 0;
+        int end = max(top, e < p.B ? s_row[e + 1] : 0);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, end, o);
+          if (lane >= o) end = max(end, up);
+        }
+        int first = __shfl_up_sync(0xffffffffu, end, 1);
+        if (lane == 0) first = top;
+        int tiles = (end - first + p.width - 1) / p.width;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int up = __shfl_up_sync(0xffffffffu, tiles, o);
           if (lane >= o) tiles += up;
         }
-        if (e < p.B) s_tile[e + 1] = before + tiles;
+        if (e < p.B) {
+          s_row[e + 1] = end;
+          s_tile[e + 1] = before + tiles;
+        }
         before += __shfl_sync(0xffffffffu, tiles, 31);
+        top = __shfl_sync(0xffffffffu, end, 31);
       }
       if (lane == 0) s_tile[0] = 0;
     }
     __syncthreads();
   }
-  const int64_t total = (GROUPED ? (int64_t)s_tile[p.B] : (int64_t)p.B * p.MT) * p.NT;
-  const int64_t first_id = blockIdx.x / (2 * splits), n_workers = gridDim.x / (2 * splits);
+  const int total = (GROUPED ? s_tile[p.B] : p.B * p.MT) * p.NT;             // (the host keeps them below 2^30)
+  const int first_id = blockIdx.x / (2 * splits), n_workers = gridDim.x / (2 * splits);
   const int kblocks_all = (p.K + 127) >> 7;
   const int kb_first = part * kblocks_all / splits, kb_end = (part + 1) * kblocks_all / splits;
 
   // work item -> matrix or expert, first column, first row, its end, width (a multiple of 32)
-  auto decode = [&](int64_t id, int& b, int& m0, int64_t& row0, int64_t& row_end, int& width) {
-    int local, tiles;
-    int64_t first, rows;
+  auto decode = [&](int id, int& b, int& m0, int& row0, int& row_end, int& width) {
+    int local, tiles, first, rows;
     if constexpr (GROUPED) {
-      const int tile = (int)(id / p.NT);                // experts' tiles follow each other, NT items to each
+      const int tile = id / p.NT;                       // experts' tiles follow each other, NT items to each
       int lo = 0, hi = p.B;                             // the last expert whose first tile is not behind this one
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -218,24 +235,24 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
       }
       b = lo;
       tiles = s_tile[b + 1] - s_tile[b];
-      local = (int)(id - (int64_t)s_tile[b] * p.NT);
+      local = id - s_tile[b] * p.NT;
       first = s_row[b];
       rows = s_row[b + 1] - first;
     } else {
-      const int64_t per = (int64_t)p.MT * p.NT;
-      b = (int)(id / per);
-      local = (int)(id - b * per);
+      const int per = p.MT * p.NT;
+      b = id / per;
+      local = id - b * per;
       tiles = p.MT;
       first = 0;
-      rows = p.M;
+      rows = (int)p.M;
     }
     // the row tile varies fastest, so that the pairs running at a time share weights in L2
     const int nt = local / tiles;
-    const int step = (int)(((rows + tiles - 1) / tiles + 31) & ~31);
+    const int step = ((rows + tiles - 1) / tiles + 31) & ~31;
     m0 = nt * 256;
-    row0 = first + (int64_t)(local - nt * tiles) * step;
+    row0 = first + (local - nt * tiles) * step;
     row_end = min(first + rows, row0 + step);
-    width = (int)((row_end - row0 + 31) & ~31);          // (tiles of at most 256 rows, rounded up to 32: none is left without rows)
+    width = (row_end - row0 + 31) & ~31;                 // (tiles of at most 256 rows, rounded up to 32: none is left without rows)
   };
 
   if (warp == 0 || warp == 2 + kInt8EpiWarps) {
@@ -243,43 +260,43 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     // one warp for the weights, which also announces the bytes of both, and one for the tokens
     const bool for_w = warp == 0;
     const bool elected = elect_one();
-    int stage = 0;
+    int group = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int64_t id = first_id; id < total && ok; id += n_workers) {
-      int b, m0, width;
-      int64_t row0, row_end;
+    for (int id = first_id; id < total && ok; id += n_workers) {
+      int b, m0, row0, row_end, width;
       decode(id, b, m0, row0, row_end, width);
-      const int half = width >> 1, my_m = m0 + (int)rank * 128, my_row = (int)row0 + (int)rank * half;
+      const int half = width >> 1, my_m = m0 + (int)rank * 128, my_row = row0 + (int)rank * half;
       const bool load_w = my_m < p.N;      // nothing of this CTA's columns exists: its results are not read
       const bool big = half > 96;
       const int small = (half + 31) >> 5;
       const uint32_t bytes = (load_w ? 128 * 128 : 0) + (big ? 128 * 128 : small * 4096);
-      for (int kb = kb_first; kb < kb_end; ++kb) {
-        if ((stage & 1) == 0) {
-          ok = mbar_wait_warp(smem_u32(&bar_empty[stage >> 1]), phase ^ 1u, &abort_flag);
-          if (!ok) break;
-        }
+      for (int kb = kb_first; kb < kb_end; kb += depth) {
+        ok = mbar_wait_warp(smem_u32(&bar_empty[group]), phase ^ 1u, &abort_flag);
+        if (!ok) break;
+        const int blocks = min(depth, kb_end - kb);
         if (elected) {
-          const uint32_t full = mapa_u32(smem_u32(&bar_full[stage]), lead);
-          const uint32_t sw = smem_base + stage * stage_bytes, sx = sw + 128 * 128;
-          const int k0 = kb * 128;
-          if (for_w) {
-            mbar_expect_tx_cluster(full, bytes);
-            if (load_w) tma2_load_3d(sw, &tmW, k0, my_m, b, full);
-          } else if (big) {
-            tma2_load_3d(sx, &tmX, k0, my_row, GROUPED ? 0 : b, full);
-          } else {
-            for (int i = 0; i < small; ++i) tma2_load_3d(sx + i * 4096, &tmXsmall, k0, my_row + 32 * i, GROUPED ? 0 : b, full);
+          const uint32_t full = mapa_u32(smem_u32(&bar_full[group]), lead);
+          if (for_w) mbar_expect_tx_cluster(full, blocks * bytes);
+          for (int k = 0; k < blocks; ++k) {
+            const uint32_t sw = smem_base + (depth * group + k) * block_bytes, sx = sw + 128 * 128;
+            const int k0 = (kb + k) * 128;
+            if (for_w) {
+              if (load_w) tma2_load_3d(sw, &tmW, k0, my_m, b, full);
+            } else if (big) {
+              tma2_load_3d(sx, &tmX, k0, my_row, GROUPED ? 0 : b, full);
+            } else {
+              for (int i = 0; i < small; ++i) tma2_load_3d(sx + i * 4096, &tmXsmall, k0, my_row + 32 * i, GROUPED ? 0 : b, full);
+            }
           }
         }
         __syncwarp();
-        if (++stage == stages) { stage = 0; phase ^= 1u; }
+        if (++group == groups) { group = 0; phase ^= 1u; }
       }
     }
-    // the commits that free the last stages must have arrived here before this CTA ends
-    for (int g = 0; g < stages / 2 && ok; ++g)
-      ok = mbar_wait_warp(smem_u32(&bar_empty[g]), 2 * g < stage ? phase : phase ^ 1u, &abort_flag);
+    // the commits that free the last groups must have arrived here before this CTA ends
+    for (int g = 0; g < groups && ok; ++g)
+      ok = mbar_wait_warp(smem_u32(&bar_empty[g]), g < group ? phase : phase ^ 1u, &abort_flag);
     if (!ok && lane == 0) {
       abort_flag = 1;
       atomicMax(p.status, (int)kStatusProducerTimeout);
@@ -292,37 +309,38 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
       constexpr uint32_t idesc_base = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(256 >> 4) << 24);
       const uint64_t wdesc0 = make_smem_desc(smem_base, 16, 1024), xdesc0 = make_smem_desc(smem_base + 128 * 128, 16, 1024);
       const bool elected = elect_one();
-      int stage = 0, acc = 0;
+      int group = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int64_t id = first_id; id < total && ok; id += n_workers) {
-        int b, m0, width;
-        int64_t row0, row_end;
+      for (int id = first_id; id < total && ok; id += n_workers) {
+        int b, m0, row0, row_end, width;
         decode(id, b, m0, row0, row_end, width);
         const uint32_t idesc = idesc_base | ((uint32_t)(width >> 3) << 17);
         ok = mbar_wait_warp(smem_u32(&bar_tmem_empty[acc]), acc_phase ^ 1u, &abort_flag);
         if (!ok) break;
         tc_fence_after();
-        for (int kb = kb_first; kb < kb_end; ++kb) {
-          ok = mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &abort_flag);
+        for (int kb = kb_first; kb < kb_end; kb += depth) {
+          ok = mbar_wait_warp(smem_u32(&bar_full[group]), phase, &abort_flag);
           if (!ok) break;
           tc_fence_after();
           if (elected) {
-            const uint64_t wdesc = wdesc0 + (uint64_t)(stage * (stage_bytes >> 4));
-            const uint64_t xdesc = xdesc0 + (uint64_t)(stage * (stage_bytes >> 4));
+            const int blocks = min(depth, kb_end - kb);
+            for (int i = 0; i < blocks; ++i) {
+              const uint64_t at = (uint64_t)((depth * group + i) * (block_bytes >> 4));
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              tc2_mma_int8(tmem_base + acc * 256, wdesc + (uint64_t)(2 * k), xdesc + (uint64_t)(2 * k), idesc, (uint32_t)(kb != kb_first || k != 0));
-            if (stage & 1) tc2_commit_to(smem_u32(&bar_empty[stage >> 1]), pair_mask);
-            if (kb == kb_end - 1) tc2_commit_to(smem_u32(&bar_tmem_full[acc]), pair_mask);
+              for (int k = 0; k < 4; ++k)
+                tc2_mma_int8(tmem_base + acc * 256, wdesc0 + at + (uint64_t)(2 * k), xdesc0 + at + (uint64_t)(2 * k), idesc,
+                             (uint32_t)(kb + i != kb_first || k != 0));
+            }
+            tc2_commit_to(smem_u32(&bar_empty[group]), pair_mask);
+            if (kb + depth >= kb_end) tc2_commit_to(smem_u32(&bar_tmem_full[acc]), pair_mask);
           }
           __syncwarp();
-          if (++stage == stages) { stage = 0; phase ^= 1u; }
+          if (++group == groups) { group = 0; phase ^= 1u; }
         }
         acc ^= 1;
         if (acc == 0) acc_phase ^= 1u;
       }
-      if (ok && (stage & 1) && elected) tc2_commit_to(smem_u32(&bar_empty[stage >> 1]), pair_mask);   // a group that is half used
       if (!ok && lane == 0) {
         abort_flag = 1;
         atomicMax(p.status, (int)kStatusMmaTimeout);
@@ -339,9 +357,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     const float* sb = after_wait(p.sb);
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int64_t id = first_id; id < total; id += n_workers) {
-      int b, m0, width;
-      int64_t row0, row_end;
+    for (int id = first_id; id < total; id += n_workers) {
+      int b, m0, row0, row_end, width;
       decode(id, b, m0, row0, row_end, width);
       const int col = m0 + (int)rank * 128 + q * 32;
       const bool mine = col < p.N;
@@ -355,7 +372,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
       const float* sa_b = sa + (GROUPED ? 0 : b * p.sa_b);
       T* out = p.out + (GROUPED ? 0 : (int64_t)b * p.M * p.N);
       auto row_scale = [&](int c) {
-        const int64_t row = row0 + c * 32 + lane;
+        const int row = row0 + c * 32 + lane;
         return row < row_end ? sa_b[row * p.sa_m] : 0.f;
       };
       float sa_next = row_scale(turn);         // a chunk ahead
@@ -400,7 +417,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
                 for (int j = 0; j < 4; ++j) v[4 * i + j] += x[j];
               }
             }
-            int8_store(p, out, wide, row_scale(c), scale, col, row0 + c * 32, (int)min((int64_t)32, row_end - row0 - c * 32), lane, park, v);
+            int8_store(p, out, wide, row_scale(c), scale, col, row0 + c * 32, min(32, row_end - row0 - c * 32), lane, park, v);
           }
         }
         break;
@@ -414,7 +431,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
           sa_next = row_scale(c + 2);
           uint32_t v[32];
           int8_load_sums(wide, t_row + c * 32, v);
-          int8_store(p, out, wide, sa_lane, scale, col, row0 + c * 32, (int)min((int64_t)32, row_end - row0 - c * 32), lane, park, v);
+          int8_store(p, out, wide, sa_lane, scale, col, row0 + c * 32, min(32, row_end - row0 - c * 32), lane, park, v);
         }
       }
       tc_fence_before();
@@ -634,9 +651,9 @@ inline int int8_resident(int cluster, int smem) {
 }
 
 // Tiles of a product that is not grouped: the least of the estimated clocks, fitted to 130 measurements of 15 products at all widths and splits
-// (5 % off on average; what it picks is within 4 % of the best, but for 700 x 700 x 700, 6.6 instead of 6.0 us).  A k-block takes what its copies
-// take, some 430 at any width, or its instructions, 2 per row and a tenth; a tile 1400 besides; the last tile's epilogue 28 per row,
-// shared out where a cluster shares the tile, for which it meets twice and moves sums.
+// (6 % off on average; what it picks is within 2 % of the best, but for 700 x 700 x 700, 6.5 instead of 5.8 us).  A k-block takes some 370 at
+// any width that its copies bound, or its instructions, 2 per row and a tenth; a tile 1400 besides; the last tile's epilogue 28 per
+// row, shared out where a cluster shares the tile, for which it meets twice and moves sums.
 struct Int8Choice { int width, splits; };
 template <auto kern>
 inline Int8Choice int8_choose(int64_t B, int64_t M, int64_t N, int64_t K, int smem) {
@@ -650,7 +667,7 @@ inline Int8Choice int8_choose(int64_t B, int64_t M, int64_t N, int64_t K, int sm
     for (int s = 1; s <= kInt8MaxSplits && s <= kb; ++s) {
       const int64_t tiles = B * MT * NT, room = std::max(1, int8_resident<kern>(2 * s, smem));
       if (s > 1 && tiles > room) break;                            // a cluster has one tile
-      const double t = (double)ceil_div(tiles, room) * ((double)ceil_div(kb, s) * std::max(430.0, 2.2 * width) + 1400) + 28.0 * width / s +
+      const double t = (double)ceil_div(tiles, room) * ((double)ceil_div(kb, s) * std::max(370.0, 2.2 * width) + 1400) + 28.0 * width / s +
                        (s > 1 ? 2900 + 31 * width : 0);
       if (t < least) { least = t; best = Int8Choice{width, s}; }
     }
@@ -670,22 +687,26 @@ inline int launch_int8_pair(const Int8Operand& X, const Int8Operand& W, Int8Para
   const int pairs = int8_resident<kern>(2, most);
   if (pairs <= 0) return YAMOE_ERR_CUDA;
   if constexpr (GROUPED) {
-    // Narrow tiles, and with them more stages, where experts have few rows (mean rows per expert, us with tiles of 64 / 128 / 256: 0.5
+    // Narrow tiles, and with them more k-blocks on their way, where experts have few rows (mean rows per expert, us with tiles of 64 / 128 / 256: 0.5
     // 5760 x 2880 93 / 96 / 101; 16 84 / 82 / 87; 64 112 / 95 / 93; 128 161 / 121 / 109).
     p.width = p.M <= 8 * (int64_t)p.B ? 64 : p.M <= 32 * (int64_t)p.B ? 128 : 256;
     p.splits = 1;
-    p.stages = int8_stages(p.width);
-    p.stage_bytes = int8_stage_bytes(p.width);
+    p.groups = int8_groups(p.width);
+    p.depth = int8_depth(p.width);
+    p.block_bytes = int8_block_bytes(p.width);
     const int64_t tiles = (ceil_div(p.M, p.width) + std::min<int64_t>(p.B, p.M)) * p.NT;       // at most
+    if (tiles >= (int64_t)1 << 30) return YAMOE_ERR_UNSUPPORTED;
     return launch_clusters(kern, 2, true, dim3((unsigned)(2 * std::min<int64_t>(tiles, pairs))), dim3(kInt8Threads), smem, st, tmW, tmX, tmXs, p);
   } else {
     const Int8Choice c = int8_choose<kern>(p.B, p.M, p.N, p.K, most);
     p.width = c.width;
     p.splits = c.splits;
-    p.stages = int8_stages(p.width);
-    p.stage_bytes = int8_stage_bytes(p.width);
+    p.groups = int8_groups(p.width);
+    p.depth = int8_depth(p.width);
+    p.block_bytes = int8_block_bytes(p.width);
     p.MT = (int)ceil_div(p.M, c.width);
     const int64_t tiles = (int64_t)p.B * p.MT * p.NT;
+    if (tiles >= (int64_t)1 << 30) return YAMOE_ERR_UNSUPPORTED;
     const int64_t grid = c.splits > 1 ? 2 * c.splits * tiles : 2 * std::min<int64_t>(tiles, pairs);
     return launch_clusters(kern, 2 * c.splits, true, dim3((unsigned)grid), dim3(kInt8Threads), smem, st, tmW, tmX, tmXs, p);
   }
