@@ -15,13 +15,57 @@
 
 namespace yb {
 
+// 1 / (1 + exp(-1.702 g)) as IEEE has it
+__device__ __forceinline__ float glu_sigmoid(float g) { return __fdiv_rn(1.f, 1.f + expf(-kAlpha * g)); }
+// Two of them by the approximate forms
+__device__ __forceinline__ uint64_t glu_sigmoid_f32x2(uint64_t g) {
+  constexpr float kLog2 = -kAlpha * 1.4426950408889634f;             // exp(x) = 2^(x log2 e)
+  float x, y;
+  unpack_f32x2(mul_f32x2(g, pack_f32x2(kLog2, kLog2)), x, y);
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(y));
+  unpack_f32x2(add_f32x2(pack_f32x2(x, y), pack_f32x2(1.f, 1.f)), x, y);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(y));
+  return pack_f32x2(x, y);
+}
+
+// The GLU of two gate / up pairs
 template <typename T>
-__device__ __forceinline__ float glu_sigmoid(float g) {
-  if constexpr (sizeof(T) == 4) return __fdiv_rn(1.f, 1.f + expf(-kAlpha * g));
-  float e, s;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * (-kAlpha * 1.4426950408889634f)));      // exp(x) = 2^(x log2 e)
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
-  return s;
+__device__ __forceinline__ void glu_two(const float (&gate)[2], const float (&up)[2], float (&y)[2]) {
+  const float g[2] = {clamp_gate(gate[0]), clamp_gate(gate[1])}, u[2] = {clamp_up(up[0]), clamp_up(up[1])};
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y[i] = (u[i] + 1.f) * (g[i] * glu_sigmoid(g[i]));
+  } else {
+    const uint64_t gg = pack_f32x2(g[0], g[1]), v = add_f32x2(pack_f32x2(u[0], u[1]), pack_f32x2(1.f, 1.f));
+    unpack_f32x2(mul_f32x2(v, mul_f32x2(gg, glu_sigmoid_f32x2(gg))), y[0], y[1]);
+  }
+}
+// Its gradients, d those of the results
+template <typename T>
+__device__ __forceinline__ void glu_two_backward(const float (&gate)[2], const float (&up)[2], const float (&d)[2], float (&d_gate)[2],
+                                                 float (&d_up)[2]) {
+  const float g[2] = {clamp_gate(gate[0]), clamp_gate(gate[1])}, u[2] = {clamp_up(up[0]), clamp_up(up[1])};
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float s = glu_sigmoid(g[i]), y = g[i] * s;
+      d_gate[i] = d[i] * (u[i] + 1.f) * (s + kAlpha * y * (1.f - s));
+      d_up[i] = d[i] * y;
+    }
+  } else {
+    const uint64_t one = pack_f32x2(1.f, 1.f), gg = pack_f32x2(g[0], g[1]), s = glu_sigmoid_f32x2(gg), y = mul_f32x2(gg, s),
+                   dd = pack_f32x2(d[0], d[1]), v = add_f32x2(pack_f32x2(u[0], u[1]), one);
+    const uint64_t rest = fma_f32x2(s, pack_f32x2(-1.f, -1.f), one), slope = fma_f32x2(mul_f32x2(y, rest), pack_f32x2(kAlpha, kAlpha), s);
+    unpack_f32x2(mul_f32x2(mul_f32x2(dd, v), slope), d_gate[0], d_gate[1]);
+    unpack_f32x2(mul_f32x2(dd, y), d_up[0], d_up[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (gate[i] > kLimit) d_gate[i] = 0.f;
+    if (fabsf(up[i]) > kLimit) d_up[i] = 0.f;
+  }
 }
 
 struct GluSaved {
@@ -106,9 +150,12 @@ glu_forward_kernel(const T* pre, T* out, const GluSaved saved, int64_t M, int W)
     if constexpr (SAVE) *reinterpret_cast<uint2*>(saved.q + row * saved.ld + k) = fp8_codes(v[i], f);
     float y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float g = clamp_gate(v[i].value(2 * j)), u = clamp_up(v[i].value(2 * j + 1));
-      y[j] = (u + 1.f) * (g * glu_sigmoid<T>(g));
+    for (int j = 0; j < 4; j += 2) {
+      const float gate[2] = {v[i].value(2 * j), v[i].value(2 * j + 2)}, up[2] = {v[i].value(2 * j + 1), v[i].value(2 * j + 3)};
+      float two[2];
+      glu_two<T>(gate, up, two);
+      y[j] = two[0];
+      y[j + 1] = two[1];
     }
     put_four<T, VEC>(dst + k / 2, y, (W - k) / 2);
   }
@@ -157,14 +204,21 @@ glu_backward_kernel(const T* dy, const uint8_t* q, const float* scale, int64_t l
     if (k >= W) break;
     float out[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float gate, up;
-      e4m3x2_values((j < 2 ? code[i].x : code[i].y) >> (16 * (j & 1)), gate, up);
-      gate *= s[i];
-      up *= s[i];
-      const float g = clamp_gate(gate), u = clamp_up(up), sig = glu_sigmoid<T>(g), y = g * sig;
-      out[2 * j] = gate > kLimit ? 0.f : d[i][j] * (u + 1.f) * (sig + kAlpha * y * (1.f - sig));
-      out[2 * j + 1] = fabsf(up) > kLimit ? 0.f : d[i][j] * y;
+    for (int j = 0; j < 4; j += 2) {
+      float gate[2], up[2], d_gate[2], d_up[2];
+      const uint32_t word = j < 2 ? code[i].x : code[i].y;
+      e4m3x2_values(word, gate[0], up[0]);
+      e4m3x2_values(word >> 16, gate[1], up[1]);
+      const uint64_t scale = pack_f32x2(s[i], s[i]);
+      unpack_f32x2(mul_f32x2(pack_f32x2(gate[0], up[0]), scale), gate[0], up[0]);
+      unpack_f32x2(mul_f32x2(pack_f32x2(gate[1], up[1]), scale), gate[1], up[1]);
+      const float two[2] = {d[i][j], d[i][j + 1]};
+      glu_two_backward<T>(gate, up, two, d_gate, d_up);
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        out[2 * (j + o)] = d_gate[o];
+        out[2 * (j + o) + 1] = d_up[o];
+      }
     }
     if constexpr (VEC) {
       if constexpr (sizeof(T) == 2) {
