@@ -28,13 +28,14 @@
 namespace yb {
 
 // A k-block: this CTA's 128 rows of weights and half of the tile's rows of tokens in boxes of 32, 128 bytes each.  Blocks come, are multiplied and
-// are given back in groups: two at a time, which spares the warps every other wait (64 x 5760 x 2880: one at a time 9.3 us, two 8.3), but for
-// the widest tiles, whose instructions take longer than the waits and of which the ring holds three groups of two (8192 x 5760 x 2880: 88, 93).
+// are given back in groups: two at a time, which spares the warps every other wait (64 x 5760 x 2880: one at a time 9.3 us, two 8.3; 2048 rows of
+// 32 experts 109, 107), but for the widest tiles of products that are not grouped, whose instructions take longer than the waits and of which
+// the ring holds three groups of two (8192 x 5760 x 2880: 88, 93).
 constexpr int int8_block_bytes(int width) { return 128 * 128 + (width + 63) / 64 * 4096; }
-constexpr int int8_depth(int width) { return width > 192 ? 1 : 2; }
+constexpr int int8_depth(int width, bool grouped) { return width > 192 && !grouped ? 1 : 2; }
 constexpr int kInt8Ring = 10 * int8_block_bytes(64), kInt8MaxGroups = 6;
-constexpr int int8_groups(int width) { return kInt8Ring / (int8_depth(width) * int8_block_bytes(width)); }
-static_assert(int8_groups(32) == 5 && int8_groups(128) == 4 && int8_groups(192) == 3 && int8_groups(256) == kInt8MaxGroups, "");
+constexpr int int8_groups(int width, int depth) { return kInt8Ring / (depth * int8_block_bytes(width)); }
+static_assert(int8_groups(32, 2) == 5 && int8_groups(128, 2) == 4 && int8_groups(192, 2) == 3 && int8_groups(256, 1) == kInt8MaxGroups, "");
 constexpr int kInt8EpiWarps = 8, kInt8Threads = 32 * (3 + kInt8EpiWarps);
 constexpr int kInt8ParkBytes = 32 * 64;                  // 32 rows of an epilogue warp's 32 columns on their way out
 constexpr int kInt8RingBytes = kInt8Ring + 1024;         // + slack for 1024-byte alignment
@@ -691,8 +692,8 @@ inline int launch_int8_pair(const Int8Operand& X, const Int8Operand& W, Int8Para
     // 5760 x 2880 93 / 96 / 101; 16 84 / 82 / 87; 64 112 / 95 / 93; 128 161 / 121 / 109).
     p.width = p.M <= 8 * (int64_t)p.B ? 64 : p.M <= 32 * (int64_t)p.B ? 128 : 256;
     p.splits = 1;
-    p.groups = int8_groups(p.width);
-    p.depth = int8_depth(p.width);
+    p.depth = int8_depth(p.width, GROUPED);
+    p.groups = int8_groups(p.width, p.depth);
     p.block_bytes = int8_block_bytes(p.width);
     const int64_t tiles = (ceil_div(p.M, p.width) + std::min<int64_t>(p.B, p.M)) * p.NT;       // at most
     if (tiles >= (int64_t)1 << 30) return YAMOE_ERR_UNSUPPORTED;
@@ -701,8 +702,8 @@ inline int launch_int8_pair(const Int8Operand& X, const Int8Operand& W, Int8Para
     const Int8Choice c = int8_choose<kern>(p.B, p.M, p.N, p.K, most);
     p.width = c.width;
     p.splits = c.splits;
-    p.groups = int8_groups(p.width);
-    p.depth = int8_depth(p.width);
+    p.depth = int8_depth(p.width, GROUPED);
+    p.groups = int8_groups(p.width, p.depth);
     p.block_bytes = int8_block_bytes(p.width);
     p.MT = (int)ceil_div(p.M, c.width);
     const int64_t tiles = (int64_t)p.B * p.MT * p.NT;
