@@ -494,12 +494,12 @@ link_rows_kernel(const int32_t* row_of, int64_t S, int64_t n_rows, int32_t* head
 }
 
 // From the tokens' side, so that d_out is read once: `wpt` warps (1, 2, 4 or 8) share a token, write the rows that only it has and add up
-// the products with all its rows, each warp its pieces, the warps in order.  The CTAs behind `token_ctas` look for the other rows: those
+// the products with all its rows, each warp its pieces, the warps in order.  The first `row_ctas` CTAs look for the other rows: those
 // of no assignment become zero, those of several the sum over them (in the order of their list, which is not fixed beyond two).
 template <typename T, typename TW, int VE, int KB>
 __global__ void __launch_bounds__(kCopyWarps * 32)
 combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_weights, const int32_t* head, const int32_t* next,
-                        int wpt, unsigned token_ctas) {
+                        int wpt, unsigned row_ctas) {
   extern __shared__ float s_dot[];              // [warps][K]
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const unsigned pieces = (unsigned)a.H / VE;
@@ -509,11 +509,11 @@ combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_w
   d_out = after_wait(d_out);
   head = after_wait(head);
   next = after_wait(next);
-  if (blockIdx.x >= token_ctas) {
-    const int64_t first = ((int64_t)(blockIdx.x - token_ctas) * kCopyWarps + w) * 32;
+  if (blockIdx.x < row_ctas) {
+    const int64_t first = ((int64_t)blockIdx.x * kCopyWarps + w) * kZeroRows;
     int h = -1;
     bool mine = false;
-    if (first + lane < a.n_rows) {
+    if (lane < kZeroRows && first + lane < a.n_rows) {
       h = head[first + lane];
       mine = h < 0 || next[h] >= 0;
     }
@@ -538,7 +538,7 @@ combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_w
     }
     return;
   }
-  const int64_t t = (int64_t)blockIdx.x * (kCopyWarps / wpt) + w / wpt;
+  const int64_t t = (int64_t)(blockIdx.x - row_ctas) * (kCopyWarps / wpt) + w / wpt;
   const int part = w % wpt;
   for (int k0 = 0; k0 < a.K && t < a.Tn; k0 += KB) {
     int r[KB];
@@ -620,7 +620,7 @@ inline int launch_combine_backward_ve(const CombineArgs<T, TW>& a, const T* d_ou
   // at least 32 warps per SM, while each has pieces of the token
   int wpt = 1;
   while (wpt < kCopyWarps && a.Tn * wpt < kSMs * 32 && a.H / VE > 32 * wpt) wpt *= 2;
-  const int64_t S = a.Tn * a.K, token = ceil_div(a.Tn * wpt, kCopyWarps), row = d_rows != nullptr ? ceil_div(a.n_rows, kCopyWarps * 32) : 0;
+  const int64_t S = a.Tn * a.K, token = ceil_div(a.Tn * wpt, kCopyWarps), row = d_rows != nullptr ? ceil_div(a.n_rows, kCopyWarps * kZeroRows) : 0;
   if (token + row > 0x7fffffff || ceil_div(S, 256) > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
   if (d_rows != nullptr && a.n_rows > 0) {
     YB_CUDA_OK(cudaMemsetAsync(head, 0xFF, (size_t)a.n_rows * sizeof(int32_t), st));
@@ -631,7 +631,7 @@ inline int launch_combine_backward_ve(const CombineArgs<T, TW>& a, const T* d_ou
   if (token + row == 0) return YAMOE_OK;
   auto kern = a.K <= 4 ? combine_backward_kernel<T, TW, VE, 4> : combine_backward_kernel<T, TW, VE, 8>;
   return launch_behind(kern, dim3((unsigned)(token + row)), dim3(kCopyWarps * 32), kCopyWarps * a.K * sizeof(float), st, a, d_out, d_rows,
-                       d_weights, (const int32_t*)head, (const int32_t*)next, wpt, (unsigned)token);
+                       d_weights, (const int32_t*)head, (const int32_t*)next, wpt, (unsigned)row);
 }
 
 inline bool pieces_of_16_bytes(int64_t row_bytes, std::initializer_list<const void*> at) {
