@@ -44,8 +44,10 @@ template <typename T, typename TW>
 static int combine_impl(const CombineCall& c, void* out, cudaStream_t st) {
   const auto a = c.args<T, TW>();
   T* o = reinterpret_cast<T*>(out);
-  return pieces_of_16_bytes(c.H * sizeof(T), {c.rows, out}) ? launch_combine_tokens_ve<T, TW, 16 / sizeof(T)>(a, o, st)
-                                                            : launch_combine_tokens_ve<T, TW, 1>(a, o, st);
+  if (pieces_of(16, c.H * sizeof(T), {c.rows, out})) return launch_combine_tokens_ve<T, TW, 16 / sizeof(T)>(a, o, st);
+  if constexpr (sizeof(T) == 2)
+    if (pieces_of(4, c.H * sizeof(T), {c.rows, out})) return launch_combine_tokens_ve<T, TW, 2>(a, o, st);
+  return launch_combine_tokens_ve<T, TW, 1>(a, o, st);
 }
 template <typename T, typename TW>
 static int combine_backward_impl(const CombineCall& c, const void* d_out, void* d_rows, void* d_weights, int32_t* head, int32_t* next,
@@ -54,9 +56,11 @@ static int combine_backward_impl(const CombineCall& c, const void* d_out, void* 
   const T* g = reinterpret_cast<const T*>(d_out);
   T* dr = reinterpret_cast<T*>(d_rows);
   TW* dw = reinterpret_cast<TW*>(d_weights);
-  return pieces_of_16_bytes(c.H * sizeof(T), {c.rows, d_out, d_rows})
-             ? launch_combine_backward_ve<T, TW, 16 / sizeof(T)>(a, g, dr, dw, head, next, st)
-             : launch_combine_backward_ve<T, TW, 1>(a, g, dr, dw, head, next, st);
+  if (pieces_of(16, c.H * sizeof(T), {c.rows, d_out, d_rows}))
+    return launch_combine_backward_ve<T, TW, 16 / sizeof(T)>(a, g, dr, dw, head, next, st);
+  if constexpr (sizeof(T) == 2)
+    if (pieces_of(4, c.H * sizeof(T), {c.rows, d_out, d_rows})) return launch_combine_backward_ve<T, TW, 2>(a, g, dr, dw, head, next, st);
+  return launch_combine_backward_ve<T, TW, 1>(a, g, dr, dw, head, next, st);
 }
 
 // the arguments that both have
