@@ -87,6 +87,7 @@ struct SortTokens : torch::autograd::Function<SortTokens> {
     const at::AutoDispatchBelowADInplaceOrView below;
     const Sorted s = sort_tokens(hidden_states, router_indices, num_experts, expert_capacity);
     ctx->mark_non_differentiable({s.row_of, s.offsets});
+    ctx->set_materialize_grads(false);                 // (zeros for the integers would be two launches)
     ctx->save_for_backward({s.row_of});
     return {s.rows, s.row_of, s.offsets};
   }
