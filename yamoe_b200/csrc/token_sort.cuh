@@ -388,9 +388,6 @@ struct CombineArgs {
     const int r = row_of[p];
     return r >= 0 && r < n_rows ? r : -1;
   }
-  __device__ __forceinline__ int64_t column(int64_t t, int k) const {
-    return indices == nullptr ? k : indices[t * K + k];
-  }
   // weight of slot k of token t; 0 for a column that does not exist
   __device__ __forceinline__ float weight(int64_t t, int k) const {
     if (weights == nullptr) return 1.f;
