@@ -416,8 +416,8 @@ int yamoe_b200_combine_tokens(const void *rows, int64_t n_rows, const int32_t *r
                               int K, int dtype, void *stream);
 
 /* Its gradients; either output may be NULL (d_weights: has to be without weights).
- *   d_rows[r,:] = sum of w[p] d_out[t(p),:] over the assignments p with row_of[p] = r, zero without any.  A row of several is summed in
- *   an order that is not fixed beyond two; the rows of yamoe_b200_sort_tokens have one at most.
+ *   d_rows[r,:] = sum of w[p] d_out[t(p),:] over the assignments p with row_of[p] = r in the order of p, zero without any.  The rows
+ *   of yamoe_b200_sort_tokens have one at most; one that more than 32 name costs a pass over row_of.
  *   d_weights   like weights: <d_out[t], rows[row_of[t*K+k]]>, 0 where there is no row; with router_indices the sum over the slots of
  *   a column, 0 for those of none.  K <= 1024. */
 size_t yamoe_b200_combine_tokens_backward_workspace_bytes(int64_t n_rows, int64_t T, int K);

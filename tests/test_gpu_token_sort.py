@@ -223,6 +223,46 @@ def test_rows_that_several_assignments_share():
     check_sum(d_w, products.sum(2), products.abs().sum(2), H + 16, "d_weights")
 
 
+@pytest.mark.parametrize("dense", [False, True])
+@pytest.mark.parametrize("H", [8, 33, 520])
+def test_rows_that_many_share_are_summed_in_order(H, dense):
+    """Weights of 24 bits: a product is rounded where it starts a sum and not where it joins one, so that the order of two shows already."""
+    from yamoe_b200 import combine_tokens
+    T, K, E = 600, 2, 5
+    row_of = torch.full((T * K,), -1, dtype=torch.int32)
+    named = {0: 1, 1: 2, 2: 3, 3: 31, 4: 32, 5: 33, 6: 300, 9: 64, 11: 2}          # rows 7, 8 and 10: nobody's
+    free = torch.randperm(T * K, generator=torch.Generator().manual_seed(0))
+    at = 0
+    for r, n in named.items():
+        row_of[free[at:at + n]] = r
+        at += n
+    row_of = row_of.view(T, K)
+    idx = torch.randint(0, E, (T, K), generator=torch.Generator().manual_seed(1))
+    w = randn(T, E if dense else K, seed=2)
+    d = randn(T, H, seed=3)
+    rows = torch.zeros(12, H, device="cuda", requires_grad=True)
+    out = combine_tokens(rows, row_of.cuda(), w.cuda(), idx.cuda() if dense else None)
+    grads = [torch.autograd.grad(out, rows, d.cuda(), retain_graph=True)[0].cpu() for _ in range(10)]
+    for g in grads[1:]:
+        assert torch.equal(g, grads[0])
+    each = (w.gather(1, idx) if dense else w).double()
+    for r in range(12):
+        t, k = torch.nonzero(row_of == r, as_tuple=True)          # in the order of the assignments
+        want, mag = torch.zeros(H, dtype=torch.float64), torch.zeros(H, dtype=torch.float64)
+        for i, j in zip(t.tolist(), k.tolist()):
+            want += each[i, j] * d[i].double()
+            mag += (each[i, j] * d[i].double()).abs()
+        check_sum(grads[0][r], want, mag, max(1, len(t)), f"row {r}")
+    # 2^24 + 1 + 1 ... - 2^24: each one is lost to ties, in the order of the assignments; any that came after -2^24 or before 2^24 would show
+    for n in (4, 40):
+        of = torch.zeros(n, 1, dtype=torch.int32)
+        d = torch.ones(n, H)
+        d[0], d[-1] = 2.0 ** 24, -2.0 ** 24
+        rows = torch.zeros(1, H, device="cuda", requires_grad=True)
+        (g,) = torch.autograd.grad(combine_tokens(rows, of.cuda()), rows, d.cuda())
+        assert not g.any()
+
+
 def test_dropped_rows_do_not_spread_what_they_hold():
     """NaN and infinities in rows that nobody owns, and a weight of zero: as the formula has it."""
     import yamoe_b200

@@ -505,7 +505,8 @@ link_rows_kernel(const int32_t* row_of, int64_t S, int64_t n_rows, int32_t* head
 
 // From the tokens' side, so that d_out is read once: `wpt` warps (1, 2, 4 or 8) share a token, write the rows that only it has and add up
 // the products with all its rows, each warp its pieces, the warps in order.  The first `row_ctas` CTAs look for the other rows: those
-// of no assignment become zero, those of several the sum over them (in the order of their list, which is not fixed beyond two).
+// of no assignment become zero, those of several the sum over them.  Atomics made the lists, so their order is not that of the
+// assignments; the sum is: up to 32 of a row are ranked by the warp, for more it goes through row_of.
 template <typename T, typename TW, int VE, int KB>
 __global__ void __launch_bounds__(kCopyWarps * 32)
 combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_weights, const int32_t* head, const int32_t* next,
@@ -529,21 +530,39 @@ combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_w
     }
     for (unsigned todo = __ballot_sync(0xffffffffu, mine); todo != 0; todo &= todo - 1) {
       const int l = __ffs(todo) - 1, p0 = __shfl_sync(0xffffffffu, h, l);
-      for (unsigned i = lane; i < pieces; i += 32) {
+      int n = 0, held = 0, place = 0;           // assignments of the row, lane's one, its place among them
+      for (int p = p0; p >= 0 && n <= 32; p = next[p]) held = n++ == lane ? p : held;
+      for (int k = 0; k < min(n, 32); ++k) place += __shfl_sync(0xffffffffu, held, k) < held;
+      const int64_t of = held / a.K;
+      const float weight = lane < n ? a.weight(of, (int)(held - of * a.K)) : 0.f;
+      for (unsigned i0 = 0; i0 < pieces; i0 += 32) {
+        const unsigned i = i0 + lane;
         float acc[VE];
 #pragma unroll
         for (int j = 0; j < VE; ++j) acc[j] = 0.f;
-        for (int p = p0; p >= 0; p = next[p]) {
-          const int64_t t = p / a.K;
-          const float wgt = a.weight(t, (int)(p - t * a.K));
+        const auto add = [&](int64_t t, float wgt) {
+          if (i >= pieces) return;
           Piece<T, VE> q;
           q.load(d_out + t * a.H + i * VE);
           float v[VE];
           q.get(v);
 #pragma unroll
           for (int j = 0; j < VE; ++j) acc[j] = fmaf(wgt, v[j], acc[j]);
+        };
+        if (n <= 32) {
+          for (int k = 0; k < n; ++k) {
+            const int from = __ffs(__ballot_sync(0xffffffffu, lane < n && place == k)) - 1;
+            add(__shfl_sync(0xffffffffu, (int)of, from), __shfl_sync(0xffffffffu, weight, from));
+          }
+        } else {
+          const int64_t S = a.Tn * a.K;
+          for (int64_t s = 0; s < S; s += 32)
+            for (unsigned hit = __ballot_sync(0xffffffffu, s + lane < S && a.row_of[s + lane] == first + l); hit != 0; hit &= hit - 1) {
+              const int64_t p = s + (__ffs(hit) - 1), t = p / a.K;
+              add(t, a.weight(t, (int)(p - t * a.K)));
+            }
         }
-        Piece<T, VE>::put(d_rows + (first + l) * a.H + i * VE, acc);
+        if (i < pieces) Piece<T, VE>::put(d_rows + (first + l) * a.H + i * VE, acc);
       }
     }
     return;
