@@ -507,10 +507,14 @@ link_rows_kernel(const int32_t* row_of, int64_t S, int64_t n_rows, int32_t* head
 // the products with all its rows, each warp its pieces, the warps in order.  The first `row_ctas` CTAs look for the other rows: those
 // of no assignment become zero, those of several the sum over them.  Atomics made the lists, so their order is not that of the
 // assignments; the sum is: up to 32 of a row are ranked by the warp, for more it goes through row_of.
-template <typename T, typename TW, int VE, int KB>
+//
+// The rows of four slots are on their way together, of more one four after the other, with d_out from L1 or L2 again: eight at once leave too few warps to an SM
+// (8192 tokens of 2880, 8 rows each: 143 / 155 us; 32 tokens 10.3 / 9.7).
+template <typename T, typename TW, int VE>
 __global__ void __launch_bounds__(kCopyWarps * 32)
 combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_weights, const int32_t* head, const int32_t* next,
                         int wpt, unsigned row_ctas) {
+  constexpr int KB = 4;
   extern __shared__ float s_dot[];              // [warps][K]
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const unsigned pieces = (unsigned)a.H / VE;
@@ -658,7 +662,7 @@ inline int launch_combine_backward_ve(const CombineArgs<T, TW>& a, const T* d_ou
     if (rc) return rc;
   }
   if (token + row == 0) return YAMOE_OK;
-  auto kern = a.K <= 4 ? combine_backward_kernel<T, TW, VE, 4> : combine_backward_kernel<T, TW, VE, 8>;
+  auto kern = combine_backward_kernel<T, TW, VE>;
   return launch_behind(kern, dim3((unsigned)(token + row)), dim3(kCopyWarps * 32), kCopyWarps * a.K * sizeof(float), st, a, d_out, d_rows,
                        d_weights, (const int32_t*)head, (const int32_t*)next, wpt, (unsigned)row);
 }
