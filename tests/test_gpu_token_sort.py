@@ -225,12 +225,13 @@ def test_rows_that_several_assignments_share():
 
 @pytest.mark.parametrize("dense", [False, True])
 @pytest.mark.parametrize("H", [8, 33, 520])
-def test_rows_that_many_share_are_summed_in_order(H, dense):
+@pytest.mark.parametrize("R", [12, 200, 1300])
+def test_rows_that_many_share_are_summed_in_order(R, H, dense):
     """Weights of 24 bits: a product is rounded where it starts a sum and not where it joins one, so that the order of two shows already."""
     from yamoe_b200 import combine_tokens
-    T, K, E = 600, 2, 5
+    T, K, E = 1400, 2, 5
     row_of = torch.full((T * K,), -1, dtype=torch.int32)
-    named = {0: 1, 1: 2, 2: 3, 3: 31, 4: 32, 5: 33, 6: 300, 9: 64, 11: 2}          # rows 7, 8 and 10: nobody's
+    named = {0: 1, 1: 2, 2: 3, 3: 31, 4: 32, 5: 33, 6: 300, 9: 255, 10: 256, 11: 257, R - 1: 700}          # the others: nobody's
     free = torch.randperm(T * K, generator=torch.Generator().manual_seed(0))
     at = 0
     for r, n in named.items():
@@ -240,13 +241,14 @@ def test_rows_that_many_share_are_summed_in_order(H, dense):
     idx = torch.randint(0, E, (T, K), generator=torch.Generator().manual_seed(1))
     w = randn(T, E if dense else K, seed=2)
     d = randn(T, H, seed=3)
-    rows = torch.zeros(12, H, device="cuda", requires_grad=True)
+    rows = torch.zeros(R, H, device="cuda", requires_grad=True)
     out = combine_tokens(rows, row_of.cuda(), w.cuda(), idx.cuda() if dense else None)
     grads = [torch.autograd.grad(out, rows, d.cuda(), retain_graph=True)[0].cpu() for _ in range(10)]
     for g in grads[1:]:
         assert torch.equal(g, grads[0])
     each = (w.gather(1, idx) if dense else w).double()
-    for r in range(12):
+    assert not grads[0][torch.tensor([r not in named for r in range(R)])].any()
+    for r in named:
         t, k = torch.nonzero(row_of == r, as_tuple=True)          # in the order of the assignments
         want, mag = torch.zeros(H, dtype=torch.float64), torch.zeros(H, dtype=torch.float64)
         for i, j in zip(t.tolist(), k.tolist()):

@@ -503,19 +503,103 @@ link_rows_kernel(const int32_t* row_of, int64_t S, int64_t n_rows, int32_t* head
   if (r >= 0 && r < n_rows) next[p] = atomicExch(head + r, (int32_t)p);
 }
 
+// The gradient of a row that several assignments name, by one warp, for 32 pieces from i0 on of every `step`.  Atomics made the links of its assignments,
+// so their order is not that of the assignments; the sum's is.  Up to 32 links are ranked; for more the warp goes through row_of, once while they fit
+// its list, again and again where they do not.
+constexpr int kListed = 256;
+template <typename T, typename TW, int VE>
+__device__ __forceinline__ void sum_shared_row(const CombineArgs<T, TW>& a, const T* d_out, T* d_rows, const int32_t* next, int64_t row, int p0,
+                                            unsigned i0, unsigned step, int32_t* list) {
+  const int lane = threadIdx.x & 31;
+  const unsigned pieces = (unsigned)a.H / VE;
+  const int64_t S = a.Tn * a.K;
+  // assignments from s on into the list, at most kListed, 128 looked at together; s: the first that was not looked at
+  const auto fill = [&](int64_t& s) {
+    int m = 0;
+    __syncwarp();
+    for (; s < S && m <= kListed - 128; s += 128) {
+      int32_t r[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) r[u] = s + 32 * u + lane < S ? a.row_of[s + 32 * u + lane] : -1;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const unsigned hit = __ballot_sync(0xffffffffu, r[u] == row);
+        if (r[u] == row) list[m + __popc(hit & ((1u << lane) - 1u))] = (int32_t)(s + 32 * u + lane);
+        m += __popc(hit);
+      }
+    }
+    __syncwarp();
+    return m;
+  };
+  int n = 0, held = 0;                          // links of the row, lane's one
+  for (int p = p0; p >= 0 && n <= 32; p = next[p]) held = n++ == lane ? p : held;
+  int64_t s = S;                                // what the list does not have begins here
+  if (n <= 32) {
+    int place = 0;
+    for (int k = 0; k < n; ++k) place += __shfl_sync(0xffffffffu, held, k) < held;
+    if (lane < n) list[place] = held;
+    __syncwarp();
+  } else {
+    s = 0;
+    n = fill(s);
+  }
+  const bool whole = s >= S;
+  for (; i0 < pieces; i0 += step) {
+    const unsigned i = i0 + lane;
+    float acc[VE];
+#pragma unroll
+    for (int j = 0; j < VE; ++j) acc[j] = 0.f;
+    if (!whole) {
+      s = 0;
+      n = fill(s);
+    }
+    while (true) {
+      for (int k0 = 0; k0 < n; k0 += 4) {
+        Piece<T, VE> q[4];
+        float wgt[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          q[k].clear();
+          wgt[k] = 0.f;
+          if (k0 + k < n) {
+            const int p = list[k0 + k], t = p / a.K;
+            wgt[k] = a.weight(t, p - t * a.K);
+            if (i < pieces) q[k].load(d_out + (int64_t)t * a.H + i * VE);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float v[VE];
+          q[k].get(v);
+#pragma unroll
+          for (int j = 0; j < VE; ++j) acc[j] = fmaf(wgt[k], v[j], acc[j]);
+        }
+      }
+      if (s >= S) break;
+      n = fill(s);
+    }
+    if (i < pieces) Piece<T, VE>::put(d_rows + row * a.H + i * VE, acc);
+  }
+}
+
 // From the tokens' side, so that d_out is read once: `wpt` warps (1, 2, 4 or 8) share a token, write the rows that only it has and add up
 // the products with all its rows, each warp its pieces, the warps in order.  The first `row_ctas` CTAs look for the other rows: those
-// of no assignment become zero, those of several the sum over them.  Atomics made the lists, so their order is not that of the
-// assignments; the sum is: up to 32 of a row are ranked by the warp, for more it goes through row_of.
+// of no assignment become zero, those of several the sum over them.  A warp looks at eight rows, or at one, or a CTA at one, where that is no more
+// than a CTA per SM: few rows may have many assignments each (8192 tokens of 2880, whose 4 rows each are any of 1000: eight to a warp
+// 1569 us, one 397; any of 149, one to a warp: 1602, any of 148, one to a CTA: 465).
 //
 // The rows of four slots are on their way together, of more one four after the other, with d_out from L1 or L2 again: eight at once leave too few warps to an SM
 // (8192 tokens of 2880, 8 rows each: 143 / 155 us; 32 tokens 10.3 / 9.7).
+struct RowShare {
+  int rows, warps;       // that a warp looks at, that share a row
+  __host__ __device__ explicit RowShare(int64_t n_rows) : rows(n_rows <= kSMs * kCopyWarps ? 1 : kZeroRows), warps(n_rows <= kSMs ? kCopyWarps : 1) {}
+};
 template <typename T, typename TW, int VE>
 __global__ void __launch_bounds__(kCopyWarps * 32)
 combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_weights, const int32_t* head, const int32_t* next,
                         int wpt, unsigned row_ctas) {
   constexpr int KB = 4;
-  extern __shared__ float s_dot[];              // [warps][K]
+  extern __shared__ float s_dot[];              // [warps][K], or a list per warp
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const unsigned pieces = (unsigned)a.H / VE;
   pdl_trigger();
@@ -525,49 +609,24 @@ combine_backward_kernel(CombineArgs<T, TW> a, const T* d_out, T* d_rows, TW* d_w
   head = after_wait(head);
   next = after_wait(next);
   if (blockIdx.x < row_ctas) {
-    const int64_t first = ((int64_t)blockIdx.x * kCopyWarps + w) * kZeroRows;
-    int h = -1;
-    bool mine = false;
-    if (lane < kZeroRows && first + lane < a.n_rows) {
+    const RowShare share(a.n_rows);
+    const unsigned unit = blockIdx.x * kCopyWarps + w, step = 32 * share.warps, i0 = unit % share.warps * 32;
+    const int64_t first = (int64_t)(unit / share.warps) * share.rows;
+    int h = 0;
+    bool nobody = false, shared = false;
+    if (lane < share.rows && first + lane < a.n_rows) {
       h = head[first + lane];
-      mine = h < 0 || next[h] >= 0;
+      nobody = h < 0;
+      shared = h >= 0 && next[h] >= 0;
     }
-    for (unsigned todo = __ballot_sync(0xffffffffu, mine); todo != 0; todo &= todo - 1) {
-      const int l = __ffs(todo) - 1, p0 = __shfl_sync(0xffffffffu, h, l);
-      int n = 0, held = 0, place = 0;           // assignments of the row, lane's one, its place among them
-      for (int p = p0; p >= 0 && n <= 32; p = next[p]) held = n++ == lane ? p : held;
-      for (int k = 0; k < min(n, 32); ++k) place += __shfl_sync(0xffffffffu, held, k) < held;
-      const int64_t of = held / a.K;
-      const float weight = lane < n ? a.weight(of, (int)(held - of * a.K)) : 0.f;
-      for (unsigned i0 = 0; i0 < pieces; i0 += 32) {
-        const unsigned i = i0 + lane;
-        float acc[VE];
-#pragma unroll
-        for (int j = 0; j < VE; ++j) acc[j] = 0.f;
-        const auto add = [&](int64_t t, float wgt) {
-          if (i >= pieces) return;
-          Piece<T, VE> q;
-          q.load(d_out + t * a.H + i * VE);
-          float v[VE];
-          q.get(v);
-#pragma unroll
-          for (int j = 0; j < VE; ++j) acc[j] = fmaf(wgt, v[j], acc[j]);
-        };
-        if (n <= 32) {
-          for (int k = 0; k < n; ++k) {
-            const int from = __ffs(__ballot_sync(0xffffffffu, lane < n && place == k)) - 1;
-            add(__shfl_sync(0xffffffffu, (int)of, from), __shfl_sync(0xffffffffu, weight, from));
-          }
-        } else {
-          const int64_t S = a.Tn * a.K;
-          for (int64_t s = 0; s < S; s += 32)
-            for (unsigned hit = __ballot_sync(0xffffffffu, s + lane < S && a.row_of[s + lane] == first + l); hit != 0; hit &= hit - 1) {
-              const int64_t p = s + (__ffs(hit) - 1), t = p / a.K;
-              add(t, a.weight(t, (int)(p - t * a.K)));
-            }
-        }
-        if (i < pieces) Piece<T, VE>::put(d_rows + (first + l) * a.H + i * VE, acc);
-      }
+    for (unsigned todo = __ballot_sync(0xffffffffu, nobody); todo != 0; todo &= todo - 1) {
+      const float zero[VE] = {};
+      for (unsigned i = i0 + lane; i < pieces; i += step) Piece<T, VE>::put(d_rows + (first + __ffs(todo) - 1) * a.H + i * VE, zero);
+    }
+    for (unsigned todo = __ballot_sync(0xffffffffu, shared); todo != 0; todo &= todo - 1) {
+      const int l = __ffs(todo) - 1;
+      sum_shared_row<T, TW, VE>(a, d_out, d_rows, next, first + l, __shfl_sync(0xffffffffu, h, l), i0, step,
+                                reinterpret_cast<int32_t*>(s_dot) + w * kListed);
     }
     return;
   }
@@ -650,10 +709,11 @@ inline int launch_combine_tokens_ve(const CombineArgs<T, TW>& a, T* out, cudaStr
 template <typename T, typename TW, int VE>
 inline int launch_combine_backward_ve(const CombineArgs<T, TW>& a, const T* d_out, T* d_rows, TW* d_weights, int32_t* head, int32_t* next,
                                       cudaStream_t st) {
+  const RowShare share(a.n_rows);
   // at least 32 warps per SM, while each has pieces of the token
   int wpt = 1;
   while (wpt < kCopyWarps && a.Tn * wpt < kSMs * 32 && a.H / VE > 32 * wpt) wpt *= 2;
-  const int64_t S = a.Tn * a.K, token = ceil_div(a.Tn * wpt, kCopyWarps), row = d_rows != nullptr ? ceil_div(a.n_rows, kCopyWarps * kZeroRows) : 0;
+  const int64_t S = a.Tn * a.K, token = ceil_div(a.Tn * wpt, kCopyWarps), row = d_rows == nullptr ? 0 : ceil_div(a.n_rows * share.warps, kCopyWarps * share.rows);
   if (token + row > 0x7fffffff || ceil_div(S, 256) > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
   if (d_rows != nullptr && a.n_rows > 0) {
     YB_CUDA_OK(cudaMemsetAsync(head, 0xFF, (size_t)a.n_rows * sizeof(int32_t), st));
@@ -663,7 +723,7 @@ inline int launch_combine_backward_ve(const CombineArgs<T, TW>& a, const T* d_ou
   }
   if (token + row == 0) return YAMOE_OK;
   auto kern = combine_backward_kernel<T, TW, VE>;
-  return launch_behind(kern, dim3((unsigned)(token + row)), dim3(kCopyWarps * 32), kCopyWarps * a.K * sizeof(float), st, a, d_out, d_rows,
+  return launch_behind(kern, dim3((unsigned)(token + row)), dim3(kCopyWarps * 32), kCopyWarps * std::max(a.K, kListed) * sizeof(float), st, a, d_out, d_rows,
                        d_weights, (const int32_t*)head, (const int32_t*)next, wpt, (unsigned)row);
 }
 
