@@ -132,9 +132,11 @@ __device__ __forceinline__ void zero_unused(const SortArgs& a, int64_t first, in
 
 // ---- small: everything in one launch ------------------------------------------------------------------------------------
 // CTAs of 32 warps, or of eight where they are enough for the assignments and the experts (16 tokens of 2880, 4 of 128 experts each: 5.3 / 2.5 us).
-inline size_t sort_small_smem(int warps, int S, int E) {
-  return ((size_t)warps * E + E + 1 + S) * sizeof(int32_t);
-}
+constexpr size_t sort_small_smem(int warps, int S, int E) { return ((size_t)warps * E + E + 1 + S) * sizeof(int32_t); }
+// With eight warps it fits what every launch may have, static arrays (a number per warp) included; with 32 a launch has to be allowed more.
+constexpr size_t kAnyLaunchSmem = 48 * 1024;
+constexpr int kSortFewMax = 256 * kSortSmallRounds, kSortFewExperts = 256;      // eight warps: assignments, experts
+static_assert(sort_small_smem(8, kSortFewMax, kSortFewExperts) + 8 * sizeof(int) <= kAnyLaunchSmem, "");
 
 template <typename P, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS)
@@ -217,7 +219,8 @@ sort_count_kernel(SortArgs a) {
   for (int e = threadIdx.x; e < a.E; e += kSortThreads) a.counts[(size_t)blockIdx.x * a.E + e] = smem_i[e];
 }
 
-inline size_t sort_rank_smem(int E) { return ((size_t)kSortWarps * E + 3 * E + 1) * sizeof(int32_t); }
+constexpr size_t sort_rank_smem(int E) { return ((size_t)kSortWarps * E + 3 * E + 1) * sizeof(int32_t); }
+static_assert(sort_rank_smem(kSortMaxExperts) + kSortWarps * sizeof(int) <= kAnyLaunchSmem, "");
 
 __global__ void __launch_bounds__(kSortThreads)
 sort_rank_kernel(SortArgs a) {
@@ -329,10 +332,11 @@ inline size_t sort_counts_bytes(int64_t S, int E) {
   return S <= kSortSmallMax ? 0 : (size_t)sort_blocks(S).blocks * E * sizeof(int32_t);
 }
 
+// Lets `kern` have up to `smem` bytes of dynamic shared memory.
 template <typename Kern>
 inline int allow_smem(Kern kern, size_t smem, PerDevice<size_t>& configured) {
   const int dev = current_device_index();
-  if (smem > 48 * 1024 && smem > configured.get(dev)) {
+  if (smem > configured.get(dev)) {
     YB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     configured.set(dev, smem);
   }
@@ -341,9 +345,11 @@ inline int allow_smem(Kern kern, size_t smem, PerDevice<size_t>& configured) {
 
 template <typename P, int WARPS>
 inline int launch_sort_small(const SortArgs& a, int64_t chunks, cudaStream_t st) {
-  static PerDevice<size_t> configured;     // per template instantiation and device
   const size_t smem = sort_small_smem(WARPS, a.S, a.E);
-  if (const int rc = allow_smem(sort_small_kernel<P, WARPS>, smem, configured)) return rc;
+  if constexpr (WARPS > 8) {                 // allowed once, for the largest call
+    static PerDevice<size_t> configured;     // per template instantiation and device
+    if (const int rc = allow_smem(sort_small_kernel<P, WARPS>, sort_small_smem(WARPS, kSortSmallMax, kSortMaxExperts), configured)) return rc;
+  }
   const int rounds = std::max(1, (int)ceil_div(a.S, 32 * WARPS));
   const int64_t work = std::max(ceil_div(a.T * chunks, WARPS), ceil_div(a.R, WARPS * kZeroRows));
   const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(work, kSMs * (32 / WARPS)));
@@ -355,13 +361,11 @@ inline int launch_sort(SortArgs a, cudaStream_t st) {
   const int64_t n = a.row_bytes / (int64_t)sizeof(P), chunks = ceil_div(n, 32);
   if (n > 0x7fffffff || a.T * chunks > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;      // 2^31 pieces of 512 bytes are 1 TB
   if (a.S <= kSortSmallMax)
-    return a.S <= 256 * kSortSmallRounds && a.E <= 256 ? launch_sort_small<P, 8>(a, chunks, st) : launch_sort_small<P, 32>(a, chunks, st);
+    return a.S <= kSortFewMax && a.E <= kSortFewExperts ? launch_sort_small<P, 8>(a, chunks, st) : launch_sort_small<P, 32>(a, chunks, st);
   const SortBlocks b = sort_blocks(a.S);
   a.parts = b.parts;
   int rc = launch_behind(sort_count_kernel, dim3(b.blocks), dim3(kSortThreads), a.E * sizeof(int32_t), st, a);
   if (rc) return rc;
-  static PerDevice<size_t> configured;
-  if ((rc = allow_smem(sort_rank_kernel, sort_rank_smem(a.E), configured))) return rc;
   if ((rc = launch_behind(sort_rank_kernel, dim3(b.blocks), dim3(kSortThreads), sort_rank_smem(a.E), st, a))) return rc;
   const int64_t copy = ceil_div(a.T * chunks, kCopyWarps), zero = ceil_div(a.R, kCopyWarps * kZeroRows);
   if (copy + zero == 0) return YAMOE_OK;
