@@ -1,0 +1,92 @@
+// Host code around launches (common.cuh) with the runtime's calls replaced: runs without a GPU.  One argument names the check.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <chrono>
+#include <condition_variable>
+#include <cstdio>
+#include <cstring>
+#include <mutex>
+#include <thread>
+
+namespace fake {
+
+std::mutex mutex;
+std::condition_variable changed;
+int largest = 0, calls = 0;           // the attribute as the runtime holds it
+bool meet = false;                    // a call waits, but not for long, until another one is over
+cudaError_t result = cudaSuccess, last = cudaSuccess;
+
+template <typename Kern>
+cudaError_t set_attribute(Kern, cudaFuncAttribute, int value) {
+  std::unique_lock<std::mutex> lock(mutex);
+  if (result != cudaSuccess) return last = result;
+  largest = value;
+  const int mine = ++calls;
+  changed.notify_all();
+  if (meet && mine == 1) changed.wait_for(lock, std::chrono::milliseconds(500), [] { return calls > 1; });
+  return cudaSuccess;
+}
+cudaError_t get_device(int* device) {
+  *device = 0;
+  return cudaSuccess;
+}
+template <typename... K, typename... A>
+cudaError_t launch(const cudaLaunchConfig_t*, void (*)(K...), A&&...) {
+  return result == cudaSuccess ? cudaSuccess : last = result;
+}
+cudaError_t memset_async(void*, int, size_t, cudaStream_t) { return result == cudaSuccess ? cudaSuccess : last = result; }
+cudaError_t get_last_error() {
+  const cudaError_t e = last;
+  last = cudaSuccess;
+  return e;
+}
+
+}  // namespace fake
+
+#define cudaFuncSetAttribute fake::set_attribute
+#define cudaGetDevice fake::get_device
+#define cudaLaunchKernelEx fake::launch
+#define cudaMemsetAsync fake::memset_async
+#define cudaGetLastError fake::get_last_error
+#include "token_sort.cuh"
+
+using namespace yb;
+
+static void kernel(int) {}
+
+#define EXPECT(x)                                        \
+  do {                                                   \
+    if (!(x)) {                                          \
+      std::printf("line %d: %s\n", __LINE__, #x);        \
+      return 1;                                          \
+    }                                                    \
+  } while (0)
+
+// Two threads ask for different sizes at the same time, whoever comes first: what the kernel may have is at least what is remembered of it.
+static int two_threads(size_t first, size_t second) {
+  static PerDevice<size_t> allowed[2];
+  PerDevice<size_t>& mine = allowed[first > second];
+  fake::largest = fake::calls = 0;
+  fake::meet = true;
+  std::thread a([&] { (void)allow_smem(kernel, first, mine); });
+  {
+    std::unique_lock<std::mutex> lock(fake::mutex);
+    fake::changed.wait_for(lock, std::chrono::seconds(5), [] { return fake::calls > 0; });
+  }
+  std::thread b([&] { (void)allow_smem(kernel, second, mine); });
+  a.join();
+  b.join();
+  EXPECT(fake::largest == 150000);
+  EXPECT(mine.get(0) == 150000);
+  // and a later call of either size finds it done
+  const int before = fake::calls;
+  EXPECT(allow_smem(kernel, 150000, mine) == 0 && allow_smem(kernel, 100000, mine) == 0 && fake::calls == before);
+  return 0;
+}
+
+int main(int, char** argv) {
+  if (!std::strcmp(argv[1], "threads")) return two_threads(150000, 100000) || two_threads(100000, 150000);
+  return 2;
+}

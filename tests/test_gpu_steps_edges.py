@@ -33,3 +33,45 @@ def test_sorts_around_48_KB_of_shared_memory(E, K, sizes):
     """What a launch may have without being allowed more counts its static arrays too.  In a process of its own, where no larger sort came before."""
     run = subprocess.run([sys.executable, "-c", SORTS % ((E, K, sizes),)], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stdout + run.stderr
+
+
+THREADS = """
+import sys
+import threading
+import torch
+sys.path.insert(0, "tests")
+import yamoe_b200
+from test_gpu_token_sort import choices, places
+sizes = [(40, 1024, 4), (900, 300, 4), (500, 1024, 8), (460, 512, 8), (8, 700, 2), (1000, 256, 4)]
+inputs = [(torch.arange(T, dtype=torch.float32)[:, None].cuda(), choices(T, K, E, seed=T)) for T, E, K in sizes]
+given = [idx.cuda() for _, idx in inputs]
+streams = [torch.cuda.Stream() for _ in sizes]
+torch.cuda.synchronize()
+start, results, wrong = threading.Barrier(len(sizes)), [None] * len(sizes), []
+
+
+def work(i):
+    try:
+        with torch.cuda.stream(streams[i]):
+            start.wait(60)
+            for _ in range(20):
+                results[i] = yamoe_b200.sort_tokens(inputs[i][0], given[i], sizes[i][1])
+    except Exception as e:
+        wrong.append(e)
+
+
+threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sizes))]
+[t.start() for t in threads]
+[t.join() for t in threads]
+torch.cuda.synchronize()
+assert not wrong, wrong
+for (T, E, K), (_, idx), (rows, row_of, offsets) in zip(sizes, inputs, results):
+    want = places(idx, E, None)
+    assert torch.equal(row_of.cpu(), want[0]) and torch.equal(offsets.cpu(), want[1]), (T, E, K)
+"""
+
+
+def test_sorts_from_several_host_threads():
+    """First calls of different sizes at the same time, each on a stream of its own."""
+    run = subprocess.run([sys.executable, "-c", THREADS], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stdout + run.stderr

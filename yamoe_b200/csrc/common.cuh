@@ -7,6 +7,7 @@
 
 #include <atomic>
 #include <cstdlib>
+#include <mutex>
 #include <utility>
 
 #include "../../include/yamoe_b200.h"
@@ -180,6 +181,20 @@ struct PerDevice {
   V get(int dev) const { return v[dev].load(std::memory_order_acquire); }
   void set(int dev, V x) { v[dev].store(x, std::memory_order_release); }
 };
+
+// Lets launches of `kern` have `smem` bytes of dynamic shared memory; `allowed` is what they may have by now.  The size belongs to the kernel and
+// not to the thread that sets it, so it only grows, under a lock: set by two threads at once, the smaller one could be the one that stays.
+template <typename Kern>
+inline cudaError_t allow_smem(Kern kern, size_t smem, PerDevice<size_t>& allowed) {
+  static std::mutex mutex;
+  const int dev = current_device_index();
+  if (smem <= allowed.get(dev)) return cudaSuccess;
+  const std::lock_guard<std::mutex> lock(mutex);
+  if (smem <= allowed.get(dev)) return cudaSuccess;
+  const cudaError_t rc = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (rc == cudaSuccess) allowed.set(dev, smem);
+  return rc;
+}
 
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl_opt(bool default_on, void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,

@@ -363,13 +363,8 @@ inline int launch_route_rows(const int64_t* router_indices, const T* routing_wei
   if (S <= kRouteClusterMaxS) {
     auto kern = route_cluster_kernel<T>;
     const size_t smem = route_cluster_smem(E);
-    static PerDevice<size_t> configured;   // per template instantiation and device
-    const int dev = current_device_index();
-    if (smem > configured.get(dev)) {
-      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-        return YAMOE_ERR_CUDA;
-      configured.set(dev, smem);
-    }
+    static PerDevice<size_t> allowed;   // per template instantiation and device
+    YB_CUDA_OK(allow_smem(kern, smem, allowed));
     const int rounds = (int)ceil_div(S, kRouteCluster * kRouteClusterThreads);
     kern<<<kRouteCluster, kRouteClusterThreads, smem, stream>>>(router_indices, routing_weights, routing_cols, (int)S, E,
                                                                 K, rounds, capacity, rt);

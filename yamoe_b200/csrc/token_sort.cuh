@@ -332,23 +332,12 @@ inline size_t sort_counts_bytes(int64_t S, int E) {
   return S <= kSortSmallMax ? 0 : (size_t)sort_blocks(S).blocks * E * sizeof(int32_t);
 }
 
-// Lets `kern` have up to `smem` bytes of dynamic shared memory.
-template <typename Kern>
-inline int allow_smem(Kern kern, size_t smem, PerDevice<size_t>& configured) {
-  const int dev = current_device_index();
-  if (smem > configured.get(dev)) {
-    YB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    configured.set(dev, smem);
-  }
-  return YAMOE_OK;
-}
-
 template <typename P, int WARPS>
 inline int launch_sort_small(const SortArgs& a, int64_t chunks, cudaStream_t st) {
   const size_t smem = sort_small_smem(WARPS, a.S, a.E);
   if constexpr (WARPS > 8) {                 // allowed once, for the largest call
-    static PerDevice<size_t> configured;     // per template instantiation and device
-    if (const int rc = allow_smem(sort_small_kernel<P, WARPS>, sort_small_smem(WARPS, kSortSmallMax, kSortMaxExperts), configured)) return rc;
+    static PerDevice<size_t> allowed;        // per template instantiation and device
+    YB_CUDA_OK(allow_smem(sort_small_kernel<P, WARPS>, sort_small_smem(WARPS, kSortSmallMax, kSortMaxExperts), allowed));
   }
   const int rounds = std::max(1, (int)ceil_div(a.S, 32 * WARPS));
   const int64_t work = std::max(ceil_div(a.T * chunks, WARPS), ceil_div(a.R, WARPS * kZeroRows));
