@@ -86,7 +86,31 @@ static int two_threads(size_t first, size_t second) {
   return 0;
 }
 
+static int memset_status() {
+  YB_CUDA_OK(cudaMemsetAsync(nullptr, 0, 4, nullptr));
+  return YAMOE_OK;
+}
+
+// A call that was refused leaves nothing for the check behind the next launch.
+static int refused() {
+  static PerDevice<size_t> allowed;
+  const auto calls = {+[] { return launch_behind(kernel, dim3(1), dim3(32), 0, nullptr, 0); },
+                      +[] { return launch_clusters(kernel, 2, true, dim3(2), dim3(32), 0, nullptr, 0); },
+                      +[] { return launch_pdl_opt(true, kernel, dim3(1), dim3(32), 0, nullptr, 0) == cudaSuccess ? (int)YAMOE_OK : (int)YAMOE_ERR_CUDA; },
+                      +[] { return launch_early(kernel, dim3(1), dim3(32), nullptr, 0) == cudaSuccess ? (int)YAMOE_OK : (int)YAMOE_ERR_CUDA; },
+                      +[] { return allow_smem(kernel, 100000, allowed) == cudaSuccess ? (int)YAMOE_OK : (int)YAMOE_ERR_CUDA; }, +[] { return memset_status(); }};
+  for (const auto& call : calls) {
+    fake::result = cudaErrorInvalidValue;
+    EXPECT(call() == YAMOE_ERR_CUDA);
+    fake::result = cudaSuccess;
+    EXPECT(fake::last == cudaSuccess);
+    EXPECT(call() == YAMOE_OK);
+  }
+  return 0;
+}
+
 int main(int, char** argv) {
+  if (!std::strcmp(argv[1], "refused")) return refused();
   if (!std::strcmp(argv[1], "threads")) return two_threads(150000, 100000) || two_threads(100000, 150000);
   return 2;
 }

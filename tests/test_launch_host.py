@@ -27,3 +27,8 @@ def check(program, name):
 def test_shared_memory_asked_for_by_two_threads(program):
     """A size that one thread has set and remembers is not made smaller by another that had asked for less."""
     check(program, "threads")
+
+
+def test_refused_calls_leave_no_error_behind(program):
+    """The runtime keeps the error of a launch, an attribute or a memset that it refused; the next launch would be taken for the one that failed."""
+    check(program, "refused")

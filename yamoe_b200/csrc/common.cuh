@@ -18,9 +18,15 @@ constexpr int kTileM = 128;          // row padding granularity of the expert-so
 constexpr float kAlpha = 1.702f;     // reference: csrc/moe.cpp:179
 constexpr float kLimit = 7.0f;       // reference: csrc/moe.cpp:175
 
+// The result of a call of the runtime, which also keeps an error for cudaGetLastError: taken back here, so that the check behind the thread's next launch
+// does not find it.
+inline cudaError_t taken(cudaError_t e) {
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e;
+}
 #define YB_CUDA_OK(expr)                                  \
   do {                                                    \
-    cudaError_t _e = (expr);                              \
+    const cudaError_t _e = yb::taken(expr);               \
     if (_e != cudaSuccess) return YAMOE_ERR_CUDA;         \
   } while (0)
 
@@ -191,7 +197,7 @@ inline cudaError_t allow_smem(Kern kern, size_t smem, PerDevice<size_t>& allowed
   if (smem <= allowed.get(dev)) return cudaSuccess;
   const std::lock_guard<std::mutex> lock(mutex);
   if (smem <= allowed.get(dev)) return cudaSuccess;
-  const cudaError_t rc = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const cudaError_t rc = taken(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   if (rc == cudaSuccess) allowed.set(dev, smem);
   return rc;
 }
@@ -209,7 +215,7 @@ inline cudaError_t launch_pdl_opt(bool default_on, void (*kern)(KArgs...), dim3 
   attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled(default_on) ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+  return taken(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...));
 }
 
 // The same for kernels without dynamic shared memory that always start early.
@@ -242,7 +248,7 @@ inline int launch_clusters(void (*kern)(KArgs...), int cluster, bool early, dim3
   attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled(early) ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t rc = cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+  const cudaError_t rc = taken(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...));
   return rc == cudaSuccess && cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
 }
 

@@ -724,7 +724,7 @@ template <class Epi, typename... KArgs>
 inline bool fp8_configure(void (*kern)(KArgs...), PerDevice<int>& done) {
   const int dev = current_device_index();
   if (done.get(dev)) return true;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8MostSmem<Epi>) != cudaSuccess) return false;
+  if (taken(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8MostSmem<Epi>)) != cudaSuccess) return false;
   done.set(dev, 1);
   return true;
 }
@@ -809,7 +809,7 @@ inline int launch_fp8_gemm(const Fp8Operand& a, const Fp8Operand& b, const Fp8Ou
   attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled(true) && !split ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmOut, p, epi) != cudaSuccess) return YAMOE_ERR_CUDA;
+  if (taken(cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmOut, p, epi)) != cudaSuccess) return YAMOE_ERR_CUDA;
   return cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
 }
 

@@ -632,7 +632,7 @@ inline int int8_resident(int cluster, int smem) {
   const int dev = current_device_index();
   int n = known[cluster].get(dev);
   if (n > 0) return n;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
+  if (taken(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(umma_sm_count() / cluster * cluster));
   cfg.blockDim = dim3(kInt8Threads);

@@ -911,7 +911,7 @@ inline int launch_moe_layer(const LayerArgs& a, const CUtensorMap& gu, const CUt
   static PerDevice<int> configured;
   const int dev = current_device_index();
   if (!configured.get(dev)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLayerSmem) != cudaSuccess) return YAMOE_ERR_CUDA;
+    YB_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLayerSmem));
     configured.set(dev, 1);
   }
   layer_router_kernel<FP8><<<(unsigned)(a.E + a.T), kRouterThreads, 0, st>>>(a);
@@ -926,7 +926,7 @@ inline int launch_moe_layer(const LayerArgs& a, const CUtensorMap& gu, const CUt
   attr[0].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, gu, dn, a) != cudaSuccess) return YAMOE_ERR_CUDA;
+  YB_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, gu, dn, a));
   return cudaGetLastError() == cudaSuccess ? YAMOE_OK : YAMOE_ERR_CUDA;
 }
 

@@ -616,7 +616,7 @@ inline int launch_umma_gemm_bn(const GemmArgs& g, const Epi& epi, int64_t max_ro
   static PerDevice<int> attr_done;   // per template instantiation and device
   const int dev = current_device_index();
   if (!attr_done.get(dev)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kTotal) != cudaSuccess)
+    if (taken(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::kTotal)) != cudaSuccess)
       return YAMOE_ERR_CUDA;
     attr_done.set(dev, 1);
   }

@@ -715,7 +715,7 @@ inline int resident_pairs(void (*kern)(KArgs...), int threads, int smem, PerDevi
   const int dev = current_device_index();
   int n = known.get(dev);
   if (n > 0) return n;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return 0;
+  if (taken(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(umma_sm_count() & ~1);
   cfg.blockDim = dim3(threads);

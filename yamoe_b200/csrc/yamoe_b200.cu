@@ -906,8 +906,8 @@ static int ep_call_prologue(const yamoe_ep_ctx_t& c, const EpCallPlan& p, const 
     static PerDevice<int> carveout_set;    // per template instantiation and device
     const int dev = current_device_index();
     if (!carveout_set.get(dev)) {
-      cudaFuncSetAttribute(ep_dispatch_fused_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                           (int)cudaSharedmemCarveoutMaxShared);
+      (void)taken(cudaFuncSetAttribute(ep_dispatch_fused_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                       (int)cudaSharedmemCarveoutMaxShared));
       carveout_set.set(dev, 1);
     }
   }
@@ -1547,8 +1547,8 @@ int yamoe_b200_prof_read(unsigned long long* out16) {
   unsigned long long zero[16] = {};
   zero[8] = zero[10] = ~0ull;          // slots that hold a minimum
   if (cudaDeviceSynchronize() != cudaSuccess) return YAMOE_ERR_CUDA;
-  if (cudaMemcpyFromSymbol(out16, g_prof, sizeof(zero)) != cudaSuccess) return YAMOE_ERR_CUDA;
-  if (cudaMemcpyToSymbol(g_prof, zero, sizeof(zero)) != cudaSuccess) return YAMOE_ERR_CUDA;
+  YB_CUDA_OK(cudaMemcpyFromSymbol(out16, g_prof, sizeof(zero)));
+  YB_CUDA_OK(cudaMemcpyToSymbol(g_prof, zero, sizeof(zero)));
   return YAMOE_OK;
 }
 #endif
