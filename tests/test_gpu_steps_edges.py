@@ -75,3 +75,30 @@ def test_sorts_from_several_host_threads():
     """First calls of different sizes at the same time, each on a stream of its own."""
     run = subprocess.run([sys.executable, "-c", THREADS], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stdout + run.stderr
+
+
+# ---- 8-bit integers
+def quantised_by_entry(x, batch, M, K, transpose):
+    """yamoe_b200_int8_quantize itself: its status, codes and scales of `batch` matrices [M, K]."""
+    from yamoe_b200 import _lib
+    rows, cols = (K, M) if transpose else (M, K)
+    ld = max(16, -(-cols // 16) * 16)
+    q = torch.full((batch, rows, ld), 77, dtype=torch.int8, device="cuda")
+    s = torch.full((batch, rows), -1.0, device="cuda")
+    out = _lib.Int8Matrix(q=q.data_ptr(), scale=s.data_ptr(), ld=ld, q_batch=rows * ld, scale_row=1, scale_batch=rows)
+    import ctypes
+    status = _lib.lib().yamoe_b200_int8_quantize(x.data_ptr() or None, ctypes.byref(out), batch, M, K, int(transpose), 1 if x.dtype == BF16 else 0,
+                                                 torch.cuda.current_stream().cuda_stream)
+    return status, q, s
+
+
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("batch,rows", [(1, 5), (3, 200)])
+def test_rows_without_values_through_the_C_entry(batch, rows, dtype, transpose):
+    """Rows of no values have the scale of a row of zeros and no codes; those of x^T are the columns of an x without rows."""
+    M, K = (0, rows) if transpose else (rows, 0)
+    status, q, s = quantised_by_entry(torch.empty(batch, M, K, dtype=dtype, device="cuda"), batch, M, K, transpose)
+    assert status == 0
+    assert bool((s == 2.0 ** -100 / 127).all()) and bool((q == 77).all())
+    assert torch.ones(4, device="cuda").sum().item() == 4          # nothing is left for the next call to report

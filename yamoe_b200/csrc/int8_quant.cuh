@@ -211,7 +211,7 @@ inline int launch_int8_quantize(const T* x, const Int8Out& d, int64_t B, int64_t
     const int64_t strips = ceil_div(K, 64);
     if (strips * kInt8MaxParts > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
     auto kern = vec ? int8_columns_quantize_kernel<T, true> : int8_columns_quantize_kernel<T, false>;
-    const int parts = (int)std::min<int64_t>(kInt8MaxParts, ceil_div(M, 256));
+    const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(kInt8MaxParts, ceil_div(M, 256)));       // (x without rows: scales alone)
     return launch_clusters(kern, parts, true, dim3((unsigned)(strips * parts), (unsigned)B), dim3(256), 0, st, x, d, M, K, parts);
   }
   int log_wpr = 0;
