@@ -102,3 +102,51 @@ def test_rows_without_values_through_the_C_entry(batch, rows, dtype, transpose):
     assert status == 0
     assert bool((s == 2.0 ** -100 / 127).all()) and bool((q == 77).all())
     assert torch.ones(4, device="cuda").sum().item() == 4          # nothing is left for the next call to report
+
+
+# ---- derivatives that the integer operators do not have
+def integer_calls():
+    import yamoe_b200
+    a, b = torch.ones(4, 32, dtype=torch.int8, device="cuda"), torch.ones(5, 32, dtype=torch.int8, device="cuda")
+    sa, sb = torch.ones(4, device="cuda"), torch.ones(5, device="cuda")
+    x = torch.randn(4, 32, generator=torch.Generator().manual_seed(0)).cuda()
+    return {"quantize": (x, lambda t: yamoe_b200.quantize_int8(t)[1]), "quantize_transposed": (x, lambda t: yamoe_b200.quantize_int8(t, True)[1]),
+            "a_scale": (sa, lambda t: yamoe_b200.int8_mm(a, t, b, sb, F32)), "b_scale": (sb, lambda t: yamoe_b200.int8_mm(a, sa, b, t, F32)),
+            "chain": (x, lambda t: yamoe_b200.int8_mm(*yamoe_b200.quantize_int8(t), b, sb))}
+
+
+CALLS = ["quantize", "quantize_transposed", "a_scale", "b_scale", "chain"]
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_integers_have_no_gradient(name):
+    """The result is that of a tensor that wants none; a backward pass that reaches the operator raises, and one that does not goes through."""
+    leaf, call = integer_calls()[name]
+    want = call(leaf)
+    assert not want.requires_grad
+    leaf = leaf.clone().requires_grad_(True)
+    out = call(leaf)
+    assert torch.equal(out, want)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        out.float().sum().backward()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        torch.autograd.grad((call(leaf).float().sum() + leaf.sum()), leaf)
+    assert leaf.grad is None
+    (g,) = torch.autograd.grad(call(leaf).detach().float().sum() + leaf.sum(), leaf)
+    assert torch.equal(g, torch.ones_like(leaf))
+    with torch.no_grad():
+        assert not call(leaf).requires_grad
+    with torch.inference_mode():
+        assert torch.equal(call(leaf), want)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_integers_refuse_forward_mode(name):
+    import torch.autograd.forward_ad as fwAD
+    leaf, call = integer_calls()[name]
+    with fwAD.dual_level():
+        for t in (fwAD.make_dual(leaf, torch.ones_like(leaf)), fwAD.make_dual(leaf.clone().requires_grad_(True), torch.ones_like(leaf))):
+            with pytest.raises(RuntimeError, match="forward"):
+                call(t)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward"):
+                call(t)

@@ -58,6 +58,15 @@ inline void differentiate_no_further(const char* op, std::initializer_list<at::T
     if (t->defined()) torch::autograd::create_gradient_edge(*t, node);
 }
 
+// The result of an operator without a gradient, where one of `from` wants one: a node that raises when it is differentiated, on the way to them.  (Torch's
+// default would be a warning then, and no gradient.)
+inline void no_gradient(const char* op, std::initializer_list<at::Tensor> from, at::Tensor& result) {
+  torch::autograd::edge_list on;
+  for (const at::Tensor& t : from)
+    for (const torch::autograd::Edge& e : torch::autograd::collect_next_edges(t)) on.push_back(e);
+  torch::autograd::create_gradient_edge(result, std::make_shared<torch::autograd::Error>(std::string(op) + " has no gradient", std::move(on)));
+}
+
 // Forward mode: a tangent that nobody takes up would count as zero.
 inline void check_no_tangent(const char* op, const at::Tensor& t) {
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;

@@ -1,5 +1,5 @@
 // Torch binding of the expert layer's steps: `sort_tokens`, `combine_tokens`, `quantize_int8`, `int8_mm` and `glu_fp8` over the C ABI, with
-// the gradients of the three that have one.
+// the gradients of the three that have one and a refusal of those of the integers.
 #include <ATen/cuda/EmptyTensor.h>
 
 #include <optional>
@@ -262,6 +262,17 @@ std::tuple<at::Tensor, at::Tensor> quantize_int8_cuda(const at::Tensor& x, bool 
   return {m.q, m.scale};
 }
 
+std::tuple<at::Tensor, at::Tensor> quantize_int8_autograd(const at::Tensor& x, bool transpose) {
+  check_no_tangent("quantize_int8", x);
+  std::tuple<at::Tensor, at::Tensor> codes;
+  {
+    const at::AutoDispatchBelowAutograd below;
+    codes = quantize_int8_cuda(x, transpose);
+  }
+  if (wants_grad({x})) no_gradient("quantize_int8", {x}, std::get<1>(codes));
+  return codes;
+}
+
 // Checks a pair of codes and scales and brings codes whose rows the kernels cannot address into a layout of their own.
 Integers operand(const char* name, const at::Tensor& q, const at::Tensor& scale, int64_t dim) {
   TORCH_CHECK(q.scalar_type() == at::kChar, "int8_mm: ", name, " must be int8, got ", q.scalar_type());
@@ -311,6 +322,19 @@ at::Tensor int8_mm_cuda(const at::Tensor& a, const at::Tensor& a_scale, const at
                            out_dtype == at::kFloat ? YAMOE_F32 : YAMOE_BF16, ws.data_ptr(), (size_t)ws.numel(), current_stream()),
         "int8_mm");
   check_device_status(ws, current_stream(), "int8_mm");
+  return out;
+}
+
+at::Tensor int8_mm_autograd(const at::Tensor& a, const at::Tensor& a_scale, const at::Tensor& b, const at::Tensor& b_scale,
+                            at::ScalarType out_dtype, const std::optional<at::Tensor>& offsets) {
+  check_no_tangent("int8_mm", a_scale);
+  check_no_tangent("int8_mm", b_scale);
+  at::Tensor out;
+  {
+    const at::AutoDispatchBelowAutograd below;
+    out = int8_mm_cuda(a, a_scale, b, b_scale, out_dtype, offsets);
+  }
+  if (wants_grad({a_scale, b_scale})) no_gradient("int8_mm", {a_scale, b_scale}, out);
   return out;
 }
 
@@ -405,6 +429,8 @@ TORCH_LIBRARY_FRAGMENT(yamoe_b200, m) {
 TORCH_LIBRARY_IMPL(yamoe_b200, AutogradCUDA, m) {
   m.impl("sort_tokens", &sort_tokens_autograd);
   m.impl("combine_tokens", &combine_tokens_autograd);
+  m.impl("quantize_int8", &quantize_int8_autograd);
+  m.impl("int8_mm", &int8_mm_autograd);
   m.impl("glu_fp8", &glu_fp8_autograd);
 }
 
