@@ -104,6 +104,26 @@ def test_rows_without_values_through_the_C_entry(batch, rows, dtype, transpose):
     assert torch.ones(4, device="cuda").sum().item() == 4          # nothing is left for the next call to report
 
 
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("B", [65535, 65536, 140001])
+def test_more_matrices_than_a_grid_has_rows(B, transpose):
+    import yamoe_b200
+    x = torch.randn(B, 2, 3, generator=torch.Generator().manual_seed(B)).cuda()
+    x[-1, 0, 0], x[0, 1, 1] = 40.0, float("inf")
+    q, s = yamoe_b200.quantize_int8(x, transpose)
+    flat = (x.transpose(1, 2) if transpose else x).reshape(-1, 2 if transpose else 3)
+    want_q, want_s = yamoe_b200.quantize_int8(flat)
+    assert torch.equal(q.reshape(flat.shape), want_q)
+    assert torch.equal(s.reshape(-1).nan_to_num(-1.0), want_s.nan_to_num(-1.0)) and bool(s.isnan().any())
+
+
+def test_numbers_of_matrices_that_are_refused():
+    import ctypes
+    from yamoe_b200 import _lib
+    out = ctypes.byref(_lib.Int8Matrix(q=4096, scale=4096, ld=16, q_batch=32, scale_row=1, scale_batch=2))
+    assert _lib.lib().yamoe_b200_int8_quantize(4096, out, 1 << 31, 2, 3, 0, 1, None) == -5
+
+
 # ---- derivatives that the integer operators do not have
 def integer_calls():
     import yamoe_b200

@@ -203,9 +203,16 @@ int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, 
   }
 }
 
+constexpr int64_t kMostGridRows = 65535;
 template <typename T>
-inline int launch_int8_quantize(const T* x, const Int8Out& d, int64_t B, int64_t M, int64_t K, bool transpose, cudaStream_t st) {
-  if (B > 65535) return YAMOE_ERR_UNSUPPORTED;
+inline int launch_int8_quantize(const T* x, Int8Out d, int64_t B, int64_t M, int64_t K, bool transpose, cudaStream_t st) {
+  for (; B > kMostGridRows; B -= kMostGridRows) {      // a matrix is a row of the grid
+    const int rc = launch_int8_quantize(x, d, kMostGridRows, M, K, transpose, st);
+    if (rc) return rc;
+    x += kMostGridRows * M * K;
+    d.q += kMostGridRows * d.q_batch;
+    d.scale += kMostGridRows * d.scale_batch;
+  }
   const bool vec = K % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   if (transpose) {
     const int64_t strips = ceil_div(K, 64);

@@ -179,7 +179,7 @@ int yamoe_b200_int8_quantize(const void* x, const yamoe_int8_matrix_t* out, int6
   if (batch == 0 || rows == 0) return YAMOE_OK;
   if (cols > 0 && (x == nullptr || !at_boundary(x, size_of(dtype)))) return YAMOE_ERR_BAD_ARG;
   if (!int8_matrix_ok(out, batch, cols)) return YAMOE_ERR_BAD_ARG;
-  if (M > kMaxRows || K > kMaxRows) return YAMOE_ERR_UNSUPPORTED;
+  if (batch > kMaxRows || M > kMaxRows || K > kMaxRows) return YAMOE_ERR_UNSUPPORTED;
   const Int8Out d{reinterpret_cast<uint8_t*>(out->q), out->scale, out->ld, out->q_batch, out->scale_row, out->scale_batch};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return dtype == YAMOE_BF16 ? launch_int8_quantize(reinterpret_cast<const __nv_bfloat16*>(x), d, batch, M, K, transpose != 0, st)
