@@ -124,6 +124,22 @@ def test_numbers_of_matrices_that_are_refused():
     assert _lib.lib().yamoe_b200_int8_quantize(4096, out, 1 << 31, 2, 3, 0, 1, None) == -5
 
 
+@pytest.mark.parametrize("M", [6, 200])
+@pytest.mark.parametrize("table", [[0, 4, 2 ** 40], [-(2 ** 35), 3, 2 ** 31], [0, 2 ** 32, 2 ** 32 + 5], [2 ** 33] * 3, [1, 3, 5]])
+def test_offsets_of_64_bits(M, table):
+    """They are kept within the rows as the numbers that they are."""
+    import yamoe_b200
+    gen = torch.Generator().manual_seed(1)
+    a, b = torch.randint(-127, 128, (M, 64), generator=gen), torch.randint(-127, 128, (2, 40, 64), generator=gen)
+    off = [min(max(o, 0), M) for o in table]
+    want = torch.zeros(M, 40)
+    for e in range(2):
+        want[off[e] : off[e + 1]] = (a[off[e] : off[e + 1]] @ b[e].T).float()
+    for given in (torch.tensor(table), torch.tensor(table).repeat_interleave(2)[::2]):
+        got = yamoe_b200.int8_mm(a.to(torch.int8).cuda(), torch.ones(M, device="cuda"), b.to(torch.int8).cuda(), torch.ones(2, 40, device="cuda"), F32, given.cuda())
+        assert torch.equal(got.cpu(), want)
+
+
 # ---- derivatives that the integer operators do not have
 def integer_calls():
     import yamoe_b200

@@ -309,7 +309,8 @@ at::Tensor int8_mm_cuda(const at::Tensor& a, const at::Tensor& a_scale, const at
     TORCH_CHECK(B <= 1024, "int8_mm: at most 1024 experts, got ", B);
     TORCH_CHECK(offsets->dim() == 1 && offsets->size(0) == B + 1 && (offsets->scalar_type() == at::kInt || offsets->scalar_type() == at::kLong),
                 "int8_mm: offsets must be int32 [E + 1]");
-    first = offsets->to(at::kInt).contiguous();
+    // 64 bits are kept within the rows before they become 32, as the kernels keep 32
+    first = (offsets->scalar_type() == at::kInt ? *offsets : offsets->clamp(0, M).to(at::kInt)).contiguous();
   } else {
     TORCH_CHECK(a.dim() == 2 || a.size(0) == B, "int8_mm: a and b must hold the same number of matrices");
   }
