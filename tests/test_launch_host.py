@@ -32,3 +32,9 @@ def test_shared_memory_asked_for_by_two_threads(program):
 def test_refused_calls_leave_no_error_behind(program):
     """The runtime keeps the error of a launch, an attribute or a memset that it refused; the next launch would be taken for the one that failed."""
     check(program, "refused")
+
+
+@pytest.mark.parametrize("name", ["tiles", "parts", "ring"])
+def test_arithmetic_that_kernels_and_launchers_share(program, name):
+    """The functions themselves, over all sizes that they may meet."""
+    check(program, name)

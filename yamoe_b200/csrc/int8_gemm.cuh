@@ -48,6 +48,8 @@ constexpr int int8_exchange_slots(int splits) { return (8 + splits - 1) / splits
 static_assert(int8_exchange_slots(2) * kInt8ChunkBytes <= kInt8Ring && int8_exchange_slots(3) * kInt8ChunkBytes <= kInt8Ring &&
               int8_exchange_slots(4) * kInt8ChunkBytes <= kInt8Ring, "the exchange takes the ring's place");
 constexpr int kInt8MaxExperts = 1024;
+// Rows of a tile where `rows` are cut into `tiles`, a multiple of 32; the last tile has the rest.
+__host__ __device__ constexpr int int8_tile_rows(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 31) & ~31; }
 
 template <typename T>
 struct Int8Params {
@@ -249,7 +251,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     }
     // the row tile varies fastest, so that the pairs running at a time share weights in L2
     const int nt = local / tiles;
-    const int step = ((rows + tiles - 1) / tiles + 31) & ~31;
+    const int step = int8_tile_rows(rows, tiles);
     m0 = nt * 256;
     row0 = first + (local - nt * tiles) * step;
     row_end = min(first + rows, row0 + step);

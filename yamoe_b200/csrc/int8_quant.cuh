@@ -106,6 +106,8 @@ int8_rows_quantize_kernel(const T* x, const Int8Out d, int64_t M, int K, int log
 // Codes are parked as [64 columns][256 rows] with the 8-byte units of a column permuted (unit rg lies at rg ^ 4 cg), so that the eight
 // columns that a warp writes at a time fall on different banks.
 constexpr int kInt8MaxParts = 4;
+inline int int8_parts(int64_t M) { return (int)std::max<int64_t>(1, std::min<int64_t>(kInt8MaxParts, ceil_div(M, 256))); }      // (x without rows: scales alone)
+__host__ __device__ constexpr int64_t int8_part_rows(int64_t M, int parts) { return ((M + parts - 1) / parts + 15) & ~(int64_t)15; }
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256, VEC && sizeof(T) == 2 ? 4 : 2)
@@ -118,7 +120,7 @@ int8_columns_quantize_kernel(const T* x, const Int8Out d, int64_t M, int64_t K, 
   __shared__ uint32_t s_keep[64];
   const int cg = threadIdx.x & 7, rg = threadIdx.x >> 3, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const unsigned part = cluster_ctarank();
-  const int64_t rows = ((M + parts - 1) / parts + 15) & ~(int64_t)15, first = part * rows, end = min(M, first + rows);
+  const int64_t rows = int8_part_rows(M, parts), first = part * rows, end = min(M, first + rows);
   const int64_t held = first + (rows - 1) / 256 * 256;         // rows from here on stay in registers
   const int64_t c0 = (int64_t)(blockIdx.x / parts) * 64, k = c0 + 8 * cg;
   const int columns = (int)max((int64_t)0, min((int64_t)8, K - k));
@@ -218,7 +220,7 @@ inline int launch_int8_quantize(const T* x, Int8Out d, int64_t B, int64_t M, int
     const int64_t strips = ceil_div(K, 64);
     if (strips * kInt8MaxParts > 0x7fffffff) return YAMOE_ERR_UNSUPPORTED;
     auto kern = vec ? int8_columns_quantize_kernel<T, true> : int8_columns_quantize_kernel<T, false>;
-    const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(kInt8MaxParts, ceil_div(M, 256)));       // (x without rows: scales alone)
+    const int parts = int8_parts(M);
     return launch_clusters(kern, parts, true, dim3((unsigned)(strips * parts), (unsigned)B), dim3(256), 0, st, x, d, M, K, parts);
   }
   int log_wpr = 0;
