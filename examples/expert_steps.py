@@ -47,6 +47,7 @@ def main(argv=None):
     x, up = normal(T, H), normal(T, H)
     best, indices = torch.topk(torch.randn(T, E, device="cuda", generator=gen), K, dim=-1)
     weights = torch.softmax(best, dim=-1).bfloat16()
+    # (`experts` takes biases, the products here have none)
     biases = torch.zeros(E, 2 * H, device="cuda").bfloat16(), torch.zeros(E, H, device="cuda").bfloat16()
 
     # (`experts` takes [T, K] weights as dense where K is the number of experts)

@@ -417,7 +417,8 @@ int yamoe_b200_combine_tokens(const void *rows, int64_t n_rows, const int32_t *r
 
 /* Its gradients; either output may be NULL (d_weights: has to be without weights).
  *   d_rows[r,:] = sum of w[p] d_out[t(p),:] over the assignments p with row_of[p] = r in the order of p, zero without any.  The rows
- *   of yamoe_b200_sort_tokens have one at most; one that more than 32 name costs a pass over row_of.
+ *   of yamoe_b200_sort_tokens have one at most; one that more than 32 name costs a pass over row_of, and one that more than 128 name
+ *   up to one more for every 32 pieces of the row (16 bytes each; 4 or one value where rows are no multiples of that), one after the other.
  *   d_weights   like weights: <d_out[t], rows[row_of[t*K+k]]>, 0 where there is no row; with router_indices the sum over the slots of
  *   a column, 0 for those of none.  K <= 1024. */
 size_t yamoe_b200_combine_tokens_backward_workspace_bytes(int64_t n_rows, int64_t T, int K);
@@ -444,7 +445,8 @@ int yamoe_b200_int8_quantize(const void *x, const yamoe_int8_matrix_t *out, int6
 
 /* out[b] [M,N] = A[b] [M,K] @ B[b] [N,K]^T of quantised matrices: the sums are exact (K < 2^17), as fp32 times A's scale, times B's, rounded
  * once to out_dtype.  With offsets (int32 [batch+1], ascending) A is ONE matrix [M,K], rows offsets[e] .. offsets[e+1]-1 of which
- * are multiplied by B[e]; the other rows of out [M,N] are zero.  batch <= 1024 then.  M, N < 2^30.  The workspace holds the status word. */
+ * are multiplied by B[e]; the other rows of out [M,N] are zero.  Offsets are kept within the rows; where they do not ascend, which expert a row goes
+ * to is not defined, nor that it is written.  batch <= 1024 then.  M, N < 2^30.  The workspace holds the status word. */
 size_t yamoe_b200_int8_mm_workspace_bytes(int64_t batch, int64_t M, int64_t N, int64_t K);
 int yamoe_b200_int8_mm(const yamoe_int8_matrix_t *a, const yamoe_int8_matrix_t *b, const int32_t *offsets, void *out,
                        int64_t batch, int64_t M, int64_t N, int64_t K, int out_dtype, void *workspace,
@@ -452,7 +454,8 @@ int yamoe_b200_int8_mm(const yamoe_int8_matrix_t *a, const yamoe_int8_matrix_t *
 
 /* The clamped GLU of the expert forward on pre-activations [M, 2N] (even columns gate, odd ones up): out [M, N].  With `codes` also the
  * checkpoint of its backward pass: e4m3 codes of the pre-activations in groups of 1 x 128 (yamoe_b200_fp8_quantize has the definition),
- * rows of `ld` bytes, 16-byte aligned, ld a multiple of 16 and at least 2N; `scales` fp32 [M, ceil(2N / 128)].  2N < 2^31.
+ * rows of `ld` bytes, 16-byte aligned, ld a multiple of 16 and at least 2N; `scales` fp32 [M, ceil(2N / 128)].  2N < 2^31 and
+ * M * ceil(2N / 512) < 2^31.
  * The backward pass is the GLU's derivative at the values of the codes, times d_out [M, N]. */
 int yamoe_b200_glu_forward(const void *pre, void *out, void *codes, float *scales, int64_t ld, int64_t M, int64_t N,
                            int dtype, void *stream);

@@ -12,7 +12,8 @@
 // begin, so nothing is padded in memory, and few rows cost few clocks.  A k-block is 128 bytes wide, one swizzle row, up to 32 KB per CTA;
 // two accumulators, so that a tile is scaled and stored while the next is multiplied.  Scales are met in the epilogue alone, unlike the
 // e4m3 products with a scale per 128 (fp8_gemm.cuh), whose sums leave TMEM after every block.  8192 x 5760 x 2880: 88 us on a cool GPU, 3.1
-// PFLOP/s, 111 for seconds on end under the power cap; 2048 rows of 32 experts, 5760 x 2880 each: 98 us, 5.7 TB/s.
+// PFLOP/s, 111 for seconds on end under the power cap; 2048 rows of 32 experts, 5760 x 2880 each: 98 us alone behind a flushed L2, 5.7 TB/s, 93 among its
+// like; 32 matrices of 64 rows 90 and 87 us, of 512 rows 189 and 211 (power).
 // Few tiles: a cluster of up to four pairs shares a tile's k-blocks; the chunks of 32 rows are dealt out among the pairs, each of which gets
 // the others' sums of its chunks through distributed shared memory.
 //
@@ -28,9 +29,9 @@
 namespace yb {
 
 // A k-block: this CTA's 128 rows of weights and half of the tile's rows of tokens in boxes of 32, 128 bytes each.  Blocks come, are multiplied and
-// are given back in groups: two at a time, which spares the warps every other wait (64 x 5760 x 2880: one at a time 9.3 us, two 8.3; 2048 rows of
-// 32 experts 109, 107), but for the widest tiles of products that are not grouped, whose instructions take longer than the waits and of which
-// the ring holds three groups of two (8192 x 5760 x 2880: 88, 93).
+// are given back in groups: two at a time, which spares the warps every other wait (64 x 5760 x 2880: one at a time 9.3 us, two 8.3; the widest tiles of
+// 2048 rows of 32 experts, which wait for HBM: 92, 93), but for the widest tiles of products that are not grouped, whose instructions take longer than
+// the waits and of which the ring holds three groups of two (8192 x 5760 x 2880, alone: 94, 98).
 constexpr int int8_block_bytes(int width) { return 128 * 128 + (width + 63) / 64 * 4096; }
 constexpr int int8_depth(int width, bool grouped) { return width > 192 && !grouped ? 1 : 2; }
 constexpr int kInt8Ring = 10 * int8_block_bytes(64), kInt8MaxGroups = 6;
@@ -690,8 +691,9 @@ inline int launch_int8_pair(const Int8Operand& X, const Int8Operand& W, Int8Para
   const int pairs = int8_resident<kern>(2, most);
   if (pairs <= 0) return YAMOE_ERR_CUDA;
   if constexpr (GROUPED) {
-    // Narrow tiles, and with them more k-blocks on their way, where experts have few rows (mean rows per expert, us with tiles of 64 / 128 / 256: 0.5
-    // 5760 x 2880 93 / 96 / 101; 16 84 / 82 / 87; 64 112 / 95 / 93; 128 161 / 121 / 109).
+    // Narrow tiles, and with them more k-blocks on their way, where experts have few rows (5760 x 2880 each of 32 experts, rows dealt out at random, among
+    // launches of its like, mean rows per expert and us with tiles of 64 / 128 / 256: 0.5 39 / 40 / 44; 16 84 / 83 / 89; 64 92 / 87 / 93; 128
+    // 147 / 110 / 101: the border between the wider two lies between 64 and 128 rows since k-blocks come in groups, higher than it is set).
     p.width = p.M <= 8 * (int64_t)p.B ? 64 : p.M <= 32 * (int64_t)p.B ? 128 : 256;
     p.splits = 1;
     p.depth = int8_depth(p.width, GROUPED);
